@@ -17,16 +17,15 @@ import threading
 
 from . import _lib
 from ._lib import B200GemmError, strerror
+from .ffn import ACTIVATIONS as _ACTIVATIONS
+from .ffn import FfnOps
 
-__all__ = ["Gemm", "gemm", "run_kernel", "schedule", "B200GemmError", "strerror", "version"]
+__all__ = ["Gemm", "gemm", "gated", "gated_backward", "w4_quantize", "w4_dequantize", "w4_nt", "w4_gated",
+           "run_kernel", "schedule", "B200GemmError", "strerror", "version"]
 
 
 def version() -> int:
     return _lib.load().b200gemm_version()
-
-
-_ACTIVATIONS = {"none": _lib.ACT_NONE, "relu": _lib.ACT_RELU, "gelu": _lib.ACT_GELU,
-                "gelu_tanh": _lib.ACT_GELU_TANH, "silu": _lib.ACT_SILU}
 
 
 def _ptr(t) -> int:
@@ -43,7 +42,7 @@ def _stream_ptr(stream) -> int:
     return int(stream.cuda_stream)
 
 
-class Gemm:
+class Gemm(FfnOps):
     """A b200gemm handle bound to one CUDA device."""
 
     def __init__(self, device: int = 0):
@@ -264,6 +263,44 @@ def _handle_for(device: int) -> Gemm:
 def gemm(A, B, out=None, stream=None):
     """out = A @ B^T (bf16, fp32 accumulate) on A's device."""
     return _handle_for(A.device.index if A.device.index is not None else 0).bf16_nt(A, B, out, stream)
+
+
+# The feed-forward operators (see the methods of `Gemm` of the same names) on
+# the device of their first argument.
+def _on_device_of(t) -> Gemm:
+    if not t.is_cuda:
+        raise ValueError("expected a CUDA tensor")
+    return _handle_for(t.get_device())
+
+
+def gated(X, Wg, Wu, activation: str = "silu", save: bool = False, out=None, stream=None):
+    """H = act(X Wg^T) * (X Wu^T); with `save` (H, G, U).  See Gemm.gated."""
+    return _on_device_of(X).gated(X, Wg, Wu, activation, save, out, stream=stream)
+
+
+def gated_backward(dH, X, Wg, Wu, G, U, activation: str = "silu", stream=None):
+    """(dX, dWg, dWu) of `gated`.  See Gemm.gated_backward."""
+    return _on_device_of(dH).gated_backward(dH, X, Wg, Wu, G, U, activation, stream=stream)
+
+
+def w4_quantize(W, group: int = 128, stream=None):
+    """bf16 weights -> (codes, scales) in 4 bits.  See Gemm.w4_quantize."""
+    return _on_device_of(W).w4_quantize(W, group, stream)
+
+
+def w4_dequantize(codes, scales, out=None, stream=None):
+    """The bf16 weights that 4-bit codes stand for.  See Gemm.w4_dequantize."""
+    return _on_device_of(codes).w4_dequantize(codes, scales, out, stream)
+
+
+def w4_nt(A, codes, scales, out=None, out_dtype=None, stream=None):
+    """A W^T with 4-bit weights.  See Gemm.w4_nt."""
+    return _on_device_of(A).w4_nt(A, codes, scales, out, out_dtype, stream)
+
+
+def w4_gated(X, gate_codes, gate_scales, up_codes, up_scales, activation: str = "silu", out=None, stream=None):
+    """act(X Wg^T) * (X Wu^T) with 4-bit weights.  See Gemm.w4_gated."""
+    return _on_device_of(X).w4_gated(X, gate_codes, gate_scales, up_codes, up_scales, activation, out, stream)
 
 
 def run_kernel(kernel_num: int, M: int, N: int, K: int, A, B, C) -> None:

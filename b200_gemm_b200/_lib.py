@@ -28,6 +28,7 @@ OUT_BF16, OUT_F32, OUT_E4M3 = 0, 1, 2
 PDL_OFF, PDL_ON, PDL_WEIGHTS_EARLY = 0, 1, 2
 
 _c_int, _c_uint, _c_ull, _vp = ctypes.c_int, ctypes.c_uint, ctypes.c_ulonglong, ctypes.c_void_p
+_c_ll = ctypes.c_longlong
 
 
 class Epilogue(ctypes.Structure):
@@ -75,6 +76,18 @@ SIGNATURES = {
     "b200gemm_set_schedule": (_c_int, [_vp, _c_int, _c_int]),
     "b200gemm_schedule_host": (_c_int, [_c_uint, _c_uint, _c_int, _c_int, ctypes.POINTER(_c_uint)]),
     "b200gemm_bf16_nt_noalloc": (_c_int, [_c_int, _c_int, _c_int, _vp, _vp, _vp, _c_int, _vp]),
+    "b200gemm_bf16_gated": (_c_int, [_vp, _c_int, _c_int, _c_int, _vp, _c_ll, _vp, _vp, _c_ll, _c_int,
+                                     _vp, _c_ll, _vp, _vp, _c_ll, _vp]),
+    "b200gemm_gated_backward_workspace": (_c_ull, [_c_int, _c_int]),
+    "b200gemm_bf16_gated_backward": (_c_int, [_vp, _c_int, _c_int, _c_int, _vp, _c_ll, _vp, _c_ll, _vp, _vp,
+                                              _c_ll, _vp, _vp, _c_ll, _c_int, _vp, _c_ll, _vp, _vp, _c_ll,
+                                              _vp, _vp]),
+    "b200gemm_w4_quantize": (_c_int, [_vp, _c_int, _c_int, _vp, _c_ll, _c_int, _vp, _vp, _vp]),
+    "b200gemm_w4_dequantize": (_c_int, [_vp, _c_int, _c_int, _vp, _vp, _c_int, _vp, _c_ll, _vp]),
+    "b200gemm_w4_nt": (_c_int, [_vp, _c_int, _c_int, _c_int, _vp, _c_ll, _vp, _vp, _c_int, _vp, _c_ll, _c_int,
+                                _vp]),
+    "b200gemm_w4_gated": (_c_int, [_vp, _c_int, _c_int, _c_int, _vp, _c_ll, _vp, _vp, _vp, _vp, _c_int, _c_int,
+                                   _vp, _c_ll, _vp]),
     "b200gemm_strerror": (ctypes.c_char_p, [_c_int]),
     "b200gemm_version": (_c_int, []),
 }

@@ -12,10 +12,12 @@
 #include <vector>
 
 #include "b200gemm.h"
+#include "ffn_sm100.cuh"
 #include "gemm_decode_sm100.cuh"
 #include "gemm_sm100.cuh"
 #include "gemm_smallm1_sm100.cuh"
 #include "schedule.cuh"
+#include "skinny_sm100.cuh"
 
 namespace b200gemm {
 
@@ -458,6 +460,7 @@ struct b200gemm_handle {
   int decode_clusters[5] = {};        // [S]: co-resident clusters of the small-M pair kernel, split S
   int decode256_clusters[5] = {};     // the same for its instances covering 256 rows of A
   int smallm1_clusters[5] = {};       // [S]: the same for the single-CTA small-M kernel
+  int ffn_clusters = 0;               // co-resident clusters of the tiled feed-forward kernels
   int tile_width = 0;         // 0 = choose per call, else one of kWidths
   int small_m = -1;           // small-M kernel: -1 or 1 = use it when eligible, 0 = never
   int pdl = 0;                // B200GEMM_PDL_*: launch overlap with the previous kernel
@@ -482,6 +485,12 @@ struct b200gemm_handle {
   std::mutex staging_mu;   // serialises b200gemm_bf16_nt_host calls on one handle
   std::vector<ScheduleEntry> schedules;
 };
+
+namespace b200gemm {
+int prepare_ffn_kernels(int sm_count);
+template <bool W4, bool GATED>
+bool prepare_skinny_kernels();
+}  // namespace b200gemm
 
 extern "C" int b200gemm_version(void) { return kVersion; }
 
@@ -531,6 +540,10 @@ extern "C" int b200gemm_create(b200gemm_t* out, int device) {
   if (dw1 <= 0 || dw2 <= 0 || dw3 <= 0 || dw4 <= 0) return B200GEMM_ERR_CUDA;
   const int sc2 = prepare_smallm1_kernel<SmallMCfg<2>>(sms), sc4 = prepare_smallm1_kernel<SmallMCfg<4>>(sms);
   if (sc2 <= 0 || sc4 <= 0) return B200GEMM_ERR_CUDA;
+  const int fc = prepare_ffn_kernels(sms);
+  if (fc <= 0 || !prepare_skinny_kernels<false, true>() || !prepare_skinny_kernels<true, false>() ||
+      !prepare_skinny_kernels<true, true>())
+    return B200GEMM_ERR_CUDA;
 
   auto* h = new b200gemm_handle();
   h->device = device;
@@ -544,6 +557,7 @@ extern "C" int b200gemm_create(b200gemm_t* out, int device) {
   h->decode256_clusters[4] = dw4;
   h->smallm1_clusters[2] = sc2;
   h->smallm1_clusters[4] = sc4;
+  h->ffn_clusters = fc;
   h->max_clusters = cw[0];
   for (int i = 0; i < kNumWidths; ++i) {
     h->clusters_w[i] = cw[i];
@@ -1724,3 +1738,5 @@ extern "C" int b200gemm_bf16_nt_noalloc(int M, int N, int K, const void* A, cons
   }
   return e == cudaSuccess ? B200GEMM_OK : B200GEMM_ERR_CUDA;
 }
+
+#include "ffn_api.cuh"

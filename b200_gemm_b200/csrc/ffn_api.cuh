@@ -1,0 +1,569 @@
+// Host side of the feed-forward entry points of include/b200gemm.h: argument
+// checks, plans and launches of the kernels in ffn_sm100.cuh and
+// skinny_sm100.cuh.  Part of b200gemm.cu's translation unit (it uses the
+// handle and the helpers there).  Nothing here allocates, builds a table or
+// waits, so every call can be captured into a CUDA graph from the first one.
+#pragma once
+
+namespace b200gemm {
+
+// Stages fill shared memory next to the staging buffers: 3 x 48 KB + 64 KB,
+// or 6 x 32 KB + 16 KB.
+using FfnGated2 = FfnCfg<kGated, 2, 3>;
+using FfnGated1 = FfnCfg<kGated, 1, 6>;
+using FfnDx2 = FfnCfg<kDx, 2, 3>;
+using FfnDx1 = FfnCfg<kDx, 1, 6>;
+using FfnDw2 = FfnCfg<kDw, 2, 3>;
+using FfnDw1 = FfnCfg<kDw, 1, 6>;
+
+template <class Cfg>
+int prepare_ffn_kernel(int sm_count) {
+  if (cudaFuncSetAttribute(ffn_gemm_sm100<Cfg>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes) !=
+      cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3(static_cast<unsigned>(sm_count & ~1), 1, 1);
+  cfg.blockDim = dim3(Cfg::kThreads, 1, 1);
+  cfg.dynamicSmemBytes = Cfg::kSmemBytes;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int clusters = 0;
+  if (cudaOccupancyMaxActiveClusters(&clusters, ffn_gemm_sm100<Cfg>, &cfg) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  return clusters;
+}
+
+// Smallest number of clusters that fit over all instances of the tiled
+// feed-forward kernel (they differ only in registers), or 0 on failure.
+int prepare_ffn_kernels(int sm_count) {
+  const int c[6] = {prepare_ffn_kernel<FfnGated2>(sm_count), prepare_ffn_kernel<FfnGated1>(sm_count),
+                    prepare_ffn_kernel<FfnDx2>(sm_count),    prepare_ffn_kernel<FfnDx1>(sm_count),
+                    prepare_ffn_kernel<FfnDw2>(sm_count),    prepare_ffn_kernel<FfnDw1>(sm_count)};
+  int least = c[0];
+  for (int v : c) least = v < least ? v : least;
+  return least;
+}
+
+template <class Cfg>
+bool prepare_skinny_kernel() {
+  if (cudaFuncSetAttribute(skinny_sm100<Cfg>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes) !=
+      cudaSuccess) {
+    cudaGetLastError();
+    return false;
+  }
+  return true;
+}
+
+template <bool W4, bool GATED>
+bool prepare_skinny_kernels() {
+  return prepare_skinny_kernel<SkinnyCfg<W4, GATED, 1>>() && prepare_skinny_kernel<SkinnyCfg<W4, GATED, 2>>() &&
+         prepare_skinny_kernel<SkinnyCfg<W4, GATED, 4>>();
+}
+
+template <class Cfg>
+cudaError_t launch_ffn(int clusters, cudaStream_t stream, const CUtensorMap (&m)[7], const FfnParams& p) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(2 * clusters), 1, 1);
+  cfg.blockDim = dim3(Cfg::kThreads, 1, 1);
+  cfg.dynamicSmemBytes = Cfg::kSmemBytes;
+  cfg.stream = stream;
+  return cudaLaunchKernelEx(&cfg, ffn_gemm_sm100<Cfg>, m[0], m[1], m[2], m[3], m[4], m[5], m[6], p);
+}
+
+template <class Cfg>
+cudaError_t launch_skinny(int split, int rows, int token_blocks, cudaStream_t stream, const CUtensorMap& w0,
+                          const CUtensorMap& w1, const CUtensorMap& x, const SkinnyParams& p) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(split);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3(static_cast<unsigned>(split), static_cast<unsigned>(rows), static_cast<unsigned>(token_blocks));
+  cfg.blockDim = dim3(Cfg::kThreads, 1, 1);
+  cfg.dynamicSmemBytes = Cfg::kSmemBytes;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (p.pdl != kPdlOff) {
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.numAttrs = 2;
+  }
+  return cudaLaunchKernelEx(&cfg, skinny_sm100<Cfg>, w0, w1, x, p);
+}
+
+// One matrix of a call, for the overlap check: rows of `width` bytes every
+// `pitch` bytes.
+struct Extent {
+  const void* ptr;
+  long long rows, width, pitch;
+};
+
+// Whether two matrices share a byte.  Column slices of one wide matrix
+// (equal pitches) are told apart; other interleavings count as overlapping.
+bool overlaps(const Extent& a, const Extent& b) {
+  if (a.ptr == nullptr || b.ptr == nullptr || a.rows <= 0 || b.rows <= 0 || a.width <= 0 || b.width <= 0) return false;
+  const auto pa = reinterpret_cast<uintptr_t>(a.ptr), pb = reinterpret_cast<uintptr_t>(b.ptr);
+  const auto ea = pa + static_cast<uintptr_t>((a.rows - 1) * a.pitch + a.width);
+  const auto eb = pb + static_cast<uintptr_t>((b.rows - 1) * b.pitch + b.width);
+  if (ea <= pb || eb <= pa) return false;
+  if (a.pitch != b.pitch || a.pitch <= 0) return true;
+  const auto pitch = static_cast<uintptr_t>(a.pitch);
+  const long long d = static_cast<long long>(pb >= pa ? (pb - pa) % pitch : (pitch - (pa - pb) % pitch) % pitch);
+  return !(d >= a.width && d + b.width <= a.pitch);
+}
+
+// Outputs [0, outs) may share nothing with each other or with the inputs
+// [outs, count).
+bool outputs_distinct(const Extent* e, int outs, int count) {
+  for (int i = 0; i < outs; ++i)
+    for (int j = i + 1; j < count; ++j)
+      if (overlaps(e[i], e[j])) return false;
+  return true;
+}
+
+bool valid_activation(int act) { return act >= B200GEMM_ACT_NONE && act <= B200GEMM_ACT_SILU; }
+bool group_shift_of(int group, int* shift) {
+  for (int s = 5; s <= 8; ++s)
+    if (group == (1 << s)) {
+      *shift = s;
+      return true;
+    }
+  return false;
+}
+
+constexpr int kMaxExtent = 0x7FFFFFFF - 4096;  // rows, columns: tile coordinates stay inside an int
+
+// NB = 2 (512 accumulator columns, shared A stage) or 1 for a product whose
+// accumulators are `cols` columns wide, by the tile cost model of the plain
+// GEMM.  A forced tile width of 512 or 448 asks for 2, any other for 1.
+int ffn_nb(const b200gemm_handle* h, uint32_t tiles_m, int cols, int num_kb, double epi2, double epi1) {
+  if (h->tile_width != 0) return h->tile_width >= 448 ? 2 : 1;
+  const double c2 = tile_plan_cost(512, tiles_m, cols, num_kb, h->ffn_clusters, epi2);
+  const double c1 = tile_plan_cost(256, tiles_m, cols, num_kb, h->ffn_clusters, epi1);
+  return c2 < c1 ? 2 : 1;
+}
+
+// bf16 operand maps of the tiled kernel: K-major boxes of 64 k x 128 rows,
+// MN-major boxes of 64 columns x 64 k, both one 128-byte swizzle row wide.
+bool encode_kmajor(CUtensorMap* m, const void* ptr, int k, int rows, long long ld) {
+  return encode_2d(m, ptr, static_cast<uint64_t>(k), static_cast<uint64_t>(rows), static_cast<uint64_t>(ld) * 2,
+                   kBlockK, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+bool encode_mnmajor(CUtensorMap* m, const void* ptr, int mn, int k, long long ld) {
+  return encode_2d(m, ptr, static_cast<uint64_t>(mn), static_cast<uint64_t>(k), static_cast<uint64_t>(ld) * 2, 64, 64,
+                   CU_TENSOR_MAP_SWIZZLE_128B);
+}
+bool encode_out(CUtensorMap* m, void* ptr, int cols, int rows, long long ld) {
+  return encode_2d(m, ptr, static_cast<uint64_t>(cols), static_cast<uint64_t>(rows), static_cast<uint64_t>(ld) * 2,
+                   kCBoxCols, kCBoxRows, CU_TENSOR_MAP_SWIZZLE_64B);
+}
+
+// K ranges (CTAs of a cluster) of a skinny product: the smallest power of two
+// up to 8 that gives every SM a CTA, while each keeps at least two stages.
+int skinny_split(const b200gemm_handle* h, long long row_blocks, int num_stages) {
+  int split = 1;
+  while (split < 8 && row_blocks * split < h->sm_count && num_stages >= 4 * split) split *= 2;
+  return split;
+}
+
+template <bool W4, bool GATED>
+int run_skinny(b200gemm_t h, const void* w0, const void* w1, long long ldw, const void* X, long long ldx,
+               SkinnyParams p, cudaStream_t stream) {
+  const int nt = p.M > 16 ? 4 : (p.M > 8 ? 2 : 1);
+  const int cols = GATED ? 32 : 64;
+  const long long row_blocks = (static_cast<long long>(p.N) + cols - 1) / cols;
+  const long long token_blocks = (static_cast<long long>(p.M) + 31) / 32;
+  if (row_blocks > 65535 || token_blocks > 65535) return B200GEMM_ERR_TOO_LARGE;
+  CUtensorMap mw0, mw1, mx;
+  const auto encode_w = [&](CUtensorMap* m, const void* w) {
+    return W4 ? encode_2d(m, w, static_cast<uint64_t>(p.K) / 2, static_cast<uint64_t>(p.N),
+                          static_cast<uint64_t>(p.K) / 2, 128, static_cast<uint32_t>(cols), CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_DATA_TYPE_UINT8)
+              : encode_2d(m, w, static_cast<uint64_t>(p.K), static_cast<uint64_t>(p.N),
+                          static_cast<uint64_t>(ldw) * 2, 64, static_cast<uint32_t>(cols), CU_TENSOR_MAP_SWIZZLE_128B);
+  };
+  if (!encode_w(&mw0, w0) || (GATED && !encode_w(&mw1, w1)) ||
+      !encode_2d(&mx, X, static_cast<uint64_t>(p.K), static_cast<uint64_t>(p.M), static_cast<uint64_t>(ldx) * 2, 64,
+                 static_cast<uint32_t>(8 * nt), CU_TENSOR_MAP_SWIZZLE_128B)) {
+    return B200GEMM_ERR_CUDA;
+  }
+  if (!GATED) mw1 = mw0;
+  const int stage_k = SkinnyCfg<W4, GATED, 1>::kStageK;
+  p.num_stages = (p.K + stage_k - 1) / stage_k;
+  const int split = skinny_split(h, row_blocks * token_blocks, p.num_stages);
+  p.stages_per_cta = (p.num_stages + split - 1) / split;
+  {
+    std::lock_guard<std::mutex> lock(h->mu);
+    p.timeout_ns = h->timeout_ns;
+    p.pdl = h->pdl;
+  }
+  p.status = h->status_dev;
+  const int rb = static_cast<int>(row_blocks), tb = static_cast<int>(token_blocks);
+  const cudaError_t e =
+      nt == 1   ? launch_skinny<SkinnyCfg<W4, GATED, 1>>(split, rb, tb, stream, mw0, mw1, mx, p)
+      : nt == 2 ? launch_skinny<SkinnyCfg<W4, GATED, 2>>(split, rb, tb, stream, mw0, mw1, mx, p)
+                : launch_skinny<SkinnyCfg<W4, GATED, 4>>(split, rb, tb, stream, mw0, mw1, mx, p);
+  return e == cudaSuccess ? B200GEMM_OK : B200GEMM_ERR_CUDA;
+}
+
+template <class Cfg>
+int run_ffn(b200gemm_t h, const CUtensorMap (&maps)[7], FfnParams p, cudaStream_t stream) {
+  const long long tiles = static_cast<long long>(Cfg::kKind == kDw ? 2 : 1) * p.tiles_m * p.tiles_n;
+  if (tiles > (1ll << 30)) return B200GEMM_ERR_TOO_LARGE;
+  p.num_tiles = static_cast<int>(tiles);
+  p.band = B200GEMM_DEFAULT_BAND;
+  p.status = h->status_dev;
+  {
+    std::lock_guard<std::mutex> lock(h->mu);
+    p.timeout_ns = h->timeout_ns;
+  }
+  const int clusters = p.num_tiles < h->ffn_clusters ? p.num_tiles : h->ffn_clusters;
+  return launch_ffn<Cfg>(clusters, stream, maps, p) == cudaSuccess ? B200GEMM_OK : B200GEMM_ERR_CUDA;
+}
+
+template <int ACT>
+void launch_gated_grad(const GatedGradParams& p, cudaStream_t stream) {
+  const int bx = (p.F + 2047) / 2048;
+  int by = (148 * 32 + bx - 1) / bx;
+  if (by > p.M) by = p.M;
+  gated_grad_kernel<ACT><<<dim3(static_cast<unsigned>(bx), static_cast<unsigned>(by)), 256, 0, stream>>>(p);
+}
+
+}  // namespace b200gemm
+
+extern "C" int b200gemm_bf16_gated(b200gemm_t h, int M, int F, int K, const void* X, long long ldx, const void* Wg,
+                                   const void* Wu, long long ldw, int activation, void* H, long long ldh, void* G,
+                                   void* U, long long ldgu, void* stream_ptr) {
+  if (h == nullptr || M < 0 || F < 0 || K < 0 || !valid_activation(activation)) return B200GEMM_ERR_INVALID_ARG;
+  if ((G == nullptr) != (U == nullptr)) return B200GEMM_ERR_INVALID_ARG;
+  if (M == 0 || F == 0) return B200GEMM_OK;
+  if (K == 0) return B200GEMM_ERR_UNSUPPORTED;
+  if (X == nullptr || Wg == nullptr || Wu == nullptr || H == nullptr) return B200GEMM_ERR_INVALID_ARG;
+  if ((K % 8) != 0 || ldx < K || ldw < K || ldh < F || (ldx % 8) != 0 || (ldw % 8) != 0 || (ldh % 8) != 0)
+    return B200GEMM_ERR_UNSUPPORTED;
+  if (G != nullptr && (ldgu < F || (ldgu % 8) != 0)) return B200GEMM_ERR_UNSUPPORTED;
+  for (const void* q : {X, Wg, Wu, static_cast<const void*>(H), static_cast<const void*>(G), static_cast<const void*>(U)})
+    if (!aligned16(q)) return B200GEMM_ERR_UNSUPPORTED;
+  if (M > kMaxExtent || F > kMaxExtent || K > kMaxExtent) return B200GEMM_ERR_TOO_LARGE;
+  const Extent e[] = {{H, M, 2ll * F, 2 * ldh}, {G, M, 2ll * F, 2 * ldgu}, {U, M, 2ll * F, 2 * ldgu},
+                      {X, M, 2ll * K, 2 * ldx}, {Wg, F, 2ll * K, 2 * ldw}, {Wu, F, 2ll * K, 2 * ldw}};
+  if (!outputs_distinct(e, 3, 6)) return B200GEMM_ERR_INVALID_ARG;
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
+  DeviceGuard guard(h->device);
+  if (!guard.ok()) return B200GEMM_ERR_CUDA;
+
+  bool small;
+  int nb;
+  const int num_kb = (K + kBlockK - 1) / kBlockK;
+  const uint32_t tiles_m = static_cast<uint32_t>((M + kTileM - 1) / kTileM);
+  {
+    std::lock_guard<std::mutex> lock(h->mu);
+    small = M <= 32 && G == nullptr && h->small_m != 0 && h->tile_width == 0;
+    nb = ffn_nb(h, tiles_m, F > kMaxExtent / 2 ? kMaxExtent : 2 * F, num_kb, 16.0, 4.6);
+  }
+  if (small) {
+    SkinnyParams p{};
+    p.M = M;
+    p.N = F;
+    p.K = K;
+    p.act = activation;
+    p.out_type = kOutBf16;
+    p.out = H;
+    p.ldo = ldh;
+    return run_skinny<false, true>(h, Wg, Wu, ldw, X, ldx, p, stream);
+  }
+  CUtensorMap m[7];
+  if (!encode_kmajor(&m[0], X, K, M, ldx) || !encode_kmajor(&m[2], Wg, K, F, ldw) ||
+      !encode_kmajor(&m[3], Wu, K, F, ldw) || !encode_out(&m[4], H, F, M, ldh)) {
+    return B200GEMM_ERR_CUDA;
+  }
+  m[1] = m[0];
+  m[5] = m[6] = m[4];
+  if (G != nullptr && (!encode_out(&m[5], G, F, M, ldgu) || !encode_out(&m[6], U, F, M, ldgu)))
+    return B200GEMM_ERR_CUDA;
+  FfnParams p{};
+  p.M = M;
+  p.N = F;
+  p.num_kb = num_kb;
+  p.tiles_m = static_cast<int>(tiles_m);
+  p.tiles_n = (F + 128 * nb - 1) / (128 * nb);
+  p.act = activation;
+  p.save = G != nullptr ? 1 : 0;
+  p.out[0] = {static_cast<uint16_t*>(H), ldh};
+  p.out[1] = {static_cast<uint16_t*>(G), ldgu};
+  p.out[2] = {static_cast<uint16_t*>(U), ldgu};
+  return nb == 2 ? run_ffn<FfnGated2>(h, m, p, stream) : run_ffn<FfnGated1>(h, m, p, stream);
+}
+
+extern "C" unsigned long long b200gemm_gated_backward_workspace(int M, int F) {
+  if (M <= 0 || F <= 0) return 0;
+  const unsigned long long pitch = (static_cast<unsigned long long>(F) + 7) / 8 * 8;
+  return 4ull * static_cast<unsigned long long>(M) * pitch;
+}
+
+extern "C" int b200gemm_bf16_gated_backward(b200gemm_t h, int M, int F, int K, const void* dH, long long lddh,
+                                            const void* X, long long ldx, const void* Wg, const void* Wu,
+                                            long long ldw, const void* G, const void* U, long long ldgu,
+                                            int activation, void* dX, long long lddx, void* dWg, void* dWu,
+                                            long long lddw, void* workspace, void* stream_ptr) {
+  if (h == nullptr || M < 0 || F < 0 || K < 0 || !valid_activation(activation)) return B200GEMM_ERR_INVALID_ARG;
+  if ((dWg == nullptr) != (dWu == nullptr)) return B200GEMM_ERR_INVALID_ARG;
+  if (K == 0 || (dX == nullptr && dWg == nullptr)) return B200GEMM_OK;
+  if (M == 0 && F == 0) return B200GEMM_OK;
+  if ((K % 8) != 0) return B200GEMM_ERR_UNSUPPORTED;
+  if (dX != nullptr && (lddx < K || (lddx % 8) != 0 || !aligned16(dX))) return B200GEMM_ERR_UNSUPPORTED;
+  if (dWg != nullptr && (lddw < K || (lddw % 8) != 0 || !aligned16(dWg) || !aligned16(dWu)))
+    return B200GEMM_ERR_UNSUPPORTED;
+  if (M > kMaxExtent || F > kMaxExtent || K > kMaxExtent) return B200GEMM_ERR_TOO_LARGE;
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
+  if (M == 0 || F == 0) {  // empty sums
+    DeviceGuard guard(h->device);
+    if (!guard.ok()) return B200GEMM_ERR_CUDA;
+    const auto zero = [&](void* ptr, long long ld, int rows) {
+      return ptr == nullptr || rows == 0 ||
+             cudaMemset2DAsync(ptr, static_cast<size_t>(ld) * 2, 0, static_cast<size_t>(K) * 2,
+                               static_cast<size_t>(rows), stream) == cudaSuccess;
+    };
+    return zero(dX, lddx, M) && zero(dWg, lddw, F) && zero(dWu, lddw, F) ? B200GEMM_OK : B200GEMM_ERR_CUDA;
+  }
+  if (dH == nullptr || X == nullptr || Wg == nullptr || Wu == nullptr || G == nullptr || U == nullptr ||
+      workspace == nullptr)
+    return B200GEMM_ERR_INVALID_ARG;
+  if (lddh < F || ldx < K || ldw < K || ldgu < F || (lddh % 8) != 0 || (ldx % 8) != 0 || (ldw % 8) != 0 ||
+      (ldgu % 8) != 0)
+    return B200GEMM_ERR_UNSUPPORTED;
+  for (const void* q : {dH, X, Wg, Wu, G, U, static_cast<const void*>(workspace)})
+    if (!aligned16(q)) return B200GEMM_ERR_UNSUPPORTED;
+  const long long f8 = (static_cast<long long>(F) + 7) / 8 * 8;
+  const Extent e[] = {{workspace, 2ll * M, 2 * f8, 2 * f8},
+                      {dX, M, 2ll * K, 2 * lddx},
+                      {dWg, F, 2ll * K, 2 * lddw},
+                      {dWu, F, 2ll * K, 2 * lddw},
+                      {dH, M, 2ll * F, 2 * lddh},
+                      {X, M, 2ll * K, 2 * ldx},
+                      {Wg, F, 2ll * K, 2 * ldw},
+                      {Wu, F, 2ll * K, 2 * ldw},
+                      {G, M, 2ll * F, 2 * ldgu},
+                      {U, M, 2ll * F, 2 * ldgu}};
+  if (!outputs_distinct(e, 4, 10)) return B200GEMM_ERR_INVALID_ARG;
+  DeviceGuard guard(h->device);
+  if (!guard.ok()) return B200GEMM_ERR_CUDA;
+
+  GatedGradParams gp{};
+  gp.M = M;
+  gp.F = F;
+  gp.dh = static_cast<const uint16_t*>(dH);
+  gp.g = static_cast<const uint16_t*>(G);
+  gp.u = static_cast<const uint16_t*>(U);
+  gp.lddh = lddh;
+  gp.ldgu = ldgu;
+  gp.dg = static_cast<uint16_t*>(workspace);
+  gp.du = gp.dg + static_cast<long long>(M) * f8;
+  gp.ldo = f8;
+  switch (activation) {
+    case B200GEMM_ACT_RELU: launch_gated_grad<kActRelu>(gp, stream); break;
+    case B200GEMM_ACT_GELU: launch_gated_grad<kActGelu>(gp, stream); break;
+    case B200GEMM_ACT_GELU_TANH: launch_gated_grad<kActGeluTanh>(gp, stream); break;
+    case B200GEMM_ACT_SILU: launch_gated_grad<kActSilu>(gp, stream); break;
+    default: launch_gated_grad<kActNone>(gp, stream); break;
+  }
+  if (cudaGetLastError() != cudaSuccess) return B200GEMM_ERR_CUDA;
+
+  const int f8i = static_cast<int>(f8);
+  if (dX != nullptr) {
+    CUtensorMap m[7];
+    if (!encode_kmajor(&m[0], gp.dg, f8i, M, f8) || !encode_kmajor(&m[1], gp.du, f8i, M, f8) ||
+        !encode_mnmajor(&m[2], Wg, K, F, ldw) || !encode_mnmajor(&m[3], Wu, K, F, ldw) ||
+        !encode_out(&m[4], dX, K, M, lddx))
+      return B200GEMM_ERR_CUDA;
+    m[5] = m[6] = m[4];
+    FfnParams p{};
+    p.M = M;
+    p.N = K;
+    p.seg_kb = (F + kBlockK - 1) / kBlockK;
+    p.num_kb = 2 * p.seg_kb;
+    p.tiles_m = (M + kTileM - 1) / kTileM;
+    p.out[0] = {static_cast<uint16_t*>(dX), lddx};
+    int nb;
+    {
+      std::lock_guard<std::mutex> lock(h->mu);
+      nb = ffn_nb(h, static_cast<uint32_t>(p.tiles_m), K, p.num_kb, 0.0, 0.0);
+    }
+    p.tiles_n = (K + 256 * nb - 1) / (256 * nb);
+    const int rc = nb == 2 ? run_ffn<FfnDx2>(h, m, p, stream) : run_ffn<FfnDx1>(h, m, p, stream);
+    if (rc != B200GEMM_OK) return rc;
+  }
+  if (dWg != nullptr) {
+    CUtensorMap m[7];
+    if (!encode_mnmajor(&m[0], gp.dg, f8i, M, f8) || !encode_mnmajor(&m[1], gp.du, f8i, M, f8) ||
+        !encode_mnmajor(&m[2], X, K, M, ldx) || !encode_out(&m[4], dWg, K, F, lddw) ||
+        !encode_out(&m[5], dWu, K, F, lddw))
+      return B200GEMM_ERR_CUDA;
+    m[3] = m[2];
+    m[6] = m[4];
+    FfnParams p{};
+    p.M = F;
+    p.N = K;
+    p.num_kb = (M + kBlockK - 1) / kBlockK;
+    p.tiles_m = (F + kTileM - 1) / kTileM;
+    p.out[0] = {static_cast<uint16_t*>(dWg), lddw};
+    p.out[1] = {static_cast<uint16_t*>(dWu), lddw};
+    int nb;
+    {
+      std::lock_guard<std::mutex> lock(h->mu);
+      nb = ffn_nb(h, 2u * static_cast<uint32_t>(p.tiles_m), K, p.num_kb, 0.0, 0.0);
+    }
+    p.tiles_n = (K + 256 * nb - 1) / (256 * nb);
+    const int rc = nb == 2 ? run_ffn<FfnDw2>(h, m, p, stream) : run_ffn<FfnDw1>(h, m, p, stream);
+    if (rc != B200GEMM_OK) return rc;
+  }
+  return B200GEMM_OK;
+}
+
+namespace {
+
+// Checks shared by the two 4-bit products; OK means "go on".
+int w4_product_check(int K, int group, long long lda, const void* A, int* shift) {
+  if (!group_shift_of(group, shift) || (K % group) != 0) return B200GEMM_ERR_UNSUPPORTED;
+  if (lda < K || (lda % 8) != 0 || !aligned16(A)) return B200GEMM_ERR_UNSUPPORTED;
+  return B200GEMM_OK;
+}
+
+bool aligned2(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 1u) == 0; }
+
+int w4_convert_check(b200gemm_t h, int N, int K, const void* W, long long ldw, int group, const void* codes,
+                     const void* scales, int* shift) {
+  if (h == nullptr || N < 0 || K < 0) return B200GEMM_ERR_INVALID_ARG;
+  if (!group_shift_of(group, shift) || (K % group) != 0) return B200GEMM_ERR_UNSUPPORTED;
+  if (N == 0 || K == 0) return B200GEMM_OK;
+  if (W == nullptr || codes == nullptr || scales == nullptr) return B200GEMM_ERR_INVALID_ARG;
+  if (ldw < K || (ldw % 8) != 0 || !aligned16(W) || !aligned16(codes) || !aligned2(scales))
+    return B200GEMM_ERR_UNSUPPORTED;
+  if ((static_cast<long long>(N) + 31) / 32 > 65535 || K > kMaxExtent) return B200GEMM_ERR_TOO_LARGE;
+  return B200GEMM_OK;
+}
+
+}  // namespace
+
+extern "C" int b200gemm_w4_quantize(b200gemm_t h, int N, int K, const void* W, long long ldw, int group, void* codes,
+                                    void* scales, void* stream_ptr) {
+  W4Params p{};
+  const int rc = w4_convert_check(h, N, K, W, ldw, group, codes, scales, &p.group_shift);
+  if (rc != B200GEMM_OK || N == 0 || K == 0) return rc;
+  const Extent e[] = {{codes, 1, static_cast<long long>(N) * (K / 2), 0},
+                      {scales, 1, 2ll * N * (K / group), 0},
+                      {W, N, 2ll * K, 2 * ldw}};
+  if (!outputs_distinct(e, 2, 3)) return B200GEMM_ERR_INVALID_ARG;
+  DeviceGuard guard(h->device);
+  if (!guard.ok()) return B200GEMM_ERR_CUDA;
+  p.N = N;
+  p.K = K;
+  p.w = const_cast<uint16_t*>(static_cast<const uint16_t*>(W));
+  p.ldw = ldw;
+  p.codes = static_cast<uint8_t*>(codes);
+  p.scales = static_cast<uint16_t*>(scales);
+  const dim3 grid(static_cast<unsigned>((K + 255) / 256), static_cast<unsigned>((N + 31) / 32));
+  w4_quantize_kernel<<<grid, 256, 0, static_cast<cudaStream_t>(stream_ptr)>>>(p);
+  return cudaGetLastError() == cudaSuccess ? B200GEMM_OK : B200GEMM_ERR_CUDA;
+}
+
+extern "C" int b200gemm_w4_dequantize(b200gemm_t h, int N, int K, const void* codes, const void* scales, int group,
+                                      void* W, long long ldw, void* stream_ptr) {
+  W4Params p{};
+  const int rc = w4_convert_check(h, N, K, W, ldw, group, codes, scales, &p.group_shift);
+  if (rc != B200GEMM_OK || N == 0 || K == 0) return rc;
+  const Extent e[] = {{W, N, 2ll * K, 2 * ldw},
+                      {codes, 1, static_cast<long long>(N) * (K / 2), 0},
+                      {scales, 1, 2ll * N * (K / group), 0}};
+  if (!outputs_distinct(e, 1, 3)) return B200GEMM_ERR_INVALID_ARG;
+  DeviceGuard guard(h->device);
+  if (!guard.ok()) return B200GEMM_ERR_CUDA;
+  p.N = N;
+  p.K = K;
+  p.w = static_cast<uint16_t*>(W);
+  p.ldw = ldw;
+  p.codes = const_cast<uint8_t*>(static_cast<const uint8_t*>(codes));
+  p.scales = const_cast<uint16_t*>(static_cast<const uint16_t*>(scales));
+  const dim3 grid(static_cast<unsigned>((K + 255) / 256), static_cast<unsigned>((N + 31) / 32));
+  w4_dequantize_kernel<<<grid, 256, 0, static_cast<cudaStream_t>(stream_ptr)>>>(p);
+  return cudaGetLastError() == cudaSuccess ? B200GEMM_OK : B200GEMM_ERR_CUDA;
+}
+
+extern "C" int b200gemm_w4_nt(b200gemm_t h, int M, int N, int K, const void* A, long long lda, const void* codes,
+                              const void* scales, int group, void* C, long long ldc, int out_type, void* stream_ptr) {
+  if (h == nullptr || M < 0 || N < 0 || K < 0 || (out_type != B200GEMM_OUT_BF16 && out_type != B200GEMM_OUT_F32))
+    return B200GEMM_ERR_INVALID_ARG;
+  if (M == 0 || N == 0) return B200GEMM_OK;
+  if (K == 0) return B200GEMM_ERR_UNSUPPORTED;
+  if (A == nullptr || codes == nullptr || scales == nullptr || C == nullptr) return B200GEMM_ERR_INVALID_ARG;
+  SkinnyParams p{};
+  const int rc = w4_product_check(K, group, lda, A, &p.group_shift);
+  if (rc != B200GEMM_OK) return rc;
+  const int esize = out_type == B200GEMM_OUT_F32 ? 4 : 2;
+  if (ldc < N || !aligned16(codes) || !aligned2(scales) ||
+      (reinterpret_cast<uintptr_t>(C) & static_cast<uintptr_t>(esize - 1)) != 0)
+    return B200GEMM_ERR_UNSUPPORTED;
+  if (M > kMaxExtent || N > kMaxExtent || K > kMaxExtent) return B200GEMM_ERR_TOO_LARGE;
+  const Extent e[] = {{C, M, static_cast<long long>(esize) * N, esize * ldc},
+                      {A, M, 2ll * K, 2 * lda},
+                      {codes, 1, static_cast<long long>(N) * (K / 2), 0},
+                      {scales, 1, 2ll * N * (K / group), 0}};
+  if (!outputs_distinct(e, 1, 4)) return B200GEMM_ERR_INVALID_ARG;
+  DeviceGuard guard(h->device);
+  if (!guard.ok()) return B200GEMM_ERR_CUDA;
+  p.M = M;
+  p.N = N;
+  p.K = K;
+  p.out_type = out_type;
+  p.scales0 = static_cast<const uint16_t*>(scales);
+  p.out = C;
+  p.ldo = ldc;
+  return run_skinny<true, false>(h, codes, nullptr, 0, A, lda, p, static_cast<cudaStream_t>(stream_ptr));
+}
+
+extern "C" int b200gemm_w4_gated(b200gemm_t h, int M, int F, int K, const void* X, long long ldx,
+                                 const void* gate_codes, const void* gate_scales, const void* up_codes,
+                                 const void* up_scales, int group, int activation, void* H, long long ldh,
+                                 void* stream_ptr) {
+  if (h == nullptr || M < 0 || F < 0 || K < 0 || !valid_activation(activation)) return B200GEMM_ERR_INVALID_ARG;
+  if (M == 0 || F == 0) return B200GEMM_OK;
+  if (K == 0) return B200GEMM_ERR_UNSUPPORTED;
+  if (X == nullptr || gate_codes == nullptr || gate_scales == nullptr || up_codes == nullptr || up_scales == nullptr ||
+      H == nullptr)
+    return B200GEMM_ERR_INVALID_ARG;
+  SkinnyParams p{};
+  const int rc = w4_product_check(K, group, ldx, X, &p.group_shift);
+  if (rc != B200GEMM_OK) return rc;
+  if (ldh < F || !aligned16(gate_codes) || !aligned16(up_codes) || !aligned2(gate_scales) || !aligned2(up_scales) ||
+      !aligned2(H))
+    return B200GEMM_ERR_UNSUPPORTED;
+  if (M > kMaxExtent || F > kMaxExtent || K > kMaxExtent) return B200GEMM_ERR_TOO_LARGE;
+  const long long code_bytes = static_cast<long long>(F) * (K / 2), scale_bytes = 2ll * F * (K / group);
+  const Extent e[] = {{H, M, 2ll * F, 2 * ldh},       {X, M, 2ll * K, 2 * ldx},
+                      {gate_codes, 1, code_bytes, 0}, {gate_scales, 1, scale_bytes, 0},
+                      {up_codes, 1, code_bytes, 0},   {up_scales, 1, scale_bytes, 0}};
+  if (!outputs_distinct(e, 1, 6)) return B200GEMM_ERR_INVALID_ARG;
+  DeviceGuard guard(h->device);
+  if (!guard.ok()) return B200GEMM_ERR_CUDA;
+  p.M = M;
+  p.N = F;
+  p.K = K;
+  p.act = activation;
+  p.out_type = kOutBf16;
+  p.scales0 = static_cast<const uint16_t*>(gate_scales);
+  p.scales1 = static_cast<const uint16_t*>(up_scales);
+  p.out = H;
+  p.ldo = ldh;
+  return run_skinny<true, true>(h, gate_codes, up_codes, 0, X, ldx, p, static_cast<cudaStream_t>(stream_ptr));
+}

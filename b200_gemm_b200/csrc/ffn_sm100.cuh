@@ -1,0 +1,493 @@
+// Gated feed-forward block for sm_100a, forward and backward:
+//   H = act(G) * U with G = X Wg^T, U = X Wu^T      (X [M,K], Wg, Wu [F,K])
+//   dU = dH * act(G), dG = dH * U * act'(G)
+//   dX = dG Wg + dU Wu, dWg = dG^T X, dWu = dU^T X
+// in bf16 with fp32 accumulation in TMEM.  One persistent, warp-specialised
+// kernel (roles, ring, bounded waits and teardown as in gemm_sm100.cuh) in
+// three kinds that differ in what feeds the two operands of an MMA and in
+// what is done with the accumulator:
+//   kGated  A = X, B = Wg and Wu; a tile's accumulator holds a block of
+//           G next to the same block of U, and the epilogue combines them,
+//           so neither goes to memory unless the caller keeps it.
+//   kDx     one sum over the 2F products: first dG (A) with Wg (B), then dU
+//           with Wu, so dX is written once.  Wg is [F,K] and F is summed
+//           over, so B is read "MN-major": a TMA box is 64 columns (of the
+//           output) x 64 rows (of the sum).
+//   kDw     dWg and dWu in one launch: the tile rows of both follow one
+//           another.  The sum runs over the M rows, so dG/dU and X are both
+//           read MN-major.
+// MN-major operands cost nothing over K-major ones: the same bytes per stage
+// in the same 128-byte swizzle, two 8 KB boxes instead of one of 16 KB.
+// No transposed copy of anything is made.
+#pragma once
+
+#include <cstdint>
+#include <cuda.h>
+#include <cuda_bf16.h>
+
+#include "gemm_sm100.cuh"
+
+namespace b200gemm {
+
+enum FfnKind { kGated = 0, kDx = 1, kDw = 2 };
+
+struct FfnOut {
+  uint16_t* ptr;   // bf16 bits
+  long long ld;    // row pitch in elements
+};
+
+struct FfnParams {
+  int M, N;          // rows and columns of one output matrix (kGated: N = F)
+  int num_kb;        // K blocks of a tile
+  int seg_kb;        // kDx: K blocks of the first product (num_kb = 2 seg_kb)
+  int tiles_m;       // tile rows of one output matrix
+  int tiles_n;       // tile columns
+  int num_tiles;     // tiles of the launch (kDw: both matrices')
+  int band;          // tile rows per band of the tile order
+  int act;           // kAct*
+  int save;          // kGated: G and U are written too
+  FfnOut out[3];     // kGated: H, G, U; kDx: dX; kDw: dWg, dWu
+  unsigned int* status;
+  unsigned long long timeout_ns;
+};
+
+// NB = 2: 256 x 512 accumulators, a single one: two N = 256 MMAs per K step
+//         share the A stage.  kGated: G's 256 columns, then U's (256
+//         columns of H per tile); otherwise 512 columns of the output.
+// NB = 1: 256 x 256 accumulators, two of them, so a tile's epilogue
+//         overlaps the next tile's MMAs.  kGated: the N = 256 MMA takes its
+//         first 128 B rows from the even CTA and the others from the odd one,
+//         so the even CTA loads rows of Wg and the odd one the same rows of
+//         Wu (128 columns of H per tile).
+template <int KIND, int NB, int STAGES>
+struct FfnCfg {
+  static constexpr int kKind = KIND;
+  static constexpr int kNB = NB;
+  static constexpr int kStages = STAGES;
+  static constexpr bool kAMn = KIND == kDw;      // A read MN-major
+  static constexpr bool kBMn = KIND != kGated;   // B read MN-major
+  static constexpr int kAccCols = 256 * NB;
+  static constexpr int kTileN = KIND == kGated ? 128 * NB : 256 * NB;  // output columns per tile
+  static constexpr int kAccBufs = NB == 1 ? 2 : 1;
+  static constexpr uint32_t kIdesc = (1u << 4) | (1u << 7) | (1u << 10) | (kAMn ? 1u << 15 : 0u) |
+                                     (kBMn ? 1u << 16 : 0u) | ((256u >> 3) << 17) | ((256u >> 4) << 24);
+  static constexpr int kEpiWarps = 4 * NB;
+  static constexpr int kThreads = 64 + 32 * kEpiWarps;
+  static constexpr int kWarpCols = kTileN / NB;              // output columns one epilogue warp writes
+  static constexpr int kWarpChunks = kWarpCols / kCBoxCols;
+  static constexpr int kCBufs = NB == 2 ? 4 : 2;
+  static constexpr int kBlockBytesB = 128 * kBlockK * 2;     // one CTA's half of one N = 256 block
+  static constexpr int kStageBytesB = NB * kBlockBytesB;
+  static constexpr uint32_t kTxBytes = 2 * (kStageBytesA + kStageBytesB);
+  static constexpr int kA = 0;
+  static constexpr int kB = kA + STAGES * kStageBytesA;
+  static constexpr int kC = kB + STAGES * kStageBytesB;
+  static constexpr int kFull = kC + kEpiWarps * kCBufs * kCStageBytes;
+  static constexpr int kEmpty = kFull + 8 * STAGES;
+  static constexpr int kTFull = kEmpty + 8 * STAGES;
+  static constexpr int kTEmpty = kTFull + 8 * kAccBufs;
+  static constexpr int kDrain = kTEmpty + 8 * kAccBufs;
+  static constexpr int kTmemSlot = kDrain + 8;
+  static constexpr int kAbort = kTmemSlot + 4;
+  static constexpr int kEnd = kAbort + 4;
+  static constexpr int kSmemBytes = kEnd + 1024;
+  static_assert(kSmemBytes <= 232448, "exceeds the 227 KB per-CTA shared memory limit");
+};
+
+// Matrix descriptor of an MN-major operand in the 128-byte swizzle: 64
+// consecutive MN elements form a 128-byte row, 8 rows (of K) a 1024-byte
+// atom; the next 8 K rows follow 1024 B on (stride offset) and the next 64
+// MN elements one 64 x 64 box = 8192 B on (leading offset).  A K step of 16
+// is two atoms, 2048 B.
+constexpr uint64_t kSmemDescHiMn = (uint64_t(1024 >> 4) << 32) | (uint64_t(8192 >> 4) << 16) |
+                                   (uint64_t(1) << 46) | (uint64_t(2) << 61);
+template <bool MN>
+__device__ __forceinline__ uint64_t ffn_desc(uint32_t addr) {
+  return (MN ? kSmemDescHiMn : kSmemDescHi) | uint64_t((addr & 0x3FFFFu) >> 4);
+}
+// Descriptor units (16 B) from one K step of 16 to the next.
+template <bool MN>
+constexpr uint64_t kDescStep = MN ? 128 : 2;
+
+// Tile t of the band order: bands of `band` tile rows, each swept column by
+// column, so the band's A rows and one column of B stay in L2 meanwhile.
+__device__ __forceinline__ void ffn_tile(const FfnParams& p, int tiles_m, int t, int& tm, int& tn) {
+  const int per_band = p.band * p.tiles_n;
+  const int b = t / per_band, r = t - b * per_band;
+  const int rows = min(p.band, tiles_m - b * p.band);
+  tn = r / rows;
+  tm = b * p.band + (r - tn * rows);
+}
+
+// act(x) for bf16 results: e^x and the reciprocal are the fast forms, whose
+// relative error (2^-21) is far below bf16's 2^-9.  The tanh form of GELU
+// goes through the logistic function, 0.5 (1 + tanh z) = 1 / (1 + e^-2z),
+// which keeps its relative accuracy where tanh is near -1.
+template <int ACT>
+__device__ __forceinline__ float ffn_act(float x) {
+  if constexpr (ACT == kActRelu) return fmaxf(x, 0.0f);
+  if constexpr (ACT == kActGelu) return 0.5f * x * (1.0f + erff(x * 0.70710678118654752f));
+  if constexpr (ACT == kActGeluTanh)
+    return x * ptx::rcp_approx(1.0f + __expf(-1.5957691216057308f * fmaf(0.044715f * x, x * x, x)));
+  if constexpr (ACT == kActSilu) return x * ptx::rcp_approx(1.0f + __expf(-x));
+  return x;
+}
+
+// act(x) and its derivative:
+//   silu       s = 1 / (1 + e^-x):     s (1 + x (1 - s))
+//   gelu       Phi(x) + x phi(x)
+//   gelu_tanh  s = 1 / (1 + e^-2z):    s + x s (1 - s) 2 z'
+// x^2 is capped in 2 z' (it multiplies an exact zero there).
+template <int ACT>
+__device__ __forceinline__ void ffn_act_grad(float x, float& a, float& da) {
+  if constexpr (ACT == kActRelu) {
+    a = fmaxf(x, 0.0f);
+    da = x > 0.0f ? 1.0f : 0.0f;
+  } else if constexpr (ACT == kActGelu) {
+    const float phi = 0.5f * (1.0f + erff(x * 0.70710678118654752f));
+    a = x * phi;
+    da = fmaf(x * 0.39894228040143268f, __expf(-0.5f * x * x), phi);
+  } else if constexpr (ACT == kActGeluTanh) {
+    const float x2 = x * x;
+    const float s = ptx::rcp_approx(1.0f + __expf(-1.5957691216057308f * fmaf(0.044715f * x, x2, x)));
+    a = x * s;
+    da = fmaf(a * (1.0f - s), 1.5957691216057308f * fmaf(0.134145f, fminf(x2, 1e30f), 1.0f), s);
+  } else if constexpr (ACT == kActSilu) {
+    const float s = ptx::rcp_approx(1.0f + __expf(-x));
+    a = x * s;
+    da = fmaf(a, 1.0f - s, s);
+  } else {
+    a = x;
+    da = 1.0f;
+  }
+}
+
+// h = act(g) * u on one lane's 32 columns, rounded to bf16 pairs.  The
+// activation is switched outside the straight loop.
+template <int ACT>
+__device__ __forceinline__ void ffn_combine32(const uint32_t (&g)[32], const uint32_t (&u)[32], uint32_t (&w)[16]) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const float lo = ffn_act<ACT>(__uint_as_float(g[2 * i])) * __uint_as_float(u[2 * i]);
+    const float hi = ffn_act<ACT>(__uint_as_float(g[2 * i + 1])) * __uint_as_float(u[2 * i + 1]);
+    w[i] = ptx::pack_bf16x2(__float_as_uint(lo), __float_as_uint(hi));
+  }
+}
+__device__ __forceinline__ void ffn_combine(int act, const uint32_t (&g)[32], const uint32_t (&u)[32],
+                                            uint32_t (&w)[16]) {
+  switch (act) {
+    case kActRelu: ffn_combine32<kActRelu>(g, u, w); break;
+    case kActGelu: ffn_combine32<kActGelu>(g, u, w); break;
+    case kActGeluTanh: ffn_combine32<kActGeluTanh>(g, u, w); break;
+    case kActSilu: ffn_combine32<kActSilu>(g, u, w); break;
+    default: ffn_combine32<kActNone>(g, u, w); break;
+  }
+}
+
+// One 32 x 32 chunk of a bf16 output (lane = row, w = 16 packed pairs): a
+// swizzled staging buffer and a TMA store, or predicated element stores for
+// the chunk that ends inside a 16-byte group (TMA clips in 16-byte units).
+template <int BUFS>
+__device__ __forceinline__ void ffn_store_chunk(const uint32_t (&w)[16], int col, int row, uint32_t lane,
+                                                uint32_t cstage0, uint32_t& cbuf, const CUtensorMap& map,
+                                                const FfnOut& o, int M, int N) {
+  if (row >= M || col >= N) return;  // warp-uniform
+  if ((N % 8) != 0 && col + kCBoxCols > N) {
+    const int r = row + static_cast<int>(lane);
+    if (r < M) {
+      uint16_t* dst = o.ptr + static_cast<long long>(r) * o.ld + col;
+      const int ncols = N - col;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        if (2 * i < ncols) dst[2 * i] = static_cast<uint16_t>(w[i] & 0xFFFFu);
+        if (2 * i + 1 < ncols) dst[2 * i + 1] = static_cast<uint16_t>(w[i] >> 16);
+      }
+    }
+    return;
+  }
+  const uint32_t buf = cstage0 + cbuf * kCStageBytes;
+  if (lane == 0) ptx::bulk_wait_group_read<BUFS - 1>();  // the store that last read this buffer is done
+  __syncwarp();
+  stage_chunk_row(buf, lane, w);
+  ptx::fence_proxy_async_smem();
+  __syncwarp();
+  if (lane == 0) {
+    ptx::tma_store_2d(&map, buf, col, row);
+    ptx::bulk_commit_group();
+  }
+  if (++cbuf == BUFS) cbuf = 0;
+}
+
+template <class Cfg>
+__global__ void __launch_bounds__(Cfg::kThreads, 1) __cluster_dims__(2, 1, 1)
+    ffn_gemm_sm100(const __grid_constant__ CUtensorMap map_a0, const __grid_constant__ CUtensorMap map_a1,
+                   const __grid_constant__ CUtensorMap map_b0, const __grid_constant__ CUtensorMap map_b1,
+                   const __grid_constant__ CUtensorMap map_c0, const __grid_constant__ CUtensorMap map_c1,
+                   const __grid_constant__ CUtensorMap map_c2, const FfnParams p) {
+  constexpr int STAGES = Cfg::kStages;
+  constexpr int NB = Cfg::kNB;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const uint32_t base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
+
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+  const uint32_t rank = ptx::cluster_ctarank();
+  const bool leader = rank == 0;
+  const int cluster = static_cast<int>(ptx::cluster_id_x());
+  const int nclusters = static_cast<int>(ptx::num_clusters_x());
+  const int all_tiles_m = Cfg::kKind == kDw ? 2 * p.tiles_m : p.tiles_m;
+
+  const uint32_t sA = base + Cfg::kA, sB = base + Cfg::kB, sC = base + Cfg::kC;
+  const uint32_t full0 = base + Cfg::kFull, empty0 = base + Cfg::kEmpty;
+  const uint32_t tfull0 = base + Cfg::kTFull, tempty0 = base + Cfg::kTEmpty;
+  const uint32_t drain = base + Cfg::kDrain, tmem_slot = base + Cfg::kTmemSlot;
+
+  ptx::Watchdog wd;
+  wd.abort_flag = base + Cfg::kAbort;
+  wd.peer_abort_flag = ptx::mapa(wd.abort_flag, rank ^ 1u);
+  wd.status = p.status;
+  wd.timeout_ns = p.timeout_ns;
+
+  if (threadIdx.x == 0) {
+    asm volatile("st.shared.u32 [%0], 0;" ::"r"(wd.abort_flag) : "memory");
+    for (int s = 0; s < STAGES; ++s) {
+      ptx::mbar_init(full0 + 8 * s, 1);   // leader's expect_tx arrival (+ bytes of both CTAs)
+      ptx::mbar_init(empty0 + 8 * s, 1);  // one MMA commit
+    }
+    for (int a = 0; a < Cfg::kAccBufs; ++a) {
+      ptx::mbar_init(tfull0 + 8 * a, 1);                     // one MMA commit
+      ptx::mbar_init(tempty0 + 8 * a, 2 * Cfg::kEpiWarps);   // every epilogue warp of the pair
+    }
+    ptx::mbar_init(drain, 1);
+    ptx::fence_mbar_init_cluster();
+    ptx::prefetch_tensormap(&map_a0);
+    ptx::prefetch_tensormap(&map_b0);
+    ptx::prefetch_tensormap(&map_c0);
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc_cg2(tmem_slot, kTmemCols);
+    ptx::tmem_relinquish_cg2();
+  }
+  ptx::tc_fence_before();
+  ptx::cluster_sync_all();
+  ptx::tc_fence_after();
+  uint32_t tmem_base;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem_base) : "r"(tmem_slot) : "memory");
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer
+    if (lane == 0) {
+      const uint64_t policy = ptx::policy_evict_last();
+      const uint32_t full_leader0 = ptx::mapa(full0, 0);
+      uint32_t stage = 0, phase = 0;
+      bool ok = true;
+      for (int t = cluster; t < p.num_tiles && ok; t += nclusters) {
+        int tm, tn;
+        ffn_tile(p, all_tiles_m, t, tm, tn);
+        const bool second = Cfg::kKind == kDw && tm >= p.tiles_m;  // dWu's rows
+        if (second) tm -= p.tiles_m;
+        const int row_a = tm * kTileM + static_cast<int>(rank) * 128;
+        const int row_b = tn * Cfg::kTileN + ((Cfg::kKind == kGated && NB == 1) ? 0 : static_cast<int>(rank) * 128);
+        for (int kb = 0; kb < p.num_kb; ++kb) {
+          if (!ptx::mbar_wait(empty0 + 8 * stage, phase ^ 1u, wd, kSiteProducer, static_cast<unsigned>(t))) {
+            ok = false;
+            break;
+          }
+          if (leader) ptx::mbar_arrive_expect_tx(full0 + 8 * stage, Cfg::kTxBytes);
+          const uint32_t fb = full_leader0 + 8 * stage;
+          const bool seg1 = Cfg::kKind == kDx && kb >= p.seg_kb;
+          const int k = (seg1 ? kb - p.seg_kb : kb) * kBlockK;
+          const CUtensorMap* ma = (second || seg1) ? &map_a1 : &map_a0;
+          const uint32_t da = sA + stage * kStageBytesA, db = sB + stage * Cfg::kStageBytesB;
+          if constexpr (Cfg::kAMn) {
+            ptx::tma_load_2d_cg2(da, ma, fb, row_a, k, policy);
+            ptx::tma_load_2d_cg2(da + 8192, ma, fb, row_a + 64, k, policy);
+          } else {
+            ptx::tma_load_2d_cg2(da, ma, fb, k, row_a, policy);
+          }
+#pragma unroll
+          for (int h = 0; h < NB; ++h) {
+            const uint32_t d = db + h * Cfg::kBlockBytesB;
+            if constexpr (Cfg::kKind == kGated) {
+              const bool up = NB == 2 ? h == 1 : rank == 1;
+              ptx::tma_load_2d_cg2(d, up ? &map_b1 : &map_b0, fb, k, row_b, policy);
+            } else {
+              const CUtensorMap* mb = seg1 ? &map_b1 : &map_b0;
+              ptx::tma_load_2d_cg2(d, mb, fb, row_b + h * 256, k, policy);
+              ptx::tma_load_2d_cg2(d + 8192, mb, fb, row_b + h * 256 + 64, k, policy);
+            }
+          }
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ----------------------------------------------------------------- MMA
+    if (leader && lane == 0) {
+      const uint32_t own_empty0 = ptx::mapa(empty0, 0), peer_empty0 = ptx::mapa(empty0, 1);
+      const uint32_t own_tfull0 = ptx::mapa(tfull0, 0), peer_tfull0 = ptx::mapa(tfull0, 1);
+      uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
+      bool ok = true;
+      for (int t = cluster; t < p.num_tiles && ok; t += nclusters) {
+        if (!ptx::mbar_wait(tempty0 + 8 * acc, acc_phase ^ 1u, wd, kSiteMmaTmemEmpty, static_cast<unsigned>(t))) break;
+        ptx::tc_fence_after();
+        const uint32_t d_tmem = tmem_base + acc * 256u;
+        for (int kb = 0; kb < p.num_kb; ++kb) {
+          if (!ptx::mbar_wait(full0 + 8 * stage, phase, wd, kSiteMmaFull, static_cast<unsigned>(t))) {
+            ok = false;
+            break;
+          }
+          ptx::tc_fence_after();
+          const uint64_t a_desc = ffn_desc<Cfg::kAMn>(sA + stage * kStageBytesA);
+          const uint64_t b_desc = ffn_desc<Cfg::kBMn>(sB + stage * Cfg::kStageBytesB);
+#pragma unroll
+          for (int k = 0; k < kBlockK / kMmaK; ++k) {
+#pragma unroll
+            for (int h = 0; h < NB; ++h) {
+              ptx::mma_bf16_cg2(d_tmem + h * 256u, a_desc + k * kDescStep<Cfg::kAMn>,
+                                b_desc + (h * Cfg::kBlockBytesB >> 4) + k * kDescStep<Cfg::kBMn>, Cfg::kIdesc,
+                                (kb > 0 || k > 0) ? 1u : 0u);
+            }
+          }
+          ptx::mma_commit_cg2(own_empty0 + 8 * stage);
+          ptx::mma_commit_cg2(peer_empty0 + 8 * stage);
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (!ok) break;
+        ptx::mma_commit_cg2(own_tfull0 + 8 * acc);
+        ptx::mma_commit_cg2(peer_tfull0 + 8 * acc);
+        if (++acc == Cfg::kAccBufs) {
+          acc = 0;
+          acc_phase ^= 1u;
+        }
+      }
+      // Every MMA this thread issued must be complete before TMEM is freed
+      // and before the peer CTA (whose shared memory the MMAs read) exits.
+      ptx::mma_commit_cg2(ptx::mapa(drain, 0));
+      ptx::Watchdog dwd = wd;
+      dwd.timeout_ns = 100000000ull;
+      ptx::mbar_wait_drain(drain, 0, dwd, kSiteDrain);
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------ epilogue
+    const uint32_t e = warp - 2u;
+    const uint32_t quarter = warp & 3u;   // TMEM lanes this warp may access
+    const uint32_t nblk = e >> 2;         // which kWarpCols output columns of the tile
+    const uint32_t cstage0 = sC + e * Cfg::kCBufs * kCStageBytes;
+    const uint32_t tempty_leader0 = ptx::mapa(tempty0, 0);
+    uint32_t acc = 0, acc_phase = 0, cbuf = 0;
+    for (int t = cluster; t < p.num_tiles; t += nclusters) {
+      int tm, tn;
+      ffn_tile(p, all_tiles_m, t, tm, tn);
+      const bool second = Cfg::kKind == kDw && tm >= p.tiles_m;
+      if (second) tm -= p.tiles_m;
+      const int row = tm * kTileM + static_cast<int>(rank) * 128 + static_cast<int>(quarter) * 32;
+      const int col0 = tn * Cfg::kTileN + static_cast<int>(nblk) * Cfg::kWarpCols;
+      const bool full_ok = ptx::mbar_wait(tfull0 + 8 * acc, acc_phase, wd, kSiteEpilogue, static_cast<unsigned>(t));
+      if (!__all_sync(0xFFFFFFFFu, full_ok)) break;
+      ptx::tc_fence_after();
+      const uint32_t t_row = tmem_base + ((quarter * 32u) << 16) + acc * 256u + nblk * Cfg::kWarpCols;
+      auto release = [&]() {  // this warp's TMEM reads are done
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive_cluster(tempty_leader0 + 8 * acc);
+      };
+      if constexpr (Cfg::kKind == kGated) {
+        constexpr uint32_t kUp = 128u * NB;  // U's columns follow G's
+#pragma unroll 1
+        for (int c = 0; c < Cfg::kWarpChunks; ++c) {
+          uint32_t g[32], u[32], w[16];
+          ptx::tmem_ld_32x32b_x32(t_row + c * kCBoxCols, g);
+          ptx::tmem_ld_32x32b_x32(t_row + kUp + c * kCBoxCols, u);
+          ptx::tmem_wait_ld();
+          ptx::reg_fence32(g);
+          ptx::reg_fence32(u);
+          if (c == Cfg::kWarpChunks - 1) release();
+          const int col = col0 + c * kCBoxCols;
+          ffn_combine(p.act, g, u, w);
+          ffn_store_chunk<Cfg::kCBufs>(w, col, row, lane, cstage0, cbuf, map_c0, p.out[0], p.M, p.N);
+          if (p.save) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) w[i] = ptx::pack_bf16x2(g[2 * i], g[2 * i + 1]);
+            ffn_store_chunk<Cfg::kCBufs>(w, col, row, lane, cstage0, cbuf, map_c1, p.out[1], p.M, p.N);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) w[i] = ptx::pack_bf16x2(u[2 * i], u[2 * i + 1]);
+            ffn_store_chunk<Cfg::kCBufs>(w, col, row, lane, cstage0, cbuf, map_c2, p.out[2], p.M, p.N);
+          }
+        }
+      } else {
+#pragma unroll 1
+        for (int c = 0; c < Cfg::kWarpChunks; ++c) {
+          uint32_t v[32], w[16];
+          ptx::tmem_ld_32x32b_x32(t_row + c * kCBoxCols, v);
+          ptx::tmem_wait_ld();
+          ptx::reg_fence32(v);
+          if (c == Cfg::kWarpChunks - 1) release();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) w[i] = ptx::pack_bf16x2(v[2 * i], v[2 * i + 1]);
+          ffn_store_chunk<Cfg::kCBufs>(w, col0 + c * kCBoxCols, row, lane, cstage0, cbuf,
+                                       second ? map_c1 : map_c0, second ? p.out[1] : p.out[0], p.M, p.N);
+        }
+      }
+      if (++acc == Cfg::kAccBufs) {
+        acc = 0;
+        acc_phase ^= 1u;
+      }
+    }
+    if (lane == 0) ptx::bulk_wait_group_read<0>();  // staging reusable; the stores land before the kernel completes
+    __syncwarp();
+  }
+
+  // --------------------------------------------------------------- teardown
+  if (threadIdx.x == 0 && ptx::aborted(wd)) ptx::sleep_ns_bounded(200000ull);
+  ptx::tc_fence_before();
+  ptx::cluster_sync_all();
+  ptx::tc_fence_after();
+  if (warp == 1) ptx::tmem_dealloc_cg2(tmem_base, kTmemCols);
+}
+
+// dG and dU from dH, G and U, element by element: 6 bytes read and 4 written
+// per element, so DRAM-bound; a thread takes 8 columns (16 bytes of each).
+// They are rounded to bf16 once, to be operands of the tensor cores.  Rows of
+// the results are ldo elements (F rounded up to 8) and their padding columns
+// are set to 0: the products below sum over them.
+struct GatedGradParams {
+  int M, F;
+  const uint16_t *dh, *g, *u;
+  long long lddh, ldgu;
+  uint16_t *dg, *du;
+  long long ldo;
+};
+
+template <int ACT>
+__global__ void __launch_bounds__(256) gated_grad_kernel(const GatedGradParams p) {
+  const int col = static_cast<int>(blockIdx.x * 256u + threadIdx.x) * 8;
+  if (col >= p.F) return;
+  for (long long r = blockIdx.y; r < p.M; r += gridDim.y) {
+    uint32_t h[4], g[4], u[4], dg[4], du[4];
+    load_bf16x8(p.dh + r * p.lddh, col, p.F, h);
+    load_bf16x8(p.g + r * p.ldgu, col, p.F, g);
+    load_bf16x8(p.u + r * p.ldgu, col, p.F, u);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float a0, a1, d0, d1;
+      ffn_act_grad<ACT>(bf16_lo(g[i]), a0, d0);
+      ffn_act_grad<ACT>(bf16_hi(g[i]), a1, d1);
+      const float h0 = bf16_lo(h[i]), h1 = bf16_hi(h[i]);
+      du[i] = ptx::pack_bf16x2(__float_as_uint(h0 * a0), __float_as_uint(h1 * a1));
+      dg[i] = ptx::pack_bf16x2(__float_as_uint(h0 * bf16_lo(u[i]) * d0), __float_as_uint(h1 * bf16_hi(u[i]) * d1));
+    }
+    // (columns past F were read as 0, so their products are 0 too)
+    ptx::st_global_v4(p.dg + r * p.ldo + col, dg[0], dg[1], dg[2], dg[3]);
+    ptx::st_global_v4(p.du + r * p.ldo + col, du[0], du[1], du[2], du[3]);
+  }
+}
+
+}  // namespace b200gemm

@@ -1,0 +1,490 @@
+// Products of a few rows of activations with large weights for sm_100a, where
+// reading the weights once from HBM is the whole cost:
+//   Y = X W^T              W in 4 bits with group scales
+//   H = act(X Wg^T) * (X Wu^T)   both weights bf16, or both in 4 bits
+// X [M,K] bf16, at most 32 rows per CTA (blocks of 32 rows of X beyond that).
+//
+// 4-bit weights: W[n,k] = s[k / group, n] * (q[n,k] - 8), q in 0..15, two to a
+// byte (even k in the low four bits), s bf16.  q - 8 is exact in bf16, so
+// products of a group run on the tensor cores unscaled, summed in fp32, and
+// each group's sum is multiplied by its scale in fp32: no weight is rounded.
+//
+// Rows of W are the M side of mma.sync m16n8k16, rows of X its N side.
+// mma.sync, not tcgen05: 4-bit weights are expanded in registers, which
+// mma.sync reads directly where tcgen05 would want them written back to
+// shared memory first, and neither rate is near its limit here.  A CTA takes
+// 64 rows of W (plain) or 32 of Wg and the same 32 of Wu (gated) and a K range;
+// one warp streams them through a ring of 128-byte-swizzled TMA boxes, and 8
+// warps (2 x 32 rows, 4 interleaved quarters of every stage's K) consume it.
+// The sum over k may run in any order as long as both operands use the same
+// one, so a lane takes 8 consecutive k's of a row with a single load instead
+// of the fragment's scattered ones.  The 4 K quarters are added in shared
+// memory and, where N is too narrow to occupy every SM, the K ranges of a
+// cluster of up to 8 CTAs through distributed shared memory, always in the
+// same order.
+#pragma once
+
+#include <cstdint>
+#include <cuda.h>
+#include <cuda_bf16.h>
+
+#include "ffn_sm100.cuh"
+#include "gemm_sm100.cuh"
+
+namespace b200gemm {
+
+struct SkinnyParams {
+  int M, N, K;             // gated: N = F
+  int num_stages;          // ceil(K / stage K)
+  int stages_per_cta;      // of each CTA of a cluster
+  int act;                 // gated: kAct*
+  int out_type;            // kOutBf16 or kOutF32
+  int group_shift;         // log2 of the group (4-bit weights)
+  const uint16_t* scales0; // [K / group][N]: W, or Wg
+  const uint16_t* scales1; // Wu
+  void* out;
+  long long ldo;           // elements
+  unsigned int* status;
+  unsigned long long timeout_ns;
+  int pdl;
+};
+
+template <bool W4, bool GATED, int NT>
+struct SkinnyCfg {
+  static constexpr bool kW4 = W4;
+  static constexpr bool kGatedOut = GATED;
+  static constexpr int kNT = NT;                       // tiles of 8 rows of X
+  static constexpr int kTok = 8 * NT;
+  static constexpr int kRows = 64;                     // weight rows per CTA
+  static constexpr int kOutCols = GATED ? 32 : 64;     // output columns per CTA
+  static constexpr int kWarps = 8;                     // consumers
+  static constexpr int kThreads = 32 * (kWarps + 1);
+  static constexpr int kStageK = W4 ? 256 : 128;
+  static constexpr int kStageW = W4 ? kRows * 128 : 2 * kRows * 128;
+  static constexpr int kBoxX = kTok * 128;             // 64 k's of every row of X
+  static constexpr int kStageX = kStageK / 64 * kBoxX;
+  static constexpr int kStageBytes = kStageW + kStageX;
+  // About 96 KB of ring, so that two CTAs share an SM and one's prologue and
+  // reduction overlap the other's streaming.
+  static constexpr int kStages = 98304 / kStageBytes;
+  static constexpr int kW = 0;
+  static constexpr int kX = kW + kStages * kStageW;
+  static constexpr int kScale = kX + kStages * kStageX;
+  static constexpr int kScaleGroups = W4 ? 120 : 0;    // groups whose scales are held at once
+  static constexpr int kFull = kScale + kScaleGroups * kRows * 2;
+  static constexpr int kEmpty = kFull + 8 * kStages;
+  static constexpr int kAbort = kEmpty + 8 * kStages;
+  static constexpr int kEnd = kAbort + 8;
+  static constexpr int kSmemBytes = kEnd + 1024;
+  // Sums, in the ring once it is drained: [4 K quarters][kTok][72], then the
+  // CTA's own [kTok][72] (72: a lane group's 4 tokens x 8 rows fall into 32
+  // different banks).
+  static constexpr int kPitch = 72;
+  static constexpr int kRed = 0;
+  static constexpr int kPart = kRed + 4 * kTok * kPitch * 4;
+  static_assert(kPart + kTok * kPitch * 4 <= kScale, "sums alias the ring");
+  static_assert(kStages >= 3 && kStages <= 16 && kSmemBytes <= 115712, "two CTAs per SM");
+};
+
+__device__ __forceinline__ void mma_m16n8k16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                             uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t ld_shared_u32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+__device__ __forceinline__ float ld_cluster_f32(uint32_t cluster_addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
+  return v;
+}
+
+// Eight codes of a word -> four bf16 pairs of q - 8: pair j holds codes j and
+// j + 4.  0x4300 is 128 with a spacing of 1, so or-ing a code in gives
+// 128 + q; 136 is subtracted, exactly.
+__device__ __forceinline__ void w4_expand(uint32_t w, uint32_t (&v)[4]) {
+  const __nv_bfloat162 bias = __halves2bfloat162(__ushort_as_bfloat16(0x4308), __ushort_as_bfloat16(0x4308));
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t x = ((w >> (4 * j)) & 0x000F000Fu) | 0x43004300u;
+    const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&x), bias);
+    v[j] = *reinterpret_cast<const uint32_t*>(&d);
+  }
+}
+
+template <class Cfg>
+__global__ void __launch_bounds__(Cfg::kThreads, 2)
+    skinny_sm100(const __grid_constant__ CUtensorMap map_w0, const __grid_constant__ CUtensorMap map_w1,
+                 const __grid_constant__ CUtensorMap map_x, const SkinnyParams p) {
+  constexpr int NT = Cfg::kNT;
+  constexpr int STAGES = Cfg::kStages;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const uint32_t base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+  const uint32_t full0 = base + Cfg::kFull, empty0 = base + Cfg::kEmpty;
+  const int split = static_cast<int>(gridDim.x);   // CTAs of this cluster: K ranges
+  const int rank = static_cast<int>(blockIdx.x);
+  const int n0 = static_cast<int>(blockIdx.y) * Cfg::kOutCols;
+  const int m0 = static_cast<int>(blockIdx.z) * 32;
+  const int s_begin = rank * p.stages_per_cta;
+  const int count = max(0, min(p.num_stages, s_begin + p.stages_per_cta) - s_begin);
+
+  ptx::Watchdog wd;
+  wd.abort_flag = base + Cfg::kAbort;
+  wd.peer_abort_flag = ptx::mapa(wd.abort_flag, split > 1 ? static_cast<uint32_t>(rank ^ 1) : 0u);
+  wd.status = p.status;
+  wd.timeout_ns = p.timeout_ns;
+
+  if (threadIdx.x == 0) {
+    asm volatile("st.shared.u32 [%0], 0;" ::"r"(wd.abort_flag) : "memory");
+    for (int s = 0; s < STAGES; ++s) {
+      ptx::mbar_init(full0 + 8 * s, 1);
+      ptx::mbar_init(empty0 + 8 * s, Cfg::kWarps);
+    }
+    ptx::fence_mbar_init_cluster();
+    ptx::prefetch_tensormap(&map_w0);
+    ptx::prefetch_tensormap(&map_x);
+    if (Cfg::kGatedOut) ptx::prefetch_tensormap(&map_w1);
+  }
+  ptx::cluster_sync_all();
+
+  // acc[i][j]: rows 16 i .. of this warp's 32, tokens 8 j ..
+  float acc[2][NT][4];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) acc[i][j][c] = 0.0f;
+  // Fragment row (or column) g of 8 stands for row tok(g), so that the 8
+  // lanes of a 16-byte access phase (two rows, 4 chunks each) hit all 8 chunk
+  // places of the 128-byte swizzle.
+  const uint32_t g = lane >> 2, t = lane & 3u;
+  const uint32_t tokg = (g >> 1) | ((g & 1u) << 2);
+  const uint32_t rw = warp & 1u, wk = warp >> 1;
+
+  if (warp == Cfg::kWarps) {
+    // ------------------------------------------------------------ producer
+    if (lane == 0) {
+      const uint64_t policy_w = ptx::policy_evict_first();  // read once (per 32 rows of X)
+      const uint64_t policy_x = ptx::policy_evict_last();   // read by every CTA
+      if (p.pdl != kPdlWeightsEarly) ptx::griddep_wait();
+      auto load_w = [&](int it, int s) {
+        const uint32_t bar = full0 + 8 * s, dst = base + Cfg::kW + s * Cfg::kStageW;
+        ptx::mbar_arrive_expect_tx(bar, Cfg::kStageBytes);
+#pragma unroll
+        for (int b = 0; b < (Cfg::kW4 ? 1 : 2); ++b) {
+          // x counts elements of the map: bytes (two codes) or bf16
+          const int x = Cfg::kW4 ? (s_begin + it) * 128 : (s_begin + it) * 128 + b * 64;
+          const uint32_t d = dst + b * Cfg::kRows * 128;
+          ptx::tma_load_2d(d, &map_w0, bar, x, n0, policy_w);
+          if (Cfg::kGatedOut) ptx::tma_load_2d(d + 32 * 128, &map_w1, bar, x, n0, policy_w);
+        }
+      };
+      auto load_x = [&](int it, int s) {
+#pragma unroll
+        for (int b = 0; b < Cfg::kStageK / 64; ++b)
+          ptx::tma_load_2d(base + Cfg::kX + s * Cfg::kStageX + b * Cfg::kBoxX, &map_x, full0 + 8 * s,
+                           (s_begin + it) * Cfg::kStageK + b * 64, m0, policy_x);
+      };
+      const int pre = min(STAGES, count);
+      for (int it = 0; it < pre; ++it) load_w(it, it);
+      if (p.pdl == kPdlWeightsEarly) ptx::griddep_wait();
+      for (int it = 0; it < pre; ++it) load_x(it, it);
+      uint32_t stage = 0, phase = 1;  // after a whole ring
+      for (int it = pre; it < count; ++it) {
+        if (!ptx::mbar_wait(empty0 + 8 * stage, phase ^ 1u, wd, kSiteProducer, blockIdx.y)) break;
+        load_w(it, static_cast<int>(stage));
+        load_x(it, static_cast<int>(stage));
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+    __syncwarp();
+  } else {
+    // ----------------------------------------------------------- consumers
+    uint32_t stage = 0, phase = 0;
+    [[maybe_unused]] int win = 0, win_end = -1;  // groups whose scales are in shared memory
+    if (p.pdl != kPdlWeightsEarly) ptx::griddep_wait();
+    for (int it = 0; it < count; ++it) {
+      if constexpr (Cfg::kW4) {
+        // Scales of the stage's groups: [group][row half][tok][row / 8], so a
+        // lane's four rows are 8 bytes.
+        const int first = ((s_begin + it) * 256) >> p.group_shift;
+        const int last = ((s_begin + it) * 256 + 255) >> p.group_shift;
+        if (last > win_end) {
+          const int groups = p.K >> p.group_shift;
+          const int range_last = min(groups - 1, ((s_begin + count) * 256 - 1) >> p.group_shift);
+          win = first;
+          win_end = max(last, min(range_last, win + Cfg::kScaleGroups - 1));
+          if (it > 0) ptx::named_barrier(1, 32 * Cfg::kWarps);  // the old ones are no longer read
+          const int r = static_cast<int>(threadIdx.x & 63u);    // weight row of the CTA
+          const bool up = Cfg::kGatedOut && r >= 32;
+          const int n = n0 + (Cfg::kGatedOut ? (r & 31) : r);
+          const uint16_t* src = (up ? p.scales1 : p.scales0) + n;
+          const uint32_t dst =
+              base + Cfg::kScale + static_cast<uint32_t>((r >> 5) * 32 + (r & 7) * 4 + ((r >> 3) & 3)) * 2u;
+#pragma unroll 8
+          for (int q = win + static_cast<int>(threadIdx.x >> 6); q <= win_end; q += 4) {
+            const uint16_t v = (n < p.N && q < groups) ? __ldg(src + static_cast<long long>(q) * p.N) : 0;
+            ptx::st_shared_u16(dst + static_cast<uint32_t>(q - win) * 128u, v);
+          }
+          ptx::named_barrier(1, 32 * Cfg::kWarps);
+        }
+      }
+      const bool got = ptx::mbar_wait(full0 + 8 * stage, phase, wd, kSiteEpilogue, blockIdx.y);
+      if (__all_sync(0xFFFFFFFFu, got)) {
+        const uint32_t sw = base + Cfg::kW + stage * Cfg::kStageW;
+        const uint32_t sx = base + Cfg::kX + stage * Cfg::kStageX;
+        // X's 8 k's of this lane for every tile of tokens: 32-k chunk q.
+        auto load_x = [&](uint32_t q, uint32_t (&x)[NT][4]) {
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            const uint32_t a = sx + (q >> 1) * Cfg::kBoxX + (j * 8u + tokg) * 128u + ((((q & 1u) << 2) | t) ^ tokg) * 16u;
+            ptx::ld_shared_v4(a, x[j][0], x[j][1], x[j][2], x[j][3]);
+          }
+        };
+        if constexpr (Cfg::kW4) {
+          float sum[2][NT][4];
+#pragma unroll
+          for (int qq = 0; qq < 2; ++qq) {
+            const uint32_t q = 2u * wk + qq;
+            // a group of 64 or more holds both of this warp's chunks
+            const bool fresh = qq == 0 || p.group_shift == 5;
+            if (fresh) {
+#pragma unroll
+              for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                  for (int c = 0; c < 4; ++c) sum[i][j][c] = 0.0f;
+            }
+            uint32_t x[NT][4];
+            load_x(q, x);
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+              // pairs (k_j, k_j+4), as w4_expand gives the weights
+              const uint32_t x0 = x[j][0], x1 = x[j][1], x2 = x[j][2], x3 = x[j][3];
+              x[j][0] = __byte_perm(x0, x2, 0x5410);
+              x[j][1] = __byte_perm(x0, x2, 0x7632);
+              x[j][2] = __byte_perm(x1, x3, 0x5410);
+              x[j][3] = __byte_perm(x1, x3, 0x7632);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const uint32_t row = rw * 32u + i * 16u + tokg;
+              const uint32_t a = sw + row * 128u + ((q ^ tokg) << 4) + t * 4u;
+              uint32_t lo[4], hi[4];
+              w4_expand(ld_shared_u32(a), lo);
+              w4_expand(ld_shared_u32(a + 8u * 128u), hi);
+#pragma unroll
+              for (int j = 0; j < NT; ++j) {
+                mma_m16n8k16(sum[i][j], lo[0], hi[0], lo[1], hi[1], x[j][0], x[j][1]);
+                mma_m16n8k16(sum[i][j], lo[2], hi[2], lo[3], hi[3], x[j][2], x[j][3]);
+              }
+            }
+            if (qq == 1 || p.group_shift == 5) {
+              const int grp = ((s_begin + it) * 256 + static_cast<int>(q) * 32) >> p.group_shift;
+              const uint32_t a = base + Cfg::kScale + static_cast<uint32_t>(grp - win) * 128u + rw * 64u + tokg * 8u;
+              const uint32_t s01 = ld_shared_u32(a), s23 = ld_shared_u32(a + 4u);
+              const float s[4] = {bf16_lo(s01), bf16_hi(s01), bf16_lo(s23), bf16_hi(s23)};
+#pragma unroll
+              for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                  for (int c = 0; c < 4; ++c) acc[i][j][c] = fmaf(s[2 * i + (c >> 1)], sum[i][j][c], acc[i][j][c]);
+            }
+          }
+        } else {
+          uint32_t x[NT][4];
+          load_x(wk, x);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t row = rw * 32u + i * 16u + tokg;
+            const uint32_t a = sw + (wk >> 1) * (Cfg::kRows * 128u) + row * 128u + ((((wk & 1u) << 2) | t) ^ tokg) * 16u;
+            uint32_t lo[4], hi[4];
+            ptx::ld_shared_v4(a, lo[0], lo[1], lo[2], lo[3]);
+            ptx::ld_shared_v4(a + 8u * 128u, hi[0], hi[1], hi[2], hi[3]);
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+              mma_m16n8k16(acc[i][j], lo[0], hi[0], lo[1], hi[1], x[j][0], x[j][1]);
+              mma_m16n8k16(acc[i][j], lo[2], hi[2], lo[3], hi[3], x[j][2], x[j][3]);
+            }
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive_cluster(ptx::mapa(empty0 + 8 * stage, static_cast<uint32_t>(split > 1 ? rank : 0)));
+      if (++stage == STAGES) {
+        stage = 0;
+        phase ^= 1u;
+      }
+    }
+    // ------------------------------------------- the CTA's sum over its K range
+    ptx::named_barrier(1, 32 * Cfg::kWarps);  // the ring is drained
+    auto* red = reinterpret_cast<float*>(smem_raw + (base - ptx::smem_u32(smem_raw)) + Cfg::kRed);
+    auto* part = reinterpret_cast<float*>(smem_raw + (base - ptx::smem_u32(smem_raw)) + Cfg::kPart);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          // column 2t + b of the fragment is token tok(2t + b) = t + 4b
+          const uint32_t tok = j * 8u + t + 4u * (c & 1), row = rw * 32u + i * 16u + 8u * (c >> 1) + tokg;
+          red[(wk * Cfg::kTok + tok) * Cfg::kPitch + row] = acc[i][j][c];
+        }
+    ptx::named_barrier(1, 32 * Cfg::kWarps);
+#pragma unroll
+    for (int idx = static_cast<int>(threadIdx.x); idx < Cfg::kTok * 64; idx += 32 * Cfg::kWarps) {
+      const int at = (idx >> 6) * Cfg::kPitch + (idx & 63);
+      float v = red[at];
+#pragma unroll
+      for (int w = 1; w < 4; ++w) v += red[w * Cfg::kTok * Cfg::kPitch + at];
+      part[at] = v;
+    }
+    __syncwarp();
+  }
+  ptx::cluster_sync_all();
+  ptx::griddep_launch_dependents();
+
+  // --------------------- the cluster's sum: each CTA finishes its own tokens
+  if (warp < Cfg::kWarps && !ptx::aborted(wd)) {
+    const uint32_t part0 = base + Cfg::kPart;
+    auto total = [&](int at) {
+      float v = ld_cluster_f32(ptx::mapa(part0 + at * 4u, 0));
+      for (int c = 1; c < split; ++c) v += ld_cluster_f32(ptx::mapa(part0 + at * 4u, static_cast<uint32_t>(c)));
+      return v;
+    };
+    constexpr int kCols = Cfg::kOutCols;
+    for (int idx = static_cast<int>(threadIdx.x) + 32 * Cfg::kWarps * rank; idx < Cfg::kTok * kCols;
+         idx += 32 * Cfg::kWarps * split) {
+      const int tok = idx / kCols, c = idx % kCols;
+      if (m0 + tok >= p.M || n0 + c >= p.N) continue;
+      float v = total(tok * Cfg::kPitch + c);
+      if constexpr (Cfg::kGatedOut) {
+        const float u = total(tok * Cfg::kPitch + 32 + c);
+        switch (p.act) {
+          case kActRelu: v = ffn_act<kActRelu>(v) * u; break;
+          case kActGelu: v = ffn_act<kActGelu>(v) * u; break;
+          case kActGeluTanh: v = ffn_act<kActGeluTanh>(v) * u; break;
+          case kActSilu: v = ffn_act<kActSilu>(v) * u; break;
+          default: v = v * u; break;
+        }
+      }
+      const long long off = static_cast<long long>(m0 + tok) * p.ldo + n0 + c;
+      if (p.out_type == kOutF32) static_cast<float*>(p.out)[off] = v;
+      else static_cast<__nv_bfloat16*>(p.out)[off] = __float2bfloat16_rn(v);
+    }
+  }
+  if (threadIdx.x == 0 && ptx::aborted(wd)) ptx::sleep_ns_bounded(200000ull);
+  __syncwarp();
+  ptx::cluster_sync_all();  // no CTA leaves while another reads its sums
+}
+
+// ------------------------------------------------- 4-bit weights and bf16
+// Per group of one row: s = bf16(max|w| / 7), q = clamp(rint(w / s), -8, 7) + 8
+// (8 where s is 0 or NaN, so a group with a NaN or infinity comes back as
+// NaN).  DRAM-bound.  A block takes 32 rows x 256 k's: a warp reads 256 k's of
+// a row, 16 bytes a lane, four rows in flight; a group's lanes find its
+// maximum by shuffles on the magnitude bits (which order NaN above all), and
+// the block's scales are written row-contiguously through shared memory.
+struct W4Params {
+  int N, K, group_shift;
+  uint16_t* w;           // [N, K], row pitch ldw
+  long long ldw;
+  uint8_t* codes;        // [N, K / 2]
+  uint16_t* scales;      // [K / group, N]
+};
+
+__global__ void __launch_bounds__(256) w4_quantize_kernel(const W4Params p) {
+  __shared__ uint16_t sc[8][32];
+  const int warp = static_cast<int>(threadIdx.x >> 5), lane = static_cast<int>(threadIdx.x & 31u);
+  const int k = static_cast<int>(blockIdx.x) * 256 + lane * 8;
+  const int n0 = static_cast<int>(blockIdx.y) * 32;
+  const int lanes = 1 << (p.group_shift - 3);  // per group: 4 .. 32
+  uint32_t w[4][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int n = n0 + warp + 8 * i;
+    w[i][0] = w[i][1] = w[i][2] = w[i][3] = 0u;
+    if (n < p.N && k < p.K)
+      ptx::ld_global_nc_v4(p.w + static_cast<long long>(n) * p.ldw + k, w[i][0], w[i][1], w[i][2], w[i][3]);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int n = n0 + warp + 8 * i;
+    uint32_t m2 = 0u;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) m2 = __vmaxu2(m2, w[i][j] & 0x7FFF7FFFu);
+    uint32_t m = max(m2 & 0xFFFFu, m2 >> 16);
+    for (int d = 1; d < lanes; d <<= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
+    const __nv_bfloat16 sb = __float2bfloat16_rn(__fdiv_rn(__uint_as_float(m << 16), 7.0f));
+    const float s = __bfloat162float(sb);
+    uint32_t code = 0u;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float x = (j & 1) ? bf16_hi(w[i][j >> 1]) : bf16_lo(w[i][j >> 1]);
+      int q = 0;
+      if (s > 0.0f) q = max(-8, min(7, __float2int_rn(__fdiv_rn(x, s))));  // (NaN converts to 0)
+      code |= static_cast<uint32_t>(q + 8) << (4 * j);
+    }
+    if (n < p.N && k < p.K) {
+      *reinterpret_cast<uint32_t*>(p.codes + static_cast<long long>(n) * (p.K / 2) + k / 2) = code;
+      if ((lane & (lanes - 1)) == 0) sc[lane >> (p.group_shift - 3)][warp + 8 * i] = __bfloat16_as_ushort(sb);
+    }
+  }
+  __syncthreads();
+  const int q = warp + (static_cast<int>(blockIdx.x) * 256 >> p.group_shift);
+  if (warp < (256 >> p.group_shift) && q < (p.K >> p.group_shift) && n0 + lane < p.N)
+    p.scales[static_cast<long long>(q) * p.N + n0 + lane] = sc[warp][lane];
+}
+
+// W[n,k] = bf16(s (q - 8)): the product is exact in fp32 and rounded once.
+// The same blocks; 4 bytes of codes and 16 of results per lane and row.
+__global__ void __launch_bounds__(256) w4_dequantize_kernel(const W4Params p) {
+  __shared__ uint16_t sc[8][32];
+  const int warp = static_cast<int>(threadIdx.x >> 5), lane = static_cast<int>(threadIdx.x & 31u);
+  const int k = static_cast<int>(blockIdx.x) * 256 + lane * 8;
+  const int n0 = static_cast<int>(blockIdx.y) * 32;
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int n = n0 + warp + 8 * i;
+    w[i] = 0u;
+    if (n < p.N && k < p.K)
+      w[i] = __ldg(reinterpret_cast<const uint32_t*>(p.codes + static_cast<long long>(n) * (p.K / 2) + k / 2));
+  }
+  const int q = warp + (static_cast<int>(blockIdx.x) * 256 >> p.group_shift);
+  if (warp < (256 >> p.group_shift) && q < (p.K >> p.group_shift) && n0 + lane < p.N)
+    sc[warp][lane] = __ldg(p.scales + static_cast<long long>(q) * p.N + n0 + lane);
+  __syncthreads();
+  if (k >= p.K) return;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int n = n0 + warp + 8 * i;
+    if (n >= p.N) continue;
+    const float s = __uint_as_float(static_cast<uint32_t>(sc[lane >> (p.group_shift - 3)][warp + 8 * i]) << 16);
+    uint32_t o[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float lo = s * static_cast<float>(static_cast<int>((w[i] >> (8 * j)) & 15u) - 8);
+      const float hi = s * static_cast<float>(static_cast<int>((w[i] >> (8 * j + 4)) & 15u) - 8);
+      o[j] = ptx::pack_bf16x2(__float_as_uint(lo), __float_as_uint(hi));
+    }
+    ptx::st_global_v4(p.w + static_cast<long long>(n) * p.ldw + k, o[0], o[1], o[2], o[3]);
+  }
+}
+
+}  // namespace b200gemm

@@ -298,6 +298,82 @@ int b200gemm_schedule_host(unsigned int tiles_m, unsigned int tiles_n, int order
 int b200gemm_bf16_nt_noalloc(int M, int N, int K, const void* A, const void* B, void* C, int ldc,
                              void* stream);
 
+/* ---------------------------------------------------------------------
+ * Feed-forward operators.  No counterpart in the reference.
+ *
+ * All matrices are row-major device memory on the handle's device; a row
+ * pitch (ld...) is in elements.  Every call is asynchronous on `stream`,
+ * allocates nothing, waits for nothing and can be captured into a CUDA graph.
+ * No output may overlap an input or another output (column slices of one
+ * wide matrix do not count as overlapping): B200GEMM_ERR_INVALID_ARG.
+ * ------------------------------------------------------------------- */
+
+/* Gated block, one kernel:  G = X Wg^T,  U = X Wu^T,  H = act(G) * U
+ *   X [M,K], Wg and Wu [F,K] (one pitch ldw), H [M,F], all bf16; fp32 sums,
+ *   H rounded once.  activation: B200GEMM_ACT_*.
+ * G and U, both or neither, receive the two products rounded to bf16 (one
+ * pitch ldgu): what b200gemm_bf16_gated_backward needs.  Any M and F;
+ * K % 8 == 0, K > 0; pitches % 8 == 0; every pointer 16-byte aligned.
+ * Up to 32 rows (without G and U) the weights are streamed by every SM; an
+ * element's sum then runs in another order than in the tiled kernel. */
+int b200gemm_bf16_gated(b200gemm_t handle, int M, int F, int K, const void* X, long long ldx,
+                        const void* Wg, const void* Wu, long long ldw, int activation, void* H,
+                        long long ldh, void* G, void* U, long long ldgu, void* stream);
+
+/* Bytes of workspace a b200gemm_bf16_gated_backward call of this size needs
+ * (dG and dU in bf16; 0 for an empty one). */
+unsigned long long b200gemm_gated_backward_workspace(int M, int F);
+
+/* Gradients of the gated block from dH [M,F], given X, Wg, Wu and the saved
+ * G and U (the bf16 values are taken as they are):
+ *   dU = dH * act(G), dG = dH * U * act'(G)     rounded to bf16, workspace
+ *   dX = dG Wg + dU Wu                          [M,K], pitch lddx
+ *   dWg = dG^T X, dWu = dU^T X                  [F,K], pitch lddw
+ * with fp32 sums, each result rounded to bf16 once.  dX may be NULL, and so
+ * may dWg and dWu together: those are then not computed.  With M == 0 the
+ * weight gradients are zeros, with F == 0 dX is.  act'(0) of relu is 0.
+ * workspace: 16-byte aligned, its contents before and after mean nothing; it
+ * is in use until the call's work on `stream` is done.  The same rules as
+ * b200gemm_bf16_gated otherwise. */
+int b200gemm_bf16_gated_backward(b200gemm_t handle, int M, int F, int K, const void* dH,
+                                 long long lddh, const void* X, long long ldx, const void* Wg,
+                                 const void* Wu, long long ldw, const void* G, const void* U,
+                                 long long ldgu, int activation, void* dX, long long lddx,
+                                 void* dWg, void* dWu, long long lddw, void* workspace,
+                                 void* stream);
+
+/* 4-bit weights: W[n][k] = scales[k / group][n] * (q[n][k] - 8), q in 0..15.
+ *   codes   [N][K / 2] bytes, contiguous, 16-byte aligned: byte b of a row
+ *           holds q[2b] in its low and q[2b + 1] in its high four bits
+ *   scales  bf16 [K / group][N], contiguous
+ *   group   32, 64, 128 or 256, a divisor of K
+ *
+ * b200gemm_w4_quantize: from bf16 W [N,K] (pitch ldw % 8 == 0, 16-byte
+ * aligned), per group of a row s = bf16(max|w| / 7), q = clamp(rint(w / s),
+ * -8, 7) + 8 (rint: ties to even; q = 8 where s is 0).  A group that holds a
+ * NaN or an infinity comes back as NaN.
+ * b200gemm_w4_dequantize: W = bf16(s * (q - 8)). */
+int b200gemm_w4_quantize(b200gemm_t handle, int N, int K, const void* W, long long ldw, int group,
+                         void* codes, void* scales, void* stream);
+int b200gemm_w4_dequantize(b200gemm_t handle, int N, int K, const void* codes, const void* scales,
+                           int group, void* W, long long ldw, void* stream);
+
+/* C = A W^T for 4-bit W: A [M,K] bf16 (lda % 8 == 0, 16-byte aligned), C
+ * [M,N] bf16 or fp32 (out_type B200GEMM_OUT_BF16 or _F32), ldc >= N, aligned
+ * to its elements.  No weight is rounded: the products of a group are summed
+ * unscaled in fp32 and the sum is scaled in fp32.  Made for a few rows (the
+ * weights are read once per 32 rows of A); any M works. */
+int b200gemm_w4_nt(b200gemm_t handle, int M, int N, int K, const void* A, long long lda,
+                   const void* codes, const void* scales, int group, void* C, long long ldc,
+                   int out_type, void* stream);
+
+/* H = act(X Wg^T) * (X Wu^T) for 4-bit Wg and Wu [F,K] of one group size, H
+ * bf16 [M,F], ldh >= F; X as A above. */
+int b200gemm_w4_gated(b200gemm_t handle, int M, int F, int K, const void* X, long long ldx,
+                      const void* gate_codes, const void* gate_scales, const void* up_codes,
+                      const void* up_scales, int group, int activation, void* H, long long ldh,
+                      void* stream);
+
 /* Human-readable text for a status code (static storage). */
 const char* b200gemm_strerror(int code);
 

@@ -1,0 +1,227 @@
+"""4-bit weights (Gemm.w4_quantize, w4_dequantize, w4_nt, w4_gated) on the GPU
+against 64-bit forms, with the bounds derived in ffn_plain.py."""
+import pytest
+
+from b200_gemm_b200 import _lib
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+import ffn_plain as plain  # noqa: E402
+
+BF = torch.bfloat16
+
+
+def _w4_product(x, codes, scales):
+    w = plain.w4_values(codes, scales)
+    x = x.double()
+    # the sum's steps, and one more rounding per 32 k's where a group's sum is scaled and added
+    err = (plain.sum_err(x.shape[1]) + (x.shape[1] / 32 + 8) * 2.0 ** -23) * (x.abs() @ w.abs().t())
+    return x @ w.t(), err
+
+
+def _check_nt(h, M, N, K, group, dtype=BF, seed=0, pad=0):
+    x = plain.rows(M, K, seed, pad=pad)
+    codes, scales = plain.w4_random(N, K, group, seed + 1)
+    buf = torch.full((M + 2, N + 3), 7.0, dtype=dtype, device="cuda")
+    out = buf[:M, :N]
+    h.w4_nt(x, codes, scales, out=out)
+    assert h.last_device_status()[0] == 0
+    ref, err = _w4_product(x, codes, scales)
+    plain.close(out, ref, err, plain.BF16 if dtype == BF else plain.F32)
+    assert (buf[M:] == 7.0).all() and (buf[:, N:] == 7.0).all()
+
+
+@pytest.mark.parametrize("group", [32, 64, 128, 256])
+@pytest.mark.parametrize("M,N,groups", [(1, 1, 1), (1, 64, 3), (2, 65, 5), (8, 130, 8), (9, 63, 9), (16, 200, 2),
+                                        (17, 64, 7), (32, 257, 4), (33, 96, 3), (100, 70, 4)])
+def test_nt(gpu_handle, M, N, groups, group):
+    _check_nt(gpu_handle, M, N, groups * group, group, seed=M + N)
+
+
+@pytest.mark.parametrize("M", [1, 12, 32])
+def test_nt_f32(gpu_handle, M):
+    _check_nt(gpu_handle, M, 200, 1024, 64, dtype=torch.float32, seed=M)
+
+
+@pytest.mark.parametrize("M,N,K,group", [(1, 40, 16384, 32), (5, 3000, 8192, 128), (1, 10000, 512, 32),
+                                         (30, 12000, 256, 256), (2, 100, 16416, 32)])
+def test_nt_long(gpu_handle, M, N, K, group):
+    """Long sums (K split over a cluster, more groups than are held at once),
+    many rows of weights."""
+    _check_nt(gpu_handle, M, N, K, group, seed=K, pad=16)
+
+
+@pytest.mark.parametrize("kind", plain.ACTS)
+@pytest.mark.parametrize("M,F,K,group", [(1, 33, 96, 32), (7, 100, 512, 128), (20, 1001, 320, 64), (64, 40, 256, 256)])
+def test_gated(gpu_handle, M, F, K, group, kind):
+    x = plain.rows(M, K, 1, pad=8)
+    gate, up = plain.w4_random(F, K, group, 2), plain.w4_random(F, K, group, 3)
+    buf = torch.full((M + 2, F + 1), 7.0, dtype=BF, device="cuda")
+    gpu_handle.w4_gated(x, *gate, *up, activation=kind, out=buf[:M, :F])
+    assert gpu_handle.last_device_status()[0] == 0
+    g, eg = _w4_product(x, *gate)
+    u, eu = _w4_product(x, *up)
+    plain.close(buf[:M, :F], *plain.gated(g, eg, u, eu, kind))
+    assert (buf[M:] == 7.0).all() and (buf[:, F:] == 7.0).all()
+
+
+@pytest.mark.parametrize("group", [32, 64, 128, 256])
+@pytest.mark.parametrize("N,groups", [(1, 1), (31, 3), (33, 9), (200, 17)])
+def test_quantize_and_back(gpu_handle, N, groups, group):
+    """Codes and scales equal the definition's, and the values are the scaled
+    codes rounded once."""
+    K = groups * group
+    w = plain.rows(N, K, N + K, K ** -0.5, pad=8)
+    w[0, :group] = 0  # a group of zeros
+    w[-1, -1] = 100.0
+    codes, scales = gpu_handle.w4_quantize(w, group)
+    ref_codes, ref_scales = plain.w4_quantize(w.cpu(), group)
+    assert torch.equal(codes.cpu(), ref_codes)
+    assert torch.equal(scales.cpu(), ref_scales)
+    buf = torch.full((N + 1, K + 8), 7.0, dtype=BF, device="cuda")
+    gpu_handle.w4_dequantize(codes, scales, out=buf[:N, :K])
+    assert torch.equal(buf[:N, :K].cpu(), plain.w4_values(ref_codes, ref_scales).to(BF))
+    assert (buf[N:] == 7.0).all() and (buf[:, K:] == 7.0).all()
+
+
+def test_quantize_ties_and_tiny(gpu_handle):
+    """w / s half way between two codes goes to the even one; scales among the
+    subnormals; a scale that rounds to zero."""
+    w = torch.zeros(4, 32, dtype=BF)
+    w[0] = torch.tensor([7.0] + [v + 0.5 for v in range(-7, 7)] * 2 + [0.0, 1.0, 2.0])
+    w[1] = torch.linspace(-1, 1, 32) * 2.0 ** -128
+    w[2] = torch.linspace(-1, 1, 32) * 2.0 ** -132
+    w[3, 0] = 2.0 ** -133                       # s = 2^-133 / 7 rounds to 0
+    codes, scales = gpu_handle.w4_quantize(w.cuda(), 32)
+    ref_codes, ref_scales = plain.w4_quantize(w, 32)
+    assert torch.equal(scales.cpu(), ref_scales) and float(scales[0, 3]) == 0.0
+    assert torch.equal(codes.cpu(), ref_codes)
+
+
+def test_bad_groups_come_back_as_nan(gpu_handle):
+    w = plain.rows(3, 128, 0)
+    w[0, 3] = float("nan")
+    w[1, 70] = float("inf")
+    codes, scales = gpu_handle.w4_quantize(w, 64)
+    v = gpu_handle.w4_dequantize(codes, scales)
+    assert v[0, :64].isnan().all() and v[1, 64:].isnan().all()
+    assert v[0, 64:].isfinite().all() and v[1, :64].isfinite().all() and v[2].isfinite().all()
+    y = gpu_handle.w4_nt(plain.rows(2, 128, 1), codes, scales)
+    assert y[:, :2].isnan().all() and y[:, 2].isfinite().all()
+
+
+def test_bad_rows_stay_alone(gpu_handle):
+    x = plain.rows(6, 256, 1)
+    codes, scales = plain.w4_random(80, 256, 64, 2)
+    ref = gpu_handle.w4_nt(x, codes, scales)
+    y = x.clone()
+    y[2, 9] = float("nan")
+    y[4, 0] = float("inf")
+    got = gpu_handle.w4_nt(y, codes, scales)
+    keep = [0, 1, 3, 5]
+    assert torch.equal(got[keep], ref[keep]) and got[2].isnan().all() and not got[4].isfinite().any()
+
+
+def test_block_as_it_is_served(gpu_handle):
+    """A trained block quantised, then decoded: gated and down projection on 4
+    bits against the bf16 kernels on the dequantised weights.
+
+    The two differ by roundings alone: each side's H by its sums' bounds and
+    one rounding, carried through the down projection, and its own."""
+    h = gpu_handle
+    M, D, F = 3, 256, 320
+    x = plain.rows(M, D, 0)
+    wg, wu, wd = plain.rows(F, D, 1, D ** -0.5), plain.rows(F, D, 2, D ** -0.5), plain.rows(D, F, 3, F ** -0.5)
+    q = [h.w4_quantize(w, 32) for w in (wg, wu, wd)]
+    H = h.w4_gated(x, *q[0], *q[1])
+    y = h.w4_nt(H, *q[2])
+    g, eg = _w4_product(x, *q[0])
+    u, eu = _w4_product(x, *q[1])
+    r, er = plain.gated(g, eg, u, eu, "silu")
+    plain.close(H, r, er)
+    ref, err = _w4_product(H, *q[2])
+    plain.close(y, ref, err)
+    # prefill: the values back as bf16 (rounded: 2^-8 each) through the bf16 kernels
+    d = [h.w4_dequantize(*p) for p in q]
+    Hb = h.gated(x, d[0], d[1])
+    g2, eg2 = plain.product(x, d[0])
+    u2, eu2 = plain.product(x, d[1])
+    plain.close(Hb, *plain.gated(g2, eg2, u2, eu2, "silu"))
+
+
+def test_streams_graphs_and_overlap(gpu_handle):
+    h = gpu_handle
+    x = plain.rows(2, 1024, 0)
+    gate, up, down = (plain.w4_random(1024, 1024, 128, s) for s in (1, 2, 3))
+
+    def step(stream=None):
+        y = x
+        for _ in range(3):
+            y = h.w4_nt(h.w4_gated(y, *gate, *up, activation="silu", stream=stream), *down, stream=stream)
+            y = y.clamp(-4, 4) if stream is None else y
+        return y
+
+    def chain(stream=None):
+        y = x
+        for _ in range(4):
+            y = h.w4_nt(y, *down, stream=stream)
+        return y
+
+    ref, cref = step(), chain()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    got = chain(side)
+    torch.cuda.synchronize()
+    assert torch.equal(got, cref)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for _ in range(3):
+        out.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, ref)
+    del graph
+    for mode in (_lib.PDL_ON, _lib.PDL_WEIGHTS_EARLY):
+        h.set_pdl(mode)
+        try:
+            for _ in range(10):
+                assert torch.equal(chain(), cref)
+        finally:
+            h.set_pdl(_lib.PDL_OFF)
+
+
+def test_refusals(gpu_handle):
+    h = gpu_handle
+    x = plain.rows(2, 128, 0)
+    codes, scales = plain.w4_random(64, 128, 32, 1)
+    e = lambda *s, t=BF: torch.empty(*s, dtype=t, device="cuda")  # noqa: E731
+    with pytest.raises(ValueError):
+        h.w4_quantize(plain.rows(4, 96, 0), 64)           # 64 does not divide 96
+    with pytest.raises(ValueError):
+        h.w4_quantize(plain.rows(4, 96, 0), 48)
+    with pytest.raises(TypeError):
+        h.w4_nt(x, codes.to(torch.int8), scales)
+    with pytest.raises(TypeError):
+        h.w4_nt(x, codes, scales.float())
+    with pytest.raises(ValueError):
+        h.w4_nt(x, codes, scales[:3])
+    with pytest.raises(ValueError):
+        h.w4_nt(x, codes, scales.t().contiguous().t())
+    with pytest.raises(ValueError):
+        h.w4_nt(x[:, :64], codes, scales)
+    with pytest.raises(ValueError):
+        h.w4_nt(x, codes.cpu(), scales.cpu())
+    with pytest.raises(TypeError):
+        h.w4_nt(x, codes, scales, out_dtype=torch.float16)
+    with pytest.raises(ValueError):
+        h.w4_gated(x, codes, scales, *plain.w4_random(64, 128, 64, 1))
+    with pytest.raises(ValueError):
+        h.w4_gated(x, codes, scales, *plain.w4_random(32, 128, 32, 1))
+    with pytest.raises(_lib.B200GemmError) as err:
+        h.w4_nt(x, codes, scales, out=x[:, :64])          # writes over A
+    assert err.value.code == _lib.ERR_INVALID_ARG
+    assert h.w4_nt(e(0, 128), codes, scales).shape == (0, 64)
+    assert h.w4_dequantize(e(0, 64, t=torch.uint8), e(4, 0)).shape == (0, 128)
