@@ -169,6 +169,39 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const W
   }
 }
 
+// The forms of arrive and wait for a barrier that this CTA alone uses: at CTA
+// scope, without the cluster-wide fence that the ones above imply.
+__device__ __forceinline__ void mbar_arrive_cta(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool mbar_try_wait_cta(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool mbar_wait_cta(uint32_t bar, uint32_t parity, const Watchdog& wd,
+                                              unsigned int site, unsigned int tile) {
+  if (mbar_try_wait_cta(bar, parity)) return true;
+  const uint64_t t0 = globaltimer_ns();
+  const uint64_t max_iters = (wd.timeout_ns >> 2) + 1024;
+  for (uint64_t it = 1;; ++it) {
+    if (mbar_try_wait_cta(bar, parity)) return true;
+    if ((it & 7) == 0) {
+      if (aborted(wd)) return false;
+      if (globaltimer_ns() - t0 > wd.timeout_ns || it > max_iters) {
+        raise_abort(wd, site, tile);
+        return false;
+      }
+    }
+  }
+}
+
 // Bounded wait that ignores the abort word: used at teardown to wait for
 // work this thread itself issued (e.g. MMAs still reading shared memory).
 __device__ __forceinline__ bool mbar_wait_drain(uint32_t bar, uint32_t parity, const Watchdog& wd,

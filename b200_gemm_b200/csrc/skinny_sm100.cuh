@@ -14,14 +14,15 @@
 // mma.sync reads directly where tcgen05 would want them written back to
 // shared memory first, and neither rate is near its limit here.  A CTA takes
 // 64 rows of W (plain) or 32 of Wg and the same 32 of Wu (gated) and a K range;
-// one warp streams them through a ring of 128-byte-swizzled TMA boxes, and 8
-// warps (2 x 32 rows, 4 interleaved quarters of every stage's K) consume it.
-// The sum over k may run in any order as long as both operands use the same
-// one, so a lane takes 8 consecutive k's of a row with a single load instead
-// of the fragment's scattered ones.  The 4 K quarters are added in shared
-// memory and, where N is too narrow to occupy every SM, the K ranges of a
-// cluster of up to 8 CTAs through distributed shared memory, always in the
-// same order.
+// streams them through a ring of 128-byte-swizzled TMA boxes, of which its 4
+// warps take whole stages in turn.  A stage has one reader, so the warp that
+// has read it refills it itself: there is no producer warp and no second
+// barrier to say that a stage is free.  The sum over k may run in any order as long as both operands use
+// the same one, so a lane takes 8 consecutive k's of a row with a single load
+// instead of the fragment's scattered ones.  The 4 warps' sums are added in
+// shared memory and, where N is too narrow to occupy every SM, those of the
+// K ranges of a cluster of up to 8 CTAs through distributed shared memory,
+// always in the same order.
 #pragma once
 
 #include <cstdint>
@@ -57,33 +58,37 @@ struct SkinnyCfg {
   static constexpr int kTok = 8 * NT;
   static constexpr int kRows = 64;                     // weight rows per CTA
   static constexpr int kOutCols = GATED ? 32 : 64;     // output columns per CTA
-  static constexpr int kWarps = 8;                     // consumers
-  static constexpr int kThreads = 32 * (kWarps + 1);
-  static constexpr int kStageK = W4 ? 256 : 128;
-  static constexpr int kStageW = W4 ? kRows * 128 : 2 * kRows * 128;
+  static constexpr int kWarps = 4;
+  static constexpr int kThreads = 32 * kWarps;
+  static constexpr int kStageK = W4 ? 256 : 64;        // 128 bytes of a weight row
+  static constexpr int kChunks = kStageK / 32;         // 32 k's each
+  static constexpr int kStageW = kRows * 128;
   static constexpr int kBoxX = kTok * 128;             // 64 k's of every row of X
   static constexpr int kStageX = kStageK / 64 * kBoxX;
   static constexpr int kStageBytes = kStageW + kStageX;
-  // About 96 KB of ring, so that two CTAs share an SM and one's prologue and
-  // reduction overlap the other's streaming.
-  static constexpr int kStages = 98304 / kStageBytes;
+  // CTAs per SM and a ring that fits that often: small CTAs, so that all of
+  // a launch's are resident at once and share HBM evenly.  (NT = 4 needs its
+  // registers, and 24 KB stages for 4-bit weights.)
+  static constexpr int kCtas = NT == 4 ? 2 : (W4 && NT == 2 ? 3 : 4);
+  // A multiple of the warps, so that a stage has the same reader every time
+  // around and that reader waits for its fillings in order: a wait by parity
+  // for the filling after next would be satisfied before the next arrived.
+  static constexpr int kStages = (NT == 4 ? 98304 : (W4 && NT == 2 ? 73728 : 53248)) / kStageBytes / kWarps * kWarps;
   static constexpr int kW = 0;
   static constexpr int kX = kW + kStages * kStageW;
-  static constexpr int kScale = kX + kStages * kStageX;
-  static constexpr int kScaleGroups = W4 ? 120 : 0;    // groups whose scales are held at once
-  static constexpr int kFull = kScale + kScaleGroups * kRows * 2;
-  static constexpr int kEmpty = kFull + 8 * kStages;
-  static constexpr int kAbort = kEmpty + 8 * kStages;
+  static constexpr int kFull = kX + kStages * kStageX;
+  static constexpr int kAbort = kFull + 8 * kStages;
   static constexpr int kEnd = kAbort + 8;
   static constexpr int kSmemBytes = kEnd + 1024;
-  // Sums, in the ring once it is drained: [4 K quarters][kTok][72], then the
-  // CTA's own [kTok][72] (72: a lane group's 4 tokens x 8 rows fall into 32
+  // Sums, in the ring once it is drained: [4 warps][kTok][72], then the CTA's
+  // own [kTok][72] (72: a lane group's 4 tokens x 8 rows fall into 32
   // different banks).
   static constexpr int kPitch = 72;
   static constexpr int kRed = 0;
-  static constexpr int kPart = kRed + 4 * kTok * kPitch * 4;
-  static_assert(kPart + kTok * kPitch * 4 <= kScale, "sums alias the ring");
-  static_assert(kStages >= 3 && kStages <= 16 && kSmemBytes <= 115712, "two CTAs per SM");
+  static constexpr int kPart = kRed + kWarps * kTok * kPitch * 4;
+  static_assert(kPart + kTok * kPitch * 4 <= kFull, "sums alias the ring");
+  static_assert(kStages >= kWarps && kStages % kWarps == 0, "one reader per stage");
+  static_assert(kCtas * (kSmemBytes + 1024) <= 233472, "CTAs per SM");
 };
 
 __device__ __forceinline__ void mma_m16n8k16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -121,7 +126,7 @@ __device__ __forceinline__ void w4_expand(uint32_t w, uint32_t (&v)[4]) {
 }
 
 template <class Cfg>
-__global__ void __launch_bounds__(Cfg::kThreads, 2)
+__global__ void __launch_bounds__(Cfg::kThreads, Cfg::kCtas)
     skinny_sm100(const __grid_constant__ CUtensorMap map_w0, const __grid_constant__ CUtensorMap map_w1,
                  const __grid_constant__ CUtensorMap map_x, const SkinnyParams p) {
   constexpr int NT = Cfg::kNT;
@@ -129,7 +134,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 2)
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-  const uint32_t full0 = base + Cfg::kFull, empty0 = base + Cfg::kEmpty;
+  const uint32_t full0 = base + Cfg::kFull;
   const int split = static_cast<int>(gridDim.x);   // CTAs of this cluster: K ranges
   const int rank = static_cast<int>(blockIdx.x);
   const int n0 = static_cast<int>(blockIdx.y) * Cfg::kOutCols;
@@ -143,228 +148,202 @@ __global__ void __launch_bounds__(Cfg::kThreads, 2)
   wd.status = p.status;
   wd.timeout_ns = p.timeout_ns;
 
+  auto load_w = [&](int it, int s) {
+    const uint32_t bar = full0 + 8 * s, dst = base + Cfg::kW + s * Cfg::kStageW;
+    const int x = (s_begin + it) * (Cfg::kW4 ? 128 : 64);  // elements of the map: bytes (two codes) or bf16
+    ptx::mbar_arrive_expect_tx(bar, Cfg::kStageBytes);
+    ptx::tma_load_2d(dst, &map_w0, bar, x, n0, ptx::policy_evict_first());  // read once (per 32 rows of X)
+    if (Cfg::kGatedOut) ptx::tma_load_2d(dst + 32 * 128, &map_w1, bar, x, n0, ptx::policy_evict_first());
+  };
+  auto load_x = [&](int it, int s) {
+#pragma unroll
+    for (int b = 0; b < Cfg::kStageK / 64; ++b)
+      ptx::tma_load_2d(base + Cfg::kX + s * Cfg::kStageX + b * Cfg::kBoxX, &map_x, full0 + 8 * s,
+                       (s_begin + it) * Cfg::kStageK + b * 64, m0, ptx::policy_evict_last());  // read by every CTA
+  };
+  const int pre = min(STAGES, count);
   if (threadIdx.x == 0) {
+    // The first ring is on its way before the other warps pass the barrier.
     asm volatile("st.shared.u32 [%0], 0;" ::"r"(wd.abort_flag) : "memory");
-    for (int s = 0; s < STAGES; ++s) {
-      ptx::mbar_init(full0 + 8 * s, 1);
-      ptx::mbar_init(empty0 + 8 * s, Cfg::kWarps);
-    }
+    for (int s = 0; s < STAGES; ++s) ptx::mbar_init(full0 + 8 * s, 1);
     ptx::fence_mbar_init_cluster();
-    ptx::prefetch_tensormap(&map_w0);
-    ptx::prefetch_tensormap(&map_x);
-    if (Cfg::kGatedOut) ptx::prefetch_tensormap(&map_w1);
+    ptx::fence_proxy_async_smem();
+    if (p.pdl != kPdlWeightsEarly) ptx::griddep_wait();
+    for (int it = 0; it < pre; ++it) load_w(it, it);
+    if (p.pdl == kPdlWeightsEarly) ptx::griddep_wait();
+    for (int it = 0; it < pre; ++it) load_x(it, it);
   }
-  ptx::cluster_sync_all();
+  __syncthreads();
 
-  // acc[i][j]: rows 16 i .. of this warp's 32, tokens 8 j ..
-  float acc[2][NT][4];
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-      for (int c = 0; c < 4; ++c) acc[i][j][c] = 0.0f;
   // Fragment row (or column) g of 8 stands for row tok(g), so that the 8
   // lanes of a 16-byte access phase (two rows, 4 chunks each) hit all 8 chunk
   // places of the 128-byte swizzle.
   const uint32_t g = lane >> 2, t = lane & 3u;
   const uint32_t tokg = (g >> 1) | ((g & 1u) << 2);
-  const uint32_t rw = warp & 1u, wk = warp >> 1;
 
-  if (warp == Cfg::kWarps) {
-    // ------------------------------------------------------------ producer
-    if (lane == 0) {
-      const uint64_t policy_w = ptx::policy_evict_first();  // read once (per 32 rows of X)
-      const uint64_t policy_x = ptx::policy_evict_last();   // read by every CTA
-      if (p.pdl != kPdlWeightsEarly) ptx::griddep_wait();
-      auto load_w = [&](int it, int s) {
-        const uint32_t bar = full0 + 8 * s, dst = base + Cfg::kW + s * Cfg::kStageW;
-        ptx::mbar_arrive_expect_tx(bar, Cfg::kStageBytes);
+  // acc[i][j]: weight rows 16 i .., tokens 8 j ..
+  float acc[4][NT][4];
 #pragma unroll
-        for (int b = 0; b < (Cfg::kW4 ? 1 : 2); ++b) {
-          // x counts elements of the map: bytes (two codes) or bf16
-          const int x = Cfg::kW4 ? (s_begin + it) * 128 : (s_begin + it) * 128 + b * 64;
-          const uint32_t d = dst + b * Cfg::kRows * 128;
-          ptx::tma_load_2d(d, &map_w0, bar, x, n0, policy_w);
-          if (Cfg::kGatedOut) ptx::tma_load_2d(d + 32 * 128, &map_w1, bar, x, n0, policy_w);
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) acc[i][j][c] = 0.0f;
+  // Scales of a stage: lane l holds those of weight rows l and l + 32 for
+  // the group that ends with chunk q, loaded one turn of this warp ahead.
+  [[maybe_unused]] uint16_t lo_sc[Cfg::kChunks], hi_sc[Cfg::kChunks];
+  const int chunk_mask = Cfg::kW4 ? (1 << (p.group_shift - 5)) - 1 : 0;  // a group's chunks
+  auto load_scales = [&](int it, uint16_t (&lo)[Cfg::kChunks], uint16_t (&hi)[Cfg::kChunks]) {
+    const int na = n0 + static_cast<int>(lane), nb = Cfg::kGatedOut ? na : na + 32;
+    const uint16_t* sb = Cfg::kGatedOut ? p.scales1 : p.scales0;
+#pragma unroll
+    for (int q = 0; q < Cfg::kChunks; ++q) {
+      lo[q] = hi[q] = 0;
+      const int k = (s_begin + it) * Cfg::kStageK + q * 32;
+      if ((q & chunk_mask) == chunk_mask && it < count && k < p.K) {
+        const long long at = static_cast<long long>(k >> p.group_shift) * p.N;
+        if (na < p.N) lo[q] = __ldg(p.scales0 + at + na);
+        if (nb < p.N) hi[q] = __ldg(sb + at + nb);
+      }
+    }
+  };
+  if (p.pdl != kPdlWeightsEarly) ptx::griddep_wait();
+  if constexpr (Cfg::kW4) load_scales(static_cast<int>(warp), lo_sc, hi_sc);
+  for (int it = static_cast<int>(warp); it < count; it += Cfg::kWarps) {
+    const int stage = it % STAGES;
+    const uint32_t phase = static_cast<uint32_t>(it / STAGES) & 1u;
+    [[maybe_unused]] uint16_t lo_next[Cfg::kChunks], hi_next[Cfg::kChunks];
+    if constexpr (Cfg::kW4) load_scales(it + Cfg::kWarps, lo_next, hi_next);
+    const bool got = ptx::mbar_wait_cta(full0 + 8 * stage, phase, wd, kSiteEpilogue, blockIdx.y);
+    if (!__all_sync(0xFFFFFFFFu, got)) break;
+    const uint32_t sw = base + Cfg::kW + stage * Cfg::kStageW;
+    const uint32_t sx = base + Cfg::kX + stage * Cfg::kStageX;
+    [[maybe_unused]] float sum[4][NT][4];
+#pragma unroll
+    for (int q = 0; q < Cfg::kChunks; ++q) {
+      // X's 8 k's of this lane for every tile of tokens
+      uint32_t x[NT][4];
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+        ptx::ld_shared_v4(sx + (q >> 1) * Cfg::kBoxX + (j * 8u + tokg) * 128u +
+                              (((static_cast<uint32_t>(q & 1) << 2) | t) ^ tokg) * 16u,
+                          x[j][0], x[j][1], x[j][2], x[j][3]);
+      if constexpr (Cfg::kW4) {
+        if (q == 0 || ((q - 1) & chunk_mask) == chunk_mask) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+              for (int c = 0; c < 4; ++c) sum[i][j][c] = 0.0f;
         }
-      };
-      auto load_x = [&](int it, int s) {
 #pragma unroll
-        for (int b = 0; b < Cfg::kStageK / 64; ++b)
-          ptx::tma_load_2d(base + Cfg::kX + s * Cfg::kStageX + b * Cfg::kBoxX, &map_x, full0 + 8 * s,
-                           (s_begin + it) * Cfg::kStageK + b * 64, m0, policy_x);
-      };
-      const int pre = min(STAGES, count);
-      for (int it = 0; it < pre; ++it) load_w(it, it);
-      if (p.pdl == kPdlWeightsEarly) ptx::griddep_wait();
-      for (int it = 0; it < pre; ++it) load_x(it, it);
-      uint32_t stage = 0, phase = 1;  // after a whole ring
-      for (int it = pre; it < count; ++it) {
-        if (!ptx::mbar_wait(empty0 + 8 * stage, phase ^ 1u, wd, kSiteProducer, blockIdx.y)) break;
-        load_w(it, static_cast<int>(stage));
-        load_x(it, static_cast<int>(stage));
-        if (++stage == STAGES) {
-          stage = 0;
-          phase ^= 1u;
+        for (int j = 0; j < NT; ++j) {
+          // pairs (k_j, k_j+4), as w4_expand gives the weights
+          const uint32_t x0 = x[j][0], x1 = x[j][1], x2 = x[j][2], x3 = x[j][3];
+          x[j][0] = __byte_perm(x0, x2, 0x5410);
+          x[j][1] = __byte_perm(x0, x2, 0x7632);
+          x[j][2] = __byte_perm(x1, x3, 0x5410);
+          x[j][3] = __byte_perm(x1, x3, 0x7632);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t a = sw + (i * 16u + tokg) * 128u + ((static_cast<uint32_t>(q) ^ tokg) << 4) + t * 4u;
+          uint32_t lo[4], hi[4];
+          w4_expand(ld_shared_u32(a), lo);
+          w4_expand(ld_shared_u32(a + 8u * 128u), hi);
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            mma_m16n8k16(sum[i][j], lo[0], hi[0], lo[1], hi[1], x[j][0], x[j][1]);
+            mma_m16n8k16(sum[i][j], lo[2], hi[2], lo[3], hi[3], x[j][2], x[j][3]);
+          }
+        }
+        if ((q & chunk_mask) == chunk_mask) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t v = i < 2 ? lo_sc[q] : hi_sc[q];
+            const float s0 = __uint_as_float(__shfl_sync(0xFFFFFFFFu, v, (i & 1) * 16 + tokg) << 16);
+            const float s1 = __uint_as_float(__shfl_sync(0xFFFFFFFFu, v, (i & 1) * 16 + 8 + tokg) << 16);
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+              acc[i][j][0] = fmaf(s0, sum[i][j][0], acc[i][j][0]);
+              acc[i][j][1] = fmaf(s0, sum[i][j][1], acc[i][j][1]);
+              acc[i][j][2] = fmaf(s1, sum[i][j][2], acc[i][j][2]);
+              acc[i][j][3] = fmaf(s1, sum[i][j][3], acc[i][j][3]);
+            }
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t a = sw + (i * 16u + tokg) * 128u + (((static_cast<uint32_t>(q) << 2) | t) ^ tokg) * 16u;
+          uint32_t lo[4], hi[4];
+          ptx::ld_shared_v4(a, lo[0], lo[1], lo[2], lo[3]);
+          ptx::ld_shared_v4(a + 8u * 128u, hi[0], hi[1], hi[2], hi[3]);
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            mma_m16n8k16(acc[i][j], lo[0], hi[0], lo[1], hi[1], x[j][0], x[j][1]);
+            mma_m16n8k16(acc[i][j], lo[2], hi[2], lo[3], hi[3], x[j][2], x[j][3]);
+          }
         }
       }
     }
     __syncwarp();
-  } else {
-    // ----------------------------------------------------------- consumers
-    uint32_t stage = 0, phase = 0;
-    [[maybe_unused]] int win = 0, win_end = -1;  // groups whose scales are in shared memory
-    if (p.pdl != kPdlWeightsEarly) ptx::griddep_wait();
-    for (int it = 0; it < count; ++it) {
-      if constexpr (Cfg::kW4) {
-        // Scales of the stage's groups: [group][row half][tok][row / 8], so a
-        // lane's four rows are 8 bytes.
-        const int first = ((s_begin + it) * 256) >> p.group_shift;
-        const int last = ((s_begin + it) * 256 + 255) >> p.group_shift;
-        if (last > win_end) {
-          const int groups = p.K >> p.group_shift;
-          const int range_last = min(groups - 1, ((s_begin + count) * 256 - 1) >> p.group_shift);
-          win = first;
-          win_end = max(last, min(range_last, win + Cfg::kScaleGroups - 1));
-          if (it > 0) ptx::named_barrier(1, 32 * Cfg::kWarps);  // the old ones are no longer read
-          const int r = static_cast<int>(threadIdx.x & 63u);    // weight row of the CTA
-          const bool up = Cfg::kGatedOut && r >= 32;
-          const int n = n0 + (Cfg::kGatedOut ? (r & 31) : r);
-          const uint16_t* src = (up ? p.scales1 : p.scales0) + n;
-          const uint32_t dst =
-              base + Cfg::kScale + static_cast<uint32_t>((r >> 5) * 32 + (r & 7) * 4 + ((r >> 3) & 3)) * 2u;
-#pragma unroll 8
-          for (int q = win + static_cast<int>(threadIdx.x >> 6); q <= win_end; q += 4) {
-            const uint16_t v = (n < p.N && q < groups) ? __ldg(src + static_cast<long long>(q) * p.N) : 0;
-            ptx::st_shared_u16(dst + static_cast<uint32_t>(q - win) * 128u, v);
-          }
-          ptx::named_barrier(1, 32 * Cfg::kWarps);
-        }
-      }
-      const bool got = ptx::mbar_wait(full0 + 8 * stage, phase, wd, kSiteEpilogue, blockIdx.y);
-      if (__all_sync(0xFFFFFFFFu, got)) {
-        const uint32_t sw = base + Cfg::kW + stage * Cfg::kStageW;
-        const uint32_t sx = base + Cfg::kX + stage * Cfg::kStageX;
-        // X's 8 k's of this lane for every tile of tokens: 32-k chunk q.
-        auto load_x = [&](uint32_t q, uint32_t (&x)[NT][4]) {
+    if (lane == 0 && it + STAGES < count) {
+      load_w(it + STAGES, stage);
+      load_x(it + STAGES, stage);
+    }
+    if constexpr (Cfg::kW4) {
 #pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            const uint32_t a = sx + (q >> 1) * Cfg::kBoxX + (j * 8u + tokg) * 128u + ((((q & 1u) << 2) | t) ^ tokg) * 16u;
-            ptx::ld_shared_v4(a, x[j][0], x[j][1], x[j][2], x[j][3]);
-          }
-        };
-        if constexpr (Cfg::kW4) {
-          float sum[2][NT][4];
-#pragma unroll
-          for (int qq = 0; qq < 2; ++qq) {
-            const uint32_t q = 2u * wk + qq;
-            // a group of 64 or more holds both of this warp's chunks
-            const bool fresh = qq == 0 || p.group_shift == 5;
-            if (fresh) {
-#pragma unroll
-              for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int j = 0; j < NT; ++j)
-#pragma unroll
-                  for (int c = 0; c < 4; ++c) sum[i][j][c] = 0.0f;
-            }
-            uint32_t x[NT][4];
-            load_x(q, x);
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-              // pairs (k_j, k_j+4), as w4_expand gives the weights
-              const uint32_t x0 = x[j][0], x1 = x[j][1], x2 = x[j][2], x3 = x[j][3];
-              x[j][0] = __byte_perm(x0, x2, 0x5410);
-              x[j][1] = __byte_perm(x0, x2, 0x7632);
-              x[j][2] = __byte_perm(x1, x3, 0x5410);
-              x[j][3] = __byte_perm(x1, x3, 0x7632);
-            }
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const uint32_t row = rw * 32u + i * 16u + tokg;
-              const uint32_t a = sw + row * 128u + ((q ^ tokg) << 4) + t * 4u;
-              uint32_t lo[4], hi[4];
-              w4_expand(ld_shared_u32(a), lo);
-              w4_expand(ld_shared_u32(a + 8u * 128u), hi);
-#pragma unroll
-              for (int j = 0; j < NT; ++j) {
-                mma_m16n8k16(sum[i][j], lo[0], hi[0], lo[1], hi[1], x[j][0], x[j][1]);
-                mma_m16n8k16(sum[i][j], lo[2], hi[2], lo[3], hi[3], x[j][2], x[j][3]);
-              }
-            }
-            if (qq == 1 || p.group_shift == 5) {
-              const int grp = ((s_begin + it) * 256 + static_cast<int>(q) * 32) >> p.group_shift;
-              const uint32_t a = base + Cfg::kScale + static_cast<uint32_t>(grp - win) * 128u + rw * 64u + tokg * 8u;
-              const uint32_t s01 = ld_shared_u32(a), s23 = ld_shared_u32(a + 4u);
-              const float s[4] = {bf16_lo(s01), bf16_hi(s01), bf16_lo(s23), bf16_hi(s23)};
-#pragma unroll
-              for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int j = 0; j < NT; ++j)
-#pragma unroll
-                  for (int c = 0; c < 4; ++c) acc[i][j][c] = fmaf(s[2 * i + (c >> 1)], sum[i][j][c], acc[i][j][c]);
-            }
-          }
-        } else {
-          uint32_t x[NT][4];
-          load_x(wk, x);
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const uint32_t row = rw * 32u + i * 16u + tokg;
-            const uint32_t a = sw + (wk >> 1) * (Cfg::kRows * 128u) + row * 128u + ((((wk & 1u) << 2) | t) ^ tokg) * 16u;
-            uint32_t lo[4], hi[4];
-            ptx::ld_shared_v4(a, lo[0], lo[1], lo[2], lo[3]);
-            ptx::ld_shared_v4(a + 8u * 128u, hi[0], hi[1], hi[2], hi[3]);
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-              mma_m16n8k16(acc[i][j], lo[0], hi[0], lo[1], hi[1], x[j][0], x[j][1]);
-              mma_m16n8k16(acc[i][j], lo[2], hi[2], lo[3], hi[3], x[j][2], x[j][3]);
-            }
-          }
-        }
-      }
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive_cluster(ptx::mapa(empty0 + 8 * stage, static_cast<uint32_t>(split > 1 ? rank : 0)));
-      if (++stage == STAGES) {
-        stage = 0;
-        phase ^= 1u;
+      for (int q = 0; q < Cfg::kChunks; ++q) {
+        lo_sc[q] = lo_next[q];
+        hi_sc[q] = hi_next[q];
       }
     }
-    // ------------------------------------------- the CTA's sum over its K range
-    ptx::named_barrier(1, 32 * Cfg::kWarps);  // the ring is drained
-    auto* red = reinterpret_cast<float*>(smem_raw + (base - ptx::smem_u32(smem_raw)) + Cfg::kRed);
-    auto* part = reinterpret_cast<float*>(smem_raw + (base - ptx::smem_u32(smem_raw)) + Cfg::kPart);
+  }
+  ptx::griddep_launch_dependents();
+  // ------------------------------------------- the CTA's sum over its K range
+  __syncthreads();  // the ring is drained
+  auto* ring = reinterpret_cast<float*>(smem_raw + (base - ptx::smem_u32(smem_raw)));
+  float* red = ring + Cfg::kRed / 4;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
+    for (int j = 0; j < NT; ++j)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          // column 2t + b of the fragment is token tok(2t + b) = t + 4b
-          const uint32_t tok = j * 8u + t + 4u * (c & 1), row = rw * 32u + i * 16u + 8u * (c >> 1) + tokg;
-          red[(wk * Cfg::kTok + tok) * Cfg::kPitch + row] = acc[i][j][c];
-        }
-    ptx::named_barrier(1, 32 * Cfg::kWarps);
+      for (int c = 0; c < 4; ++c) {
+        // column 2t + b of the fragment is token tok(2t + b) = t + 4b
+        const uint32_t tok = j * 8u + t + 4u * (c & 1), row = i * 16u + 8u * (c >> 1) + tokg;
+        red[(warp * Cfg::kTok + tok) * Cfg::kPitch + row] = acc[i][j][c];
+      }
+  __syncthreads();
+  if (split > 1) {
+    float* part = ring + Cfg::kPart / 4;
 #pragma unroll
     for (int idx = static_cast<int>(threadIdx.x); idx < Cfg::kTok * 64; idx += 32 * Cfg::kWarps) {
       const int at = (idx >> 6) * Cfg::kPitch + (idx & 63);
       float v = red[at];
 #pragma unroll
-      for (int w = 1; w < 4; ++w) v += red[w * Cfg::kTok * Cfg::kPitch + at];
+      for (int w = 1; w < Cfg::kWarps; ++w) v += red[w * Cfg::kTok * Cfg::kPitch + at];
       part[at] = v;
     }
-    __syncwarp();
   }
-  ptx::cluster_sync_all();
-  ptx::griddep_launch_dependents();
+  if (split > 1) ptx::cluster_sync_all();
 
-  // --------------------- the cluster's sum: each CTA finishes its own tokens
-  if (warp < Cfg::kWarps && !ptx::aborted(wd)) {
-    const uint32_t part0 = base + Cfg::kPart;
+  // --------- the sum over the warps or over the cluster, whose CTAs share it out
+  if (!ptx::aborted(wd)) {
     auto total = [&](int at) {
-      float v = ld_cluster_f32(ptx::mapa(part0 + at * 4u, 0));
-      for (int c = 1; c < split; ++c) v += ld_cluster_f32(ptx::mapa(part0 + at * 4u, static_cast<uint32_t>(c)));
+      if (split == 1) {
+        const uint32_t a = base + Cfg::kRed + at * 4u;
+        float v = __uint_as_float(ld_shared_u32(a));
+#pragma unroll
+        for (int w = 1; w < Cfg::kWarps; ++w)
+          v += __uint_as_float(ld_shared_u32(a + w * Cfg::kTok * Cfg::kPitch * 4u));
+        return v;
+      }
+      const uint32_t a = base + Cfg::kPart + at * 4u;
+      float v = ld_cluster_f32(ptx::mapa(a, 0));
+      for (int c = 1; c < split; ++c) v += ld_cluster_f32(ptx::mapa(a, static_cast<uint32_t>(c)));
       return v;
     };
     constexpr int kCols = Cfg::kOutCols;
@@ -390,7 +369,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 2)
   }
   if (threadIdx.x == 0 && ptx::aborted(wd)) ptx::sleep_ns_bounded(200000ull);
   __syncwarp();
-  ptx::cluster_sync_all();  // no CTA leaves while another reads its sums
+  if (split > 1) ptx::cluster_sync_all();  // no CTA leaves while another reads its sums
 }
 
 // ------------------------------------------------- 4-bit weights and bf16

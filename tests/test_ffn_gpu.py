@@ -46,6 +46,13 @@ def test_gated(gpu_handle, M, F, K, kind):
     _check_gated(gpu_handle, M, F, K, kind, save=False, seed=M + F)
 
 
+@pytest.mark.parametrize("M,F,K", [(1, 14000, 4096), (8, 5001, 2056), (12, 3001, 4096), (32, 6000, 2048), (1, 40, 8192)])
+def test_gated_few_rows_long(gpu_handle, M, F, K):
+    """Few rows against many and long weights: every ring goes around many
+    times, every SM holds several blocks; and a width that splits K."""
+    _check_gated(gpu_handle, M, F, K, "silu", save=False, seed=M)
+
+
 @pytest.mark.parametrize("width", [512, 256])
 @pytest.mark.parametrize("save", [False, True])
 @pytest.mark.parametrize("M,F,K", [(1, 7, 8), (300, 1001, 520), (2, 128, 64)])
