@@ -268,9 +268,10 @@ def gemm(A, B, out=None, stream=None):
 # The feed-forward operators (see the methods of `Gemm` of the same names) on
 # the device of their first argument.
 def _on_device_of(t) -> Gemm:
-    if not t.is_cuda:
+    device = t.get_device()
+    if device < 0:
         raise ValueError("expected a CUDA tensor")
-    return _handle_for(t.get_device())
+    return _handles.get(device) or _handle_for(device)
 
 
 def gated(X, Wg, Wu, activation: str = "silu", save: bool = False, out=None, stream=None):

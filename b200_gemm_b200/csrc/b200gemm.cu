@@ -488,8 +488,7 @@ struct b200gemm_handle {
 
 namespace b200gemm {
 int prepare_ffn_kernels(int sm_count);
-template <bool W4, bool GATED>
-bool prepare_skinny_kernels();
+bool prepare_all_skinny_kernels();
 }  // namespace b200gemm
 
 extern "C" int b200gemm_version(void) { return kVersion; }
@@ -541,9 +540,7 @@ extern "C" int b200gemm_create(b200gemm_t* out, int device) {
   const int sc2 = prepare_smallm1_kernel<SmallMCfg<2>>(sms), sc4 = prepare_smallm1_kernel<SmallMCfg<4>>(sms);
   if (sc2 <= 0 || sc4 <= 0) return B200GEMM_ERR_CUDA;
   const int fc = prepare_ffn_kernels(sms);
-  if (fc <= 0 || !prepare_skinny_kernels<false, true>() || !prepare_skinny_kernels<true, false>() ||
-      !prepare_skinny_kernels<true, true>())
-    return B200GEMM_ERR_CUDA;
+  if (fc <= 0 || !prepare_all_skinny_kernels()) return B200GEMM_ERR_CUDA;
 
   auto* h = new b200gemm_handle();
   h->device = device;

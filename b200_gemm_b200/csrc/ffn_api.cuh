@@ -63,10 +63,16 @@ bool prepare_skinny_kernel() {
   return true;
 }
 
-template <bool W4, bool GATED>
+template <bool W4, bool GATED, bool G32>
 bool prepare_skinny_kernels() {
-  return prepare_skinny_kernel<SkinnyCfg<W4, GATED, 1>>() && prepare_skinny_kernel<SkinnyCfg<W4, GATED, 2>>() &&
-         prepare_skinny_kernel<SkinnyCfg<W4, GATED, 4>>();
+  return prepare_skinny_kernel<SkinnyCfg<W4, GATED, 1, G32>>() && prepare_skinny_kernel<SkinnyCfg<W4, GATED, 2, G32>>() &&
+         prepare_skinny_kernel<SkinnyCfg<W4, GATED, 4, G32>>();
+}
+
+bool prepare_all_skinny_kernels() {
+  return prepare_skinny_kernels<false, true, false>() && prepare_skinny_kernels<true, false, false>() &&
+         prepare_skinny_kernels<true, false, true>() && prepare_skinny_kernels<true, true, false>() &&
+         prepare_skinny_kernels<true, true, true>();
 }
 
 template <class Cfg>
@@ -177,7 +183,7 @@ int skinny_split(const b200gemm_handle* h, long long row_blocks, int num_stages)
   return split;
 }
 
-template <bool W4, bool GATED>
+template <bool W4, bool GATED, bool G32 = false>
 int run_skinny(b200gemm_t h, const void* w0, const void* w1, long long ldw, const void* X, long long ldx,
                SkinnyParams p, cudaStream_t stream) {
   const int nt = p.M > 16 ? 4 : (p.M > 8 ? 2 : 1);
@@ -211,9 +217,9 @@ int run_skinny(b200gemm_t h, const void* w0, const void* w1, long long ldw, cons
   p.status = h->status_dev;
   const int rb = static_cast<int>(row_blocks), tb = static_cast<int>(token_blocks);
   const cudaError_t e =
-      nt == 1   ? launch_skinny<SkinnyCfg<W4, GATED, 1>>(split, rb, tb, stream, mw0, mw1, mx, p)
-      : nt == 2 ? launch_skinny<SkinnyCfg<W4, GATED, 2>>(split, rb, tb, stream, mw0, mw1, mx, p)
-                : launch_skinny<SkinnyCfg<W4, GATED, 4>>(split, rb, tb, stream, mw0, mw1, mx, p);
+      nt == 1   ? launch_skinny<SkinnyCfg<W4, GATED, 1, G32>>(split, rb, tb, stream, mw0, mw1, mx, p)
+      : nt == 2 ? launch_skinny<SkinnyCfg<W4, GATED, 2, G32>>(split, rb, tb, stream, mw0, mw1, mx, p)
+                : launch_skinny<SkinnyCfg<W4, GATED, 4, G32>>(split, rb, tb, stream, mw0, mw1, mx, p);
   return e == cudaSuccess ? B200GEMM_OK : B200GEMM_ERR_CUDA;
 }
 
@@ -529,7 +535,9 @@ extern "C" int b200gemm_w4_nt(b200gemm_t h, int M, int N, int K, const void* A, 
   p.scales0 = static_cast<const uint16_t*>(scales);
   p.out = C;
   p.ldo = ldc;
-  return run_skinny<true, false>(h, codes, nullptr, 0, A, lda, p, static_cast<cudaStream_t>(stream_ptr));
+  const cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
+  return group == 32 ? run_skinny<true, false, true>(h, codes, nullptr, 0, A, lda, p, stream)
+                     : run_skinny<true, false>(h, codes, nullptr, 0, A, lda, p, stream);
 }
 
 extern "C" int b200gemm_w4_gated(b200gemm_t h, int M, int F, int K, const void* X, long long ldx,
@@ -565,5 +573,7 @@ extern "C" int b200gemm_w4_gated(b200gemm_t h, int M, int F, int K, const void* 
   p.scales1 = static_cast<const uint16_t*>(up_scales);
   p.out = H;
   p.ldo = ldh;
-  return run_skinny<true, true>(h, gate_codes, up_codes, 0, X, ldx, p, static_cast<cudaStream_t>(stream_ptr));
+  const cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
+  return group == 32 ? run_skinny<true, true, true>(h, gate_codes, up_codes, 0, X, ldx, p, stream)
+                     : run_skinny<true, true>(h, gate_codes, up_codes, 0, X, ldx, p, stream);
 }

@@ -50,9 +50,12 @@ struct SkinnyParams {
   int pdl;
 };
 
-template <bool W4, bool GATED, int NT>
+// G32: groups of 32, whose sums are scaled after every 32-k chunk (4-bit
+// weights); without it a group holds 2, 4 or 8 chunks.
+template <bool W4, bool GATED, int NT, bool G32 = false>
 struct SkinnyCfg {
   static constexpr bool kW4 = W4;
+  static constexpr bool kG32 = G32;
   static constexpr bool kGatedOut = GATED;
   static constexpr int kNT = NT;                       // tiles of 8 rows of X
   static constexpr int kTok = 8 * NT;
@@ -93,11 +96,21 @@ struct SkinnyCfg {
 
 __device__ __forceinline__ void mma_m16n8k16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                              uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
       "{%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// The same with a zero accumulator going in.
+__device__ __forceinline__ void mma_m16n8k16_zero(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                                  uint32_t b0, uint32_t b1) {
+  asm(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%10, %10, %10, %10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 
 __device__ __forceinline__ uint32_t ld_shared_u32(uint32_t addr) {
@@ -114,12 +127,23 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t cluster_addr) {
 
 // Eight codes of a word -> four bf16 pairs of q - 8: pair j holds codes j and
 // j + 4.  0x4300 is 128 with a spacing of 1, so or-ing a code in gives
-// 128 + q; 136 is subtracted, exactly.
-__device__ __forceinline__ void w4_expand(uint32_t w, uint32_t (&v)[4]) {
+// 128 + q; 136 is subtracted, exactly.  And-or is one instruction on the
+// logic pipe when mask and magic number come from registers (W4Const: opaque
+// to the compiler, which otherwise keeps them as immediates and takes two).
+struct W4Const {
+  uint32_t mask, magic;
+};
+__device__ __forceinline__ W4Const w4_const() {
+  W4Const c;
+  asm volatile("mov.u32 %0, 0x000F000F;\n\tmov.u32 %1, 0x43004300;" : "=r"(c.mask), "=r"(c.magic));
+  return c;
+}
+__device__ __forceinline__ void w4_expand(uint32_t w, const W4Const& k, uint32_t (&v)[4]) {
   const __nv_bfloat162 bias = __halves2bfloat162(__ushort_as_bfloat16(0x4308), __ushort_as_bfloat16(0x4308));
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const uint32_t x = ((w >> (4 * j)) & 0x000F000Fu) | 0x43004300u;
+    uint32_t x;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(x) : "r"(w >> (4 * j)), "r"(k.mask), "r"(k.magic));
     const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&x), bias);
     v[j] = *reinterpret_cast<const uint32_t*>(&d);
   }
@@ -148,18 +172,20 @@ __global__ void __launch_bounds__(Cfg::kThreads, Cfg::kCtas)
   wd.status = p.status;
   wd.timeout_ns = p.timeout_ns;
 
+  const uint64_t policy_w = ptx::policy_evict_first();  // read once (per 32 rows of X)
+  const uint64_t policy_x = ptx::policy_evict_last();   // read by every CTA
   auto load_w = [&](int it, int s) {
     const uint32_t bar = full0 + 8 * s, dst = base + Cfg::kW + s * Cfg::kStageW;
     const int x = (s_begin + it) * (Cfg::kW4 ? 128 : 64);  // elements of the map: bytes (two codes) or bf16
     ptx::mbar_arrive_expect_tx(bar, Cfg::kStageBytes);
-    ptx::tma_load_2d(dst, &map_w0, bar, x, n0, ptx::policy_evict_first());  // read once (per 32 rows of X)
-    if (Cfg::kGatedOut) ptx::tma_load_2d(dst + 32 * 128, &map_w1, bar, x, n0, ptx::policy_evict_first());
+    ptx::tma_load_2d(dst, &map_w0, bar, x, n0, policy_w);
+    if (Cfg::kGatedOut) ptx::tma_load_2d(dst + 32 * 128, &map_w1, bar, x, n0, policy_w);
   };
   auto load_x = [&](int it, int s) {
 #pragma unroll
     for (int b = 0; b < Cfg::kStageK / 64; ++b)
       ptx::tma_load_2d(base + Cfg::kX + s * Cfg::kStageX + b * Cfg::kBoxX, &map_x, full0 + 8 * s,
-                       (s_begin + it) * Cfg::kStageK + b * 64, m0, ptx::policy_evict_last());  // read by every CTA
+                       (s_begin + it) * Cfg::kStageK + b * 64, m0, policy_x);
   };
   const int pre = min(STAGES, count);
   if (threadIdx.x == 0) {
@@ -181,6 +207,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, Cfg::kCtas)
   const uint32_t g = lane >> 2, t = lane & 3u;
   const uint32_t tokg = (g >> 1) | ((g & 1u) << 2);
 
+  [[maybe_unused]] const W4Const w4c = w4_const();
   // acc[i][j]: weight rows 16 i .., tokens 8 j ..
   float acc[4][NT][4];
 #pragma unroll
@@ -191,45 +218,75 @@ __global__ void __launch_bounds__(Cfg::kThreads, Cfg::kCtas)
       for (int c = 0; c < 4; ++c) acc[i][j][c] = 0.0f;
   // Scales of a stage: lane l holds those of weight rows l and l + 32 for
   // the group that ends with chunk q, loaded one turn of this warp ahead.
-  [[maybe_unused]] uint16_t lo_sc[Cfg::kChunks], hi_sc[Cfg::kChunks];
-  const int chunk_mask = Cfg::kW4 ? (1 << (p.group_shift - 5)) - 1 : 0;  // a group's chunks
-  auto load_scales = [&](int it, uint16_t (&lo)[Cfg::kChunks], uint16_t (&hi)[Cfg::kChunks]) {
-    const int na = n0 + static_cast<int>(lane), nb = Cfg::kGatedOut ? na : na + 32;
-    const uint16_t* sb = Cfg::kGatedOut ? p.scales1 : p.scales0;
+  [[maybe_unused]] float lo_sc[Cfg::kChunks], hi_sc[Cfg::kChunks];
+  [[maybe_unused]] uint32_t lo_next[Cfg::kChunks] = {}, hi_next[Cfg::kChunks] = {};
+  const int chunk_mask = Cfg::kG32 || !Cfg::kW4 ? 0 : (1 << (p.group_shift - 5)) - 1;  // a group's chunks
+  // (rows past N take the last row's scales: their sums are not written)
+  const int na = min(n0 + static_cast<int>(lane), p.N - 1);
+  const int nb = Cfg::kGatedOut ? na : min(n0 + static_cast<int>(lane) + 32, p.N - 1);
+  const uint16_t* scales_a = p.scales0 + na;
+  const uint16_t* scales_b = (Cfg::kGatedOut ? p.scales1 : p.scales0) + nb;
+  auto load_scales = [&](int it) {
+    if (it >= count) return;
+    const int k0 = (s_begin + it) * Cfg::kStageK;
+    const long long at = static_cast<long long>(k0 >> p.group_shift) * p.N;
+    const uint16_t *pa = scales_a + at, *pb = scales_b + at;
+    const int left = p.K - k0;  // k's past K: scale 0 (their weights and X are 0)
+    if (left >= Cfg::kStageK) {
 #pragma unroll
-    for (int q = 0; q < Cfg::kChunks; ++q) {
-      lo[q] = hi[q] = 0;
-      const int k = (s_begin + it) * Cfg::kStageK + q * 32;
-      if ((q & chunk_mask) == chunk_mask && it < count && k < p.K) {
-        const long long at = static_cast<long long>(k >> p.group_shift) * p.N;
-        if (na < p.N) lo[q] = __ldg(p.scales0 + at + na);
-        if (nb < p.N) hi[q] = __ldg(sb + at + nb);
+      for (int q = 0; q < Cfg::kChunks; ++q) {
+        if ((q & chunk_mask) == chunk_mask) {
+          lo_next[q] = __ldg(pa);
+          hi_next[q] = __ldg(pb);
+          pa += p.N;
+          pb += p.N;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int q = 0; q < Cfg::kChunks; ++q) {
+        if ((q & chunk_mask) == chunk_mask) {
+          lo_next[q] = q * 32 < left ? __ldg(pa) : 0;
+          hi_next[q] = q * 32 < left ? __ldg(pb) : 0;
+          pa += p.N;
+          pb += p.N;
+        }
       }
     }
   };
+  auto take_scales = [&]() {
+#pragma unroll
+    for (int q = 0; q < Cfg::kChunks; ++q) {
+      lo_sc[q] = __uint_as_float(lo_next[q] << 16);
+      hi_sc[q] = __uint_as_float(hi_next[q] << 16);
+    }
+  };
   if (p.pdl != kPdlWeightsEarly) ptx::griddep_wait();
-  if constexpr (Cfg::kW4) load_scales(static_cast<int>(warp), lo_sc, hi_sc);
+  if constexpr (Cfg::kW4) load_scales(static_cast<int>(warp));
   for (int it = static_cast<int>(warp); it < count; it += Cfg::kWarps) {
     const int stage = it % STAGES;
     const uint32_t phase = static_cast<uint32_t>(it / STAGES) & 1u;
-    [[maybe_unused]] uint16_t lo_next[Cfg::kChunks], hi_next[Cfg::kChunks];
-    if constexpr (Cfg::kW4) load_scales(it + Cfg::kWarps, lo_next, hi_next);
+    if constexpr (Cfg::kW4) {
+      take_scales();
+      load_scales(it + Cfg::kWarps);
+    }
     const bool got = ptx::mbar_wait_cta(full0 + 8 * stage, phase, wd, kSiteEpilogue, blockIdx.y);
     if (!__all_sync(0xFFFFFFFFu, got)) break;
-    const uint32_t sw = base + Cfg::kW + stage * Cfg::kStageW;
-    const uint32_t sx = base + Cfg::kX + stage * Cfg::kStageX;
+    // Shared addresses: stages, boxes and groups of 8 rows are 1024-byte
+    // aligned and a row is 128 bytes, so a chunk's place is one exclusive-or.
+    const uint32_t aw = base + Cfg::kW + stage * Cfg::kStageW + tokg * 128u + (Cfg::kW4 ? (tokg << 4) + t * 4u : (t ^ tokg) << 4);
+    const uint32_t ax = base + Cfg::kX + stage * Cfg::kStageX + tokg * 128u + ((t ^ tokg) << 4);
     [[maybe_unused]] float sum[4][NT][4];
 #pragma unroll
     for (int q = 0; q < Cfg::kChunks; ++q) {
       // X's 8 k's of this lane for every tile of tokens
       uint32_t x[NT][4];
+      const uint32_t axq = ax ^ (static_cast<uint32_t>(q & 1) << 6);
 #pragma unroll
       for (int j = 0; j < NT; ++j)
-        ptx::ld_shared_v4(sx + (q >> 1) * Cfg::kBoxX + (j * 8u + tokg) * 128u +
-                              (((static_cast<uint32_t>(q & 1) << 2) | t) ^ tokg) * 16u,
-                          x[j][0], x[j][1], x[j][2], x[j][3]);
+        ptx::ld_shared_v4(axq + (q >> 1) * Cfg::kBoxX + j * 1024u, x[j][0], x[j][1], x[j][2], x[j][3]);
       if constexpr (Cfg::kW4) {
-        if (q == 0 || ((q - 1) & chunk_mask) == chunk_mask) {
+        if (!Cfg::kG32 && (q == 0 || ((q - 1) & chunk_mask) == chunk_mask)) {
 #pragma unroll
           for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -246,24 +303,25 @@ __global__ void __launch_bounds__(Cfg::kThreads, Cfg::kCtas)
           x[j][2] = __byte_perm(x1, x3, 0x5410);
           x[j][3] = __byte_perm(x1, x3, 0x7632);
         }
+        const uint32_t awq = aw ^ (static_cast<uint32_t>(q) << 4);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint32_t a = sw + (i * 16u + tokg) * 128u + ((static_cast<uint32_t>(q) ^ tokg) << 4) + t * 4u;
           uint32_t lo[4], hi[4];
-          w4_expand(ld_shared_u32(a), lo);
-          w4_expand(ld_shared_u32(a + 8u * 128u), hi);
+          w4_expand(ld_shared_u32(awq + i * 2048u), w4c, lo);
+          w4_expand(ld_shared_u32(awq + i * 2048u + 1024u), w4c, hi);
 #pragma unroll
           for (int j = 0; j < NT; ++j) {
-            mma_m16n8k16(sum[i][j], lo[0], hi[0], lo[1], hi[1], x[j][0], x[j][1]);
+            if (Cfg::kG32) mma_m16n8k16_zero(sum[i][j], lo[0], hi[0], lo[1], hi[1], x[j][0], x[j][1]);
+            else mma_m16n8k16(sum[i][j], lo[0], hi[0], lo[1], hi[1], x[j][0], x[j][1]);
             mma_m16n8k16(sum[i][j], lo[2], hi[2], lo[3], hi[3], x[j][2], x[j][3]);
           }
         }
         if ((q & chunk_mask) == chunk_mask) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const uint32_t v = i < 2 ? lo_sc[q] : hi_sc[q];
-            const float s0 = __uint_as_float(__shfl_sync(0xFFFFFFFFu, v, (i & 1) * 16 + tokg) << 16);
-            const float s1 = __uint_as_float(__shfl_sync(0xFFFFFFFFu, v, (i & 1) * 16 + 8 + tokg) << 16);
+            const float v = i < 2 ? lo_sc[q] : hi_sc[q];
+            const float s0 = __shfl_sync(0xFFFFFFFFu, v, (i & 1) * 16 + tokg);
+            const float s1 = __shfl_sync(0xFFFFFFFFu, v, (i & 1) * 16 + 8 + tokg);
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
               acc[i][j][0] = fmaf(s0, sum[i][j][0], acc[i][j][0]);
@@ -274,12 +332,12 @@ __global__ void __launch_bounds__(Cfg::kThreads, Cfg::kCtas)
           }
         }
       } else {
+        const uint32_t awq = aw ^ (static_cast<uint32_t>(q) << 6);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint32_t a = sw + (i * 16u + tokg) * 128u + (((static_cast<uint32_t>(q) << 2) | t) ^ tokg) * 16u;
           uint32_t lo[4], hi[4];
-          ptx::ld_shared_v4(a, lo[0], lo[1], lo[2], lo[3]);
-          ptx::ld_shared_v4(a + 8u * 128u, hi[0], hi[1], hi[2], hi[3]);
+          ptx::ld_shared_v4(awq + i * 2048u, lo[0], lo[1], lo[2], lo[3]);
+          ptx::ld_shared_v4(awq + i * 2048u + 1024u, hi[0], hi[1], hi[2], hi[3]);
 #pragma unroll
           for (int j = 0; j < NT; ++j) {
             mma_m16n8k16(acc[i][j], lo[0], hi[0], lo[1], hi[1], x[j][0], x[j][1]);
@@ -292,13 +350,6 @@ __global__ void __launch_bounds__(Cfg::kThreads, Cfg::kCtas)
     if (lane == 0 && it + STAGES < count) {
       load_w(it + STAGES, stage);
       load_x(it + STAGES, stage);
-    }
-    if constexpr (Cfg::kW4) {
-#pragma unroll
-      for (int q = 0; q < Cfg::kChunks; ++q) {
-        lo_sc[q] = lo_next[q];
-        hi_sc[q] = hi_next[q];
-      }
     }
   }
   ptx::griddep_launch_dependents();

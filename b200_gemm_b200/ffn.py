@@ -16,6 +16,18 @@ from . import _lib
 ACTIVATIONS = {"none": _lib.ACT_NONE, "relu": _lib.ACT_RELU, "gelu": _lib.ACT_GELU,
                "gelu_tanh": _lib.ACT_GELU_TANH, "silu": _lib.ACT_SILU}
 W4_GROUPS = (32, 64, 128, 256)
+_NO_CONTEXT = contextlib.nullcontext()
+_torch_module = None
+
+
+def _torch():
+    """torch, imported when a call first needs it."""
+    global _torch_module
+    if _torch_module is None:
+        import torch
+
+        _torch_module = torch
+    return _torch_module
 
 
 def _activation(name: str) -> int:
@@ -26,43 +38,44 @@ def _activation(name: str) -> int:
 
 
 class FfnOps:
-    """Mixin of `Gemm` (uses its `_lib`, `_h` and `device`)."""
+    """Mixin of `Gemm` (uses its `_lib`, `_h` and `device`).  A call's checks
+    are kept to a few microseconds: at one token they are a good part of it."""
 
     # --------------------------------------------------------------- helpers
     def _check(self, t, name: str, dtype, rows=None, cols=None) -> int:
         """Checks a row-major matrix argument; returns its row pitch."""
+        shape = t.shape
+        if (t.dtype is dtype and t.get_device() == self.device and len(shape) == 2
+                and (rows is None or shape[0] == rows) and (cols is None or shape[1] == cols)):
+            pitch, step = t.stride()
+            if step == 1 or shape[1] <= 1:
+                return pitch if shape[0] > 1 else 8 * ((shape[1] + 7) // 8)  # (one row's stride means nothing)
+            raise ValueError(f"{name} must be row-major (stride(1) == 1)")
         if t.dtype != dtype:
             raise TypeError(f"{name} must be {dtype}")
-        if not t.is_cuda or t.get_device() != self.device:
+        if t.get_device() != self.device:
             raise ValueError(f"{name} must be on cuda:{self.device}")
-        if t.dim() != 2 or (rows is not None and t.shape[0] != rows) or (cols is not None and t.shape[1] != cols):
-            want = f"[{'*' if rows is None else rows}, {'*' if cols is None else cols}]"
-            raise ValueError(f"{name} must have shape {want}, not {list(t.shape)}")
-        r, c = t.shape
-        if c > 1 and t.stride(1) != 1:
-            raise ValueError(f"{name} must be row-major (stride(1) == 1)")
-        return t.stride(0) if r > 1 else 8 * ((c + 7) // 8)  # (one row's stride means nothing)
+        want = f"[{'*' if rows is None else rows}, {'*' if cols is None else cols}]"
+        raise ValueError(f"{name} must have shape {want}, not {list(shape)}")
 
     def _where(self, stream):
         """(stream pointer, context in which the call's tensors are allocated)."""
-        import torch
-
+        torch = _torch()
         if stream is None:
-            return int(torch.cuda.current_stream(self.device).cuda_stream), contextlib.nullcontext()
+            return torch._C._cuda_getCurrentRawStream(self.device), _NO_CONTEXT
         if isinstance(stream, int):
             stream = torch.cuda.ExternalStream(stream, device=self.device)
         if stream.device.index != self.device:
             raise ValueError(f"stream must belong to cuda:{self.device}")
         return int(stream.cuda_stream), torch.cuda.stream(stream)
 
-    def _empty(self, rows: int, cols: int, dtype=None):
-        """A [rows, cols] matrix whose rows start on 16-byte boundaries."""
-        import torch
-
-        dtype = torch.bfloat16 if dtype is None else dtype
-        if cols % 8 == 0:
-            return torch.empty(rows, cols, device=f"cuda:{self.device}", dtype=dtype)
-        return torch.empty(rows, 8 * ((cols + 7) // 8), device=f"cuda:{self.device}", dtype=dtype)[:, :cols]
+    def _empty(self, rows: int, cols: int, dtype):
+        """A [rows, cols] matrix whose rows start on 16-byte boundaries, and its
+        row pitch."""
+        torch = _torch()
+        pitch = 8 * ((cols + 7) // 8)
+        t = torch.empty((rows, pitch), dtype=dtype, device=torch.device("cuda", self.device))
+        return (t if pitch == cols else t[:, :cols]), pitch
 
     # ------------------------------------------------------------ gated block
     def gated(self, X, Wg, Wu, activation: str = "silu", save: bool = False, out=None, gate_out=None, up_out=None,
@@ -74,8 +87,7 @@ class FfnOps:
         to bf16, which `gated_backward` takes.  `out`, `gate_out` and `up_out`
         may be given, the last two with one row stride; nothing may overlap
         what is written.  activation: none, relu, gelu, gelu_tanh, silu."""
-        import torch
-
+        torch = _torch()
         act = _activation(activation)
         bf16 = torch.bfloat16
         ldx = self._check(X, "X", bf16)
@@ -87,14 +99,14 @@ class FfnOps:
         ptr, where = self._where(stream)
         ldgu = 0
         with where:
-            H = self._empty(M, F) if out is None else out
-            ldh = self._check(H, "out", bf16, M, F)
+            H, ldh = self._empty(M, F, bf16) if out is None else (out, self._check(out, "out", bf16, M, F))
             G = U = None
             if save or gate_out is not None or up_out is not None:
-                G = self._empty(M, F) if gate_out is None else gate_out
-                U = self._empty(M, F) if up_out is None else up_out
-                ldgu = self._check(G, "gate_out", bf16, M, F)
-                if self._check(U, "up_out", bf16, M, F) != ldgu:
+                G, ldgu = (self._empty(M, F, bf16) if gate_out is None
+                           else (gate_out, self._check(gate_out, "gate_out", bf16, M, F)))
+                U, ldu = (self._empty(M, F, bf16) if up_out is None
+                          else (up_out, self._check(up_out, "up_out", bf16, M, F)))
+                if ldu != ldgu:
                     raise ValueError("gate_out and up_out must have the same row stride")
             rc = self._lib.b200gemm_bf16_gated(
                 self._h, M, F, K, X.data_ptr(), ldx, Wg.data_ptr(), Wu.data_ptr(), ldw, act, H.data_ptr(), ldh,
@@ -110,8 +122,7 @@ class FfnOps:
         dU = dH act(G) and dG = dH U act'(G) are rounded to bf16 before the
         products (they are tensor-core operands); sums are fp32.  With
         `input_grad` or `weight_grad` off the matching results are None."""
-        import torch
-
+        torch = _torch()
         act = _activation(activation)
         bf16 = torch.bfloat16
         lddh = self._check(dH, "dH", bf16)
@@ -126,16 +137,21 @@ class FfnOps:
             raise ValueError("G and U must have the same row stride")
         ptr, where = self._where(stream)
         with where:
-            dX = self._empty(M, K) if input_grad else None
-            dWg, dWu = (self._empty(F, K), self._empty(F, K)) if weight_grad else (None, None)
+            dX = dWg = dWu = None
+            lddx = lddw = 0
+            if input_grad:
+                dX, lddx = self._empty(M, K, bf16)
+            if weight_grad:
+                dWg, lddw = self._empty(F, K, bf16)
+                dWu, lddw = self._empty(F, K, bf16)
             # Freed when this returns: the allocator hands it on in the order of
             # the stream that it was allocated for, which is the call's.
             ws = torch.empty(max(16, self._lib.b200gemm_gated_backward_workspace(M, F)), dtype=torch.uint8,
-                             device=f"cuda:{self.device}")
+                             device=torch.device("cuda", self.device))
             rc = self._lib.b200gemm_bf16_gated_backward(
                 self._h, M, F, K, dH.data_ptr(), lddh, X.data_ptr(), ldx, Wg.data_ptr(), Wu.data_ptr(), ldw,
-                G.data_ptr(), U.data_ptr(), ldgu, act, None if dX is None else dX.data_ptr(), K,
-                None if dWg is None else dWg.data_ptr(), None if dWu is None else dWu.data_ptr(), K,
+                G.data_ptr(), U.data_ptr(), ldgu, act, None if dX is None else dX.data_ptr(), lddx,
+                None if dWg is None else dWg.data_ptr(), None if dWu is None else dWu.data_ptr(), lddw,
                 ws.data_ptr(), ptr)
         _lib.check(rc, "b200gemm_bf16_gated_backward")
         return dX, dWg, dWu
@@ -143,22 +159,20 @@ class FfnOps:
     # --------------------------------------------------------- 4-bit weights
     def _w4(self, codes, scales, name: str, K=None, N=None):
         """Checks 4-bit weights; returns (N, K, group)."""
-        import torch
-
-        if codes.dtype != torch.uint8 or scales.dtype != torch.bfloat16:
+        torch = _torch()
+        if codes.dtype is not torch.uint8 or scales.dtype is not torch.bfloat16:
             raise TypeError(f"{name}: codes must be torch.uint8 and scales torch.bfloat16")
-        for t in (codes, scales):
-            if not t.is_cuda or t.get_device() != self.device:
-                raise ValueError(f"{name} must be on cuda:{self.device}")
-            if t.dim() != 2 or not t.is_contiguous():
-                raise ValueError(f"{name}: codes [N, K / 2] and scales [K / group, N] must be contiguous")
-        n, k = codes.shape[0], 2 * codes.shape[1]
+        if codes.get_device() != self.device or scales.get_device() != self.device:
+            raise ValueError(f"{name} must be on cuda:{self.device}")
+        cs, ss = codes.shape, scales.shape
+        if len(cs) != 2 or len(ss) != 2 or not codes.is_contiguous() or not scales.is_contiguous():
+            raise ValueError(f"{name}: codes [N, K / 2] and scales [K / group, N] must be contiguous")
+        n, k, groups = cs[0], 2 * cs[1], ss[0]
         if (N is not None and n != N) or (K is not None and k != K):
             raise ValueError(f"{name}: codes of a [{n}, {k}] weight where [{n if N is None else N}, "
                              f"{k if K is None else K}] is needed")
-        groups = scales.shape[0]
-        if scales.shape[1] != n or groups == 0 or k % groups != 0 or k // groups not in W4_GROUPS:
-            raise ValueError(f"{name}: scales {list(scales.shape)} do not fit codes {list(codes.shape)} with a group "
+        if ss[1] != n or groups == 0 or k % groups != 0 or k // groups not in W4_GROUPS:
+            raise ValueError(f"{name}: scales {list(ss)} do not fit codes {list(cs)} with a group "
                              f"of {', '.join(map(str, W4_GROUPS))}")
         return n, k, k // groups
 
@@ -167,8 +181,7 @@ class FfnOps:
         256) consecutive k of a row s = bf16(max|w| / 7) and
         q = clamp(rint(w / s), -8, 7) + 8.  codes: uint8 [N, K / 2], the even k
         in the low four bits; scales: bf16 [K / group, N]."""
-        import torch
-
+        torch = _torch()
         ldw = self._check(W, "W", torch.bfloat16)
         N, K = W.shape
         if group not in W4_GROUPS or K % group != 0 or K == 0:
@@ -186,13 +199,12 @@ class FfnOps:
         """The bf16 [N, K] weights that the codes stand for, bf16(s (q - 8)).
         For long prompts: `bf16_nt` with these beats `w4_nt` from about 200
         rows on."""
-        import torch
-
+        torch = _torch()
         N, K, group = self._w4(codes, scales, "weights")
         ptr, where = self._where(stream)
         with where:
-            W = self._empty(N, K) if out is None else out
-            ldw = self._check(W, "out", torch.bfloat16, N, K)
+            bf16 = torch.bfloat16
+            W, ldw = self._empty(N, K, bf16) if out is None else (out, self._check(out, "out", bf16, N, K))
             rc = self._lib.b200gemm_w4_dequantize(self._h, N, K, codes.data_ptr(), scales.data_ptr(), group,
                                                   W.data_ptr(), ldw, ptr)
         _lib.check(rc, "b200gemm_w4_dequantize")
@@ -202,8 +214,7 @@ class FfnOps:
         """out = A W^T for 4-bit weights W (see `w4_quantize`): bf16 A [M, K],
         out [M, N] bf16 (default) or fp32.  No weight is rounded: group sums of
         A (q - 8) are scaled in fp32."""
-        import torch
-
+        torch = _torch()
         N, K, group = self._w4(codes, scales, "weights")
         lda = self._check(A, "A", torch.bfloat16, None, K)
         M = A.shape[0]
@@ -213,8 +224,8 @@ class FfnOps:
             raise TypeError("out_dtype must be torch.bfloat16 or torch.float32")
         ptr, where = self._where(stream)
         with where:
-            C = self._empty(M, N, out_dtype) if out is None else out
-            ldc = self._check(C, "out", out_dtype, M, N)
+            C, ldc = (self._empty(M, N, out_dtype) if out is None
+                      else (out, self._check(out, "out", out_dtype, M, N)))
             rc = self._lib.b200gemm_w4_nt(self._h, M, N, K, A.data_ptr(), lda, codes.data_ptr(), scales.data_ptr(),
                                           group, C.data_ptr(), ldc,
                                           _lib.OUT_F32 if out_dtype == torch.float32 else _lib.OUT_BF16, ptr)
@@ -224,8 +235,7 @@ class FfnOps:
     def w4_gated(self, X, gate_codes, gate_scales, up_codes, up_scales, activation: str = "silu", out=None,
                  stream=None):
         """H = act(X Wg^T) * (X Wu^T) for 4-bit Wg and Wu [F, K] of one group."""
-        import torch
-
+        torch = _torch()
         act = _activation(activation)
         F, K, group = self._w4(gate_codes, gate_scales, "gate weights")
         if self._w4(up_codes, up_scales, "up weights", K, F)[2] != group:
@@ -234,8 +244,8 @@ class FfnOps:
         M = X.shape[0]
         ptr, where = self._where(stream)
         with where:
-            H = self._empty(M, F) if out is None else out
-            ldh = self._check(H, "out", torch.bfloat16, M, F)
+            bf16 = torch.bfloat16
+            H, ldh = self._empty(M, F, bf16) if out is None else (out, self._check(out, "out", bf16, M, F))
             rc = self._lib.b200gemm_w4_gated(self._h, M, F, K, X.data_ptr(), ldx, gate_codes.data_ptr(),
                                              gate_scales.data_ptr(), up_codes.data_ptr(), up_scales.data_ptr(), group,
                                              act, H.data_ptr(), ldh, ptr)
