@@ -426,10 +426,11 @@ __global__ void __launch_bounds__(Cfg::kThreads, Cfg::kCtas)
 // ------------------------------------------------- 4-bit weights and bf16
 // Per group of one row: s = bf16(max|w| / 7), q = clamp(rint(w / s), -8, 7) + 8
 // (8 where s is 0 or NaN, so a group with a NaN or infinity comes back as
-// NaN).  DRAM-bound.  A block takes 32 rows x 256 k's: a warp reads 256 k's of
-// a row, 16 bytes a lane, four rows in flight; a group's lanes find its
-// maximum by shuffles on the magnitude bits (which order NaN above all), and
-// the block's scales are written row-contiguously through shared memory.
+// NaN).  DRAM-bound once the arithmetic is a handful of instructions per
+// weight.  A block takes 32 rows x 256 k's: a warp reads 256 k's of a row, 16
+// bytes a lane, four rows in flight; a group's lanes find its maximum by
+// shuffles on the magnitude bits (which order NaN above all), and the block's
+// scales are written row-contiguously through shared memory.
 struct W4Params {
   int N, K, group_shift;
   uint16_t* w;           // [N, K], row pitch ldw
@@ -438,42 +439,81 @@ struct W4Params {
   uint16_t* scales;      // [K / group, N]
 };
 
+// Codes of 8 weights (4 words of bf16 pairs) for scale s.  The quotient of
+// two bf16 numbers is either a tie k + 1/2 exactly or at least 2^-10 off one
+// (2w - (2k + 1)s is a multiple of the smaller operand's last place), while
+// w * (1 / s) is within 2^-20 of it below 8.  So one fused multiply-add onto
+// 1.5 * 2^11, where fp32 has a spacing of 2^-12, gives the quotient on a grid
+// that holds the ties and moves nothing across one, and a second addition
+// onto 1.5 * 2^23 + 8 rounds it to the integer (ties to even) and leaves q + 8
+// in the low four bits.  |w / s| <= 7 (1 + 2^-8) here, so nothing is clamped;
+// where s is so small that it has lost digits or 1 / s overflows, the
+// division is done as such.
+__device__ __forceinline__ uint32_t w4_codes(const uint32_t (&w)[4], float s) {
+  uint32_t code = 0u;
+  if (s >= 1e-30f && s <= 1e37f) {
+    const float r = ptx::rcp_approx(s);
+    constexpr float kGrid = 1.5f * 2048.0f, kInt = 1.5f * 8388608.0f + 8.0f;
+    // Eight sums of 1.5 * 2^23 + 8 + q, shifted up and added: their constant
+    // parts add up to kBase.
+    constexpr uint32_t kOne = 0x4B400000u, kBase = kOne * 0x11111111u;
+#pragma unroll
+    for (int j = 3; j >= 0; --j) {
+      code = (code << 4) + __float_as_uint(fmaf(bf16_hi(w[j]), r, kGrid) + (kInt - kGrid));
+      code = (code << 4) + __float_as_uint(fmaf(bf16_lo(w[j]), r, kGrid) + (kInt - kGrid));
+    }
+    code -= kBase;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float x = (j & 1) ? bf16_hi(w[j >> 1]) : bf16_lo(w[j >> 1]);
+      int q = 0;
+      if (s > 0.0f) q = max(-8, min(7, __float2int_rn(__fdiv_rn(x, s))));  // (NaN converts to 0)
+      code |= static_cast<uint32_t>(q + 8) << (4 * j);
+    }
+  }
+  return code;
+}
+
 __global__ void __launch_bounds__(256) w4_quantize_kernel(const W4Params p) {
   __shared__ uint16_t sc[8][32];
   const int warp = static_cast<int>(threadIdx.x >> 5), lane = static_cast<int>(threadIdx.x & 31u);
   const int k = static_cast<int>(blockIdx.x) * 256 + lane * 8;
   const int n0 = static_cast<int>(blockIdx.y) * 32;
   const int lanes = 1 << (p.group_shift - 3);  // per group: 4 .. 32
+  const int rows = k < p.K ? p.N - n0 - warp : 0;  // of this lane: row 8 i is one of them while 8 i < rows
   uint32_t w[4][4];
+  const uint16_t* src = p.w + static_cast<long long>(n0 + warp) * p.ldw + k;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int n = n0 + warp + 8 * i;
     w[i][0] = w[i][1] = w[i][2] = w[i][3] = 0u;
-    if (n < p.N && k < p.K)
-      ptx::ld_global_nc_v4(p.w + static_cast<long long>(n) * p.ldw + k, w[i][0], w[i][1], w[i][2], w[i][3]);
+    if (8 * i < rows) ptx::ld_global_nc_v4(src, w[i][0], w[i][1], w[i][2], w[i][3]);
+    src += 8 * p.ldw;
   }
+  uint32_t m[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int n = n0 + warp + 8 * i;
     uint32_t m2 = 0u;
 #pragma unroll
     for (int j = 0; j < 4; ++j) m2 = __vmaxu2(m2, w[i][j] & 0x7FFF7FFFu);
-    uint32_t m = max(m2 & 0xFFFFu, m2 >> 16);
-    for (int d = 1; d < lanes; d <<= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
-    const __nv_bfloat16 sb = __float2bfloat16_rn(__fdiv_rn(__uint_as_float(m << 16), 7.0f));
-    const float s = __bfloat162float(sb);
-    uint32_t code = 0u;
+    m[i] = max(m2 & 0xFFFFu, m2 >> 16);
+  }
+  for (int d = 1; d < lanes; d <<= 1) {  // (the four rows' shuffles in flight together)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float x = (j & 1) ? bf16_hi(w[i][j >> 1]) : bf16_lo(w[i][j >> 1]);
-      int q = 0;
-      if (s > 0.0f) q = max(-8, min(7, __float2int_rn(__fdiv_rn(x, s))));  // (NaN converts to 0)
-      code |= static_cast<uint32_t>(q + 8) << (4 * j);
-    }
-    if (n < p.N && k < p.K) {
-      *reinterpret_cast<uint32_t*>(p.codes + static_cast<long long>(n) * (p.K / 2) + k / 2) = code;
+    for (int i = 0; i < 4; ++i) m[i] = max(m[i], __shfl_xor_sync(0xFFFFFFFFu, m[i], d));
+  }
+  uint8_t* dst = p.codes + static_cast<long long>(n0 + warp) * (p.K / 2) + k / 2;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    // max / 7 by a product: like the quotients below, max / 7 is never within
+    // 2^-12 of a bf16 rounding border without being a bf16 number itself.
+    const __nv_bfloat16 sb = __float2bfloat16_rn(__uint_as_float(m[i] << 16) * (1.0f / 7.0f));
+    const uint32_t code = w4_codes(w[i], __bfloat162float(sb));
+    if (8 * i < rows) {
+      *reinterpret_cast<uint32_t*>(dst) = code;
       if ((lane & (lanes - 1)) == 0) sc[lane >> (p.group_shift - 3)][warp + 8 * i] = __bfloat16_as_ushort(sb);
     }
+    dst += 4ll * p.K;
   }
   __syncthreads();
   const int q = warp + (static_cast<int>(blockIdx.x) * 256 >> p.group_shift);
@@ -481,8 +521,9 @@ __global__ void __launch_bounds__(256) w4_quantize_kernel(const W4Params p) {
     p.scales[static_cast<long long>(q) * p.N + n0 + lane] = sc[warp][lane];
 }
 
-// W[n,k] = bf16(s (q - 8)): the product is exact in fp32 and rounded once.
-// The same blocks; 4 bytes of codes and 16 of results per lane and row.
+// W[n,k] = bf16(s (q - 8)): q - 8 is exact in bf16 (w4_expand), so one bf16
+// multiplication per pair is the one rounding.  The same blocks; 4 bytes of
+// codes and 16 of results per lane and row.
 __global__ void __launch_bounds__(256) w4_dequantize_kernel(const W4Params p) {
   __shared__ uint16_t sc[8][32];
   const int warp = static_cast<int>(threadIdx.x >> 5), lane = static_cast<int>(threadIdx.x & 31u);
@@ -501,19 +542,24 @@ __global__ void __launch_bounds__(256) w4_dequantize_kernel(const W4Params p) {
     sc[warp][lane] = __ldg(p.scales + static_cast<long long>(q) * p.N + n0 + lane);
   __syncthreads();
   if (k >= p.K) return;
+  const W4Const c = w4_const();
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int n = n0 + warp + 8 * i;
     if (n >= p.N) continue;
-    const float s = __uint_as_float(static_cast<uint32_t>(sc[lane >> (p.group_shift - 3)][warp + 8 * i]) << 16);
-    uint32_t o[4];
+    const __nv_bfloat16 s1 = __ushort_as_bfloat16(sc[lane >> (p.group_shift - 3)][warp + 8 * i]);
+    const __nv_bfloat162 s2 = __halves2bfloat162(s1, s1);
+    uint32_t v[4];
+    w4_expand(w[i], c, v);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float lo = s * static_cast<float>(static_cast<int>((w[i] >> (8 * j)) & 15u) - 8);
-      const float hi = s * static_cast<float>(static_cast<int>((w[i] >> (8 * j + 4)) & 15u) - 8);
-      o[j] = ptx::pack_bf16x2(__float_as_uint(lo), __float_as_uint(hi));
+      const __nv_bfloat162 d = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&v[j]), s2);
+      v[j] = *reinterpret_cast<const uint32_t*>(&d);
     }
-    ptx::st_global_v4(p.w + static_cast<long long>(n) * p.ldw + k, o[0], o[1], o[2], o[3]);
+    // pairs (k_j, k_j+4) back into order
+    ptx::st_global_v4(p.w + static_cast<long long>(n) * p.ldw + k, __byte_perm(v[0], v[1], 0x5410),
+                      __byte_perm(v[2], v[3], 0x5410), __byte_perm(v[0], v[1], 0x7632),
+                      __byte_perm(v[2], v[3], 0x7632));
   }
 }
 
