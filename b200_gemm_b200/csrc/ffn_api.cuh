@@ -11,10 +11,8 @@ namespace b200gemm {
 // or 6 x 32 KB + 16 KB.
 using FfnGated2 = FfnCfg<kGated, 2, 3>;
 using FfnGated1 = FfnCfg<kGated, 1, 6>;
-using FfnDx2 = FfnCfg<kDx, 2, 3>;
-using FfnDx1 = FfnCfg<kDx, 1, 6>;
-using FfnDw2 = FfnCfg<kDw, 2, 3>;
-using FfnDw1 = FfnCfg<kDw, 1, 6>;
+using FfnGrads2 = FfnCfg<kGrads, 2, 3>;
+using FfnGrads1 = FfnCfg<kGrads, 1, 6>;
 
 template <class Cfg>
 int prepare_ffn_kernel(int sm_count) {
@@ -45,9 +43,8 @@ int prepare_ffn_kernel(int sm_count) {
 // Smallest number of clusters that fit over all instances of the tiled
 // feed-forward kernel (they differ only in registers), or 0 on failure.
 int prepare_ffn_kernels(int sm_count) {
-  const int c[6] = {prepare_ffn_kernel<FfnGated2>(sm_count), prepare_ffn_kernel<FfnGated1>(sm_count),
-                    prepare_ffn_kernel<FfnDx2>(sm_count),    prepare_ffn_kernel<FfnDx1>(sm_count),
-                    prepare_ffn_kernel<FfnDw2>(sm_count),    prepare_ffn_kernel<FfnDw1>(sm_count)};
+  const int c[4] = {prepare_ffn_kernel<FfnGated2>(sm_count), prepare_ffn_kernel<FfnGated1>(sm_count),
+                    prepare_ffn_kernel<FfnGrads2>(sm_count), prepare_ffn_kernel<FfnGrads1>(sm_count)};
   int least = c[0];
   for (int v : c) least = v < least ? v : least;
   return least;
@@ -76,13 +73,20 @@ bool prepare_all_skinny_kernels() {
 }
 
 template <class Cfg>
-cudaError_t launch_ffn(int clusters, cudaStream_t stream, const CUtensorMap (&m)[7], const FfnParams& p) {
+cudaError_t launch_ffn(int clusters, cudaStream_t stream, const FfnMaps& m, const FfnParams& p, bool overlap) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(2 * clusters), 1, 1);
   cfg.blockDim = dim3(Cfg::kThreads, 1, 1);
   cfg.dynamicSmemBytes = Cfg::kSmemBytes;
   cfg.stream = stream;
-  return cudaLaunchKernelEx(&cfg, ffn_gemm_sm100<Cfg>, m[0], m[1], m[2], m[3], m[4], m[5], m[6], p);
+  cudaLaunchAttribute attr[1];
+  if (overlap) {
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+  }
+  return cudaLaunchKernelEx(&cfg, ffn_gemm_sm100<Cfg>, m, p);
 }
 
 template <class Cfg>
@@ -150,14 +154,41 @@ bool group_shift_of(int group, int* shift) {
 
 constexpr int kMaxExtent = 0x7FFFFFFF - 4096;  // rows, columns: tile coordinates stay inside an int
 
-// NB = 2 (512 accumulator columns, shared A stage) or 1 for a product whose
-// accumulators are `cols` columns wide, by the tile cost model of the plain
-// GEMM.  A forced tile width of 512 or 448 asks for 2, any other for 1.
-int ffn_nb(const b200gemm_handle* h, uint32_t tiles_m, int cols, int num_kb, double epi2, double epi1) {
+// Time of one tile of num_kb K blocks in the units of tile_plan_cost: a 256 x
+// 256 tile (NB = 1, its epilogue hidden) or a 256 x 512 one (NB = 2) whose
+// epilogue costs `epi` more than the plain one.
+double ffn_tile_time(int nb, int num_kb, double epi) {
+  return nb == 2 ? (2.0 * num_kb + 13.0) * 0.8545 / 0.85 + epi : num_kb / 0.85 + 4.0;
+}
+
+// The gated block's NB: by waves of tiles.  A forced tile width of 512 or 448
+// asks for 2, any other for 1.
+int ffn_gated_nb(const b200gemm_handle* h, int tiles_m, int F, int num_kb) {
   if (h->tile_width != 0) return h->tile_width >= 448 ? 2 : 1;
-  const double c2 = tile_plan_cost(512, tiles_m, cols, num_kb, h->ffn_clusters, epi2);
-  const double c1 = tile_plan_cost(256, tiles_m, cols, num_kb, h->ffn_clusters, epi1);
-  return c2 < c1 ? 2 : 1;
+  double cost[3];
+  for (int nb = 1; nb <= 2; ++nb) {
+    const long long tiles = static_cast<long long>(tiles_m) * ((F + 128ll * nb - 1) / (128 * nb));
+    cost[nb] = static_cast<double>((tiles + h->ffn_clusters - 1) / h->ffn_clusters) *
+               ffn_tile_time(nb, num_kb, 12.0);
+  }
+  return cost[2] < cost[1] ? 2 : 1;
+}
+
+// The same for the gradients, whose tiles fill the clusters' time together:
+// the mean load and half a dW tile, or what the dX tiles alone take.
+int ffn_grads_nb(const b200gemm_handle* h, int m, int f, int k, bool dx, bool dw) {
+  if (h->tile_width != 0) return h->tile_width >= 448 ? 2 : 1;
+  double cost[3];
+  const double g = h->ffn_clusters;
+  for (int nb = 1; nb <= 2; ++nb) {
+    const double tn = (k + 256ll * nb - 1) / (256 * nb);
+    const double n1 = dx ? tn * ((m + 255ll) / 256) : 0.0, n2 = dw ? 2.0 * tn * ((f + 255ll) / 256) : 0.0;
+    const double t1 = ffn_tile_time(nb, 2 * ((f + 63) / 64), 0.0), t2 = ffn_tile_time(nb, (m + 63) / 64, 0.0);
+    const double mean = (n1 * t1 + n2 * t2) / g + (n2 > 0.0 ? 0.5 * t2 : 0.0);
+    const double alone = static_cast<double>(static_cast<long long>((n1 + g - 1.0) / g)) * t1;
+    cost[nb] = mean > alone ? mean : alone;
+  }
+  return cost[2] < cost[1] ? 2 : 1;
 }
 
 // bf16 operand maps of the tiled kernel: K-major boxes of 64 k x 128 rows,
@@ -223,19 +254,30 @@ int run_skinny(b200gemm_t h, const void* w0, const void* w1, long long ldw, cons
   return e == cudaSuccess ? B200GEMM_OK : B200GEMM_ERR_CUDA;
 }
 
+FfnSet ffn_set(int M, int N, int num_kb, int tile_n, int matrices) {
+  FfnSet s;
+  s.M = M;
+  s.N = N;
+  s.num_kb = num_kb;
+  s.tiles_m = (M + kTileM - 1) / kTileM;
+  s.tiles_n = (N + tile_n - 1) / tile_n;
+  const long long tiles = static_cast<long long>(matrices) * s.tiles_m * s.tiles_n;
+  s.tiles = tiles > (1ll << 29) ? -1 : static_cast<int>(tiles);  // -1: too many
+  return s;
+}
+
 template <class Cfg>
-int run_ffn(b200gemm_t h, const CUtensorMap (&maps)[7], FfnParams p, cudaStream_t stream) {
-  const long long tiles = static_cast<long long>(Cfg::kKind == kDw ? 2 : 1) * p.tiles_m * p.tiles_n;
-  if (tiles > (1ll << 30)) return B200GEMM_ERR_TOO_LARGE;
-  p.num_tiles = static_cast<int>(tiles);
+int run_ffn(b200gemm_t h, const FfnMaps& maps, FfnParams p, cudaStream_t stream, bool overlap) {
+  if (p.first.tiles < 0 || p.second.tiles < 0) return B200GEMM_ERR_TOO_LARGE;
   p.band = B200GEMM_DEFAULT_BAND;
   p.status = h->status_dev;
   {
     std::lock_guard<std::mutex> lock(h->mu);
     p.timeout_ns = h->timeout_ns;
   }
-  const int clusters = p.num_tiles < h->ffn_clusters ? p.num_tiles : h->ffn_clusters;
-  return launch_ffn<Cfg>(clusters, stream, maps, p) == cudaSuccess ? B200GEMM_OK : B200GEMM_ERR_CUDA;
+  const int tiles = p.first.tiles + p.second.tiles;
+  const int clusters = tiles < h->ffn_clusters ? tiles : h->ffn_clusters;
+  return launch_ffn<Cfg>(clusters, stream, maps, p, overlap) == cudaSuccess ? B200GEMM_OK : B200GEMM_ERR_CUDA;
 }
 
 template <int ACT>
@@ -272,11 +314,10 @@ extern "C" int b200gemm_bf16_gated(b200gemm_t h, int M, int F, int K, const void
   bool small;
   int nb;
   const int num_kb = (K + kBlockK - 1) / kBlockK;
-  const uint32_t tiles_m = static_cast<uint32_t>((M + kTileM - 1) / kTileM);
   {
     std::lock_guard<std::mutex> lock(h->mu);
     small = M <= 32 && G == nullptr && h->small_m != 0 && h->tile_width == 0;
-    nb = ffn_nb(h, tiles_m, F > kMaxExtent / 2 ? kMaxExtent : 2 * F, num_kb, 16.0, 4.6);
+    nb = ffn_gated_nb(h, (M + kTileM - 1) / kTileM, F, num_kb);
   }
   if (small) {
     SkinnyParams p{};
@@ -289,27 +330,23 @@ extern "C" int b200gemm_bf16_gated(b200gemm_t h, int M, int F, int K, const void
     p.ldo = ldh;
     return run_skinny<false, true>(h, Wg, Wu, ldw, X, ldx, p, stream);
   }
-  CUtensorMap m[7];
-  if (!encode_kmajor(&m[0], X, K, M, ldx) || !encode_kmajor(&m[2], Wg, K, F, ldw) ||
-      !encode_kmajor(&m[3], Wu, K, F, ldw) || !encode_out(&m[4], H, F, M, ldh)) {
+  FfnMaps m;
+  if (!encode_kmajor(&m.a0, X, K, M, ldx) || !encode_kmajor(&m.b0, Wg, K, F, ldw) ||
+      !encode_kmajor(&m.b1, Wu, K, F, ldw) || !encode_out(&m.c[0], H, F, M, ldh)) {
     return B200GEMM_ERR_CUDA;
   }
-  m[1] = m[0];
-  m[5] = m[6] = m[4];
-  if (G != nullptr && (!encode_out(&m[5], G, F, M, ldgu) || !encode_out(&m[6], U, F, M, ldgu)))
+  m.a1 = m.w0 = m.w1 = m.x = m.a0;  // (not read)
+  m.c[1] = m.c[2] = m.c[0];
+  if (G != nullptr && (!encode_out(&m.c[1], G, F, M, ldgu) || !encode_out(&m.c[2], U, F, M, ldgu)))
     return B200GEMM_ERR_CUDA;
   FfnParams p{};
-  p.M = M;
-  p.N = F;
-  p.num_kb = num_kb;
-  p.tiles_m = static_cast<int>(tiles_m);
-  p.tiles_n = (F + 128 * nb - 1) / (128 * nb);
+  p.first = ffn_set(M, F, num_kb, 128 * nb, 1);
   p.act = activation;
   p.save = G != nullptr ? 1 : 0;
   p.out[0] = {static_cast<uint16_t*>(H), ldh};
   p.out[1] = {static_cast<uint16_t*>(G), ldgu};
   p.out[2] = {static_cast<uint16_t*>(U), ldgu};
-  return nb == 2 ? run_ffn<FfnGated2>(h, m, p, stream) : run_ffn<FfnGated1>(h, m, p, stream);
+  return nb == 2 ? run_ffn<FfnGated2>(h, m, p, stream, false) : run_ffn<FfnGated1>(h, m, p, stream, false);
 }
 
 extern "C" unsigned long long b200gemm_gated_backward_workspace(int M, int F) {
@@ -387,54 +424,29 @@ extern "C" int b200gemm_bf16_gated_backward(b200gemm_t h, int M, int F, int K, c
   if (cudaGetLastError() != cudaSuccess) return B200GEMM_ERR_CUDA;
 
   const int f8i = static_cast<int>(f8);
-  if (dX != nullptr) {
-    CUtensorMap m[7];
-    if (!encode_kmajor(&m[0], gp.dg, f8i, M, f8) || !encode_kmajor(&m[1], gp.du, f8i, M, f8) ||
-        !encode_mnmajor(&m[2], Wg, K, F, ldw) || !encode_mnmajor(&m[3], Wu, K, F, ldw) ||
-        !encode_out(&m[4], dX, K, M, lddx))
-      return B200GEMM_ERR_CUDA;
-    m[5] = m[6] = m[4];
-    FfnParams p{};
-    p.M = M;
-    p.N = K;
-    p.seg_kb = (F + kBlockK - 1) / kBlockK;
-    p.num_kb = 2 * p.seg_kb;
-    p.tiles_m = (M + kTileM - 1) / kTileM;
-    p.out[0] = {static_cast<uint16_t*>(dX), lddx};
-    int nb;
-    {
-      std::lock_guard<std::mutex> lock(h->mu);
-      nb = ffn_nb(h, static_cast<uint32_t>(p.tiles_m), K, p.num_kb, 0.0, 0.0);
-    }
-    p.tiles_n = (K + 256 * nb - 1) / (256 * nb);
-    const int rc = nb == 2 ? run_ffn<FfnDx2>(h, m, p, stream) : run_ffn<FfnDx1>(h, m, p, stream);
-    if (rc != B200GEMM_OK) return rc;
+  FfnMaps m;
+  if (!encode_kmajor(&m.a0, gp.dg, f8i, M, f8) || !encode_kmajor(&m.a1, gp.du, f8i, M, f8) ||
+      !encode_mnmajor(&m.b0, Wg, K, F, ldw) || !encode_mnmajor(&m.b1, Wu, K, F, ldw) ||
+      !encode_mnmajor(&m.w0, gp.dg, f8i, M, f8) || !encode_mnmajor(&m.w1, gp.du, f8i, M, f8) ||
+      !encode_mnmajor(&m.x, X, K, M, ldx) || (dX != nullptr && !encode_out(&m.c[0], dX, K, M, lddx)) ||
+      (dWg != nullptr && (!encode_out(&m.c[1], dWg, K, F, lddw) || !encode_out(&m.c[2], dWu, K, F, lddw))))
+    return B200GEMM_ERR_CUDA;
+  if (dX == nullptr) m.c[0] = m.c[1];  // (not written)
+  if (dWg == nullptr) m.c[1] = m.c[2] = m.c[0];
+  int nb;
+  {
+    std::lock_guard<std::mutex> lock(h->mu);
+    nb = ffn_grads_nb(h, M, F, K, dX != nullptr, dWg != nullptr);
   }
-  if (dWg != nullptr) {
-    CUtensorMap m[7];
-    if (!encode_mnmajor(&m[0], gp.dg, f8i, M, f8) || !encode_mnmajor(&m[1], gp.du, f8i, M, f8) ||
-        !encode_mnmajor(&m[2], X, K, M, ldx) || !encode_out(&m[4], dWg, K, F, lddw) ||
-        !encode_out(&m[5], dWu, K, F, lddw))
-      return B200GEMM_ERR_CUDA;
-    m[3] = m[2];
-    m[6] = m[4];
-    FfnParams p{};
-    p.M = F;
-    p.N = K;
-    p.num_kb = (M + kBlockK - 1) / kBlockK;
-    p.tiles_m = (F + kTileM - 1) / kTileM;
-    p.out[0] = {static_cast<uint16_t*>(dWg), lddw};
-    p.out[1] = {static_cast<uint16_t*>(dWu), lddw};
-    int nb;
-    {
-      std::lock_guard<std::mutex> lock(h->mu);
-      nb = ffn_nb(h, 2u * static_cast<uint32_t>(p.tiles_m), K, p.num_kb, 0.0, 0.0);
-    }
-    p.tiles_n = (K + 256 * nb - 1) / (256 * nb);
-    const int rc = nb == 2 ? run_ffn<FfnDw2>(h, m, p, stream) : run_ffn<FfnDw1>(h, m, p, stream);
-    if (rc != B200GEMM_OK) return rc;
-  }
-  return B200GEMM_OK;
+  FfnParams p{};
+  p.seg_kb = (F + kBlockK - 1) / kBlockK;
+  p.first = ffn_set(M, K, 2 * p.seg_kb, 256 * nb, dX != nullptr ? 1 : 0);
+  p.second = ffn_set(F, K, (M + kBlockK - 1) / kBlockK, 256 * nb, dWg != nullptr ? 2 : 0);
+  p.ahead = static_cast<int>(ffn_tile_time(nb, p.first.num_kb, 0.0) / ffn_tile_time(nb, p.second.num_kb, 0.0) + 0.5);
+  p.out[0] = {static_cast<uint16_t*>(dX), lddx};
+  p.out[1] = {static_cast<uint16_t*>(dWg), lddw};
+  p.out[2] = {static_cast<uint16_t*>(dWu), lddw};
+  return nb == 2 ? run_ffn<FfnGrads2>(h, m, p, stream, true) : run_ffn<FfnGrads1>(h, m, p, stream, true);
 }
 
 namespace {

@@ -3,22 +3,26 @@
 //   dU = dH * act(G), dG = dH * U * act'(G)
 //   dX = dG Wg + dU Wu, dWg = dG^T X, dWu = dU^T X
 // in bf16 with fp32 accumulation in TMEM.  One persistent, warp-specialised
-// kernel (roles, ring, bounded waits and teardown as in gemm_sm100.cuh) in
-// three kinds that differ in what feeds the two operands of an MMA and in
-// what is done with the accumulator:
-//   kGated  A = X, B = Wg and Wu; a tile's accumulator holds a block of
-//           G next to the same block of U, and the epilogue combines them,
-//           so neither goes to memory unless the caller keeps it.
-//   kDx     one sum over the 2F products: first dG (A) with Wg (B), then dU
-//           with Wu, so dX is written once.  Wg is [F,K] and F is summed
-//           over, so B is read "MN-major": a TMA box is 64 columns (of the
-//           output) x 64 rows (of the sum).
-//   kDw     dWg and dWu in one launch: the tile rows of both follow one
-//           another.  The sum runs over the M rows, so dG/dU and X are both
-//           read MN-major.
+// kernel (roles, ring, bounded waits and teardown as in gemm_sm100.cuh) with
+// three kinds of tile, which differ in what feeds the two operands of an MMA
+// and in what is done with the accumulator:
+//   gated  A = X, B = Wg and Wu; a tile's accumulator holds a block of G next
+//          to the same block of U, and the epilogue combines them, so neither
+//          goes to memory unless the caller keeps it.
+//   dX     one sum over the 2F products: first dG (A) with Wg (B), then dU
+//          with Wu, so dX is written once.  Wg is [F,K] and F is summed over,
+//          so B is read "MN-major": a TMA box is 64 columns (of the output) x
+//          64 rows (of the sum).
+//   dW     dWg's tile rows, then dWu's.  The sum runs over the M rows, so
+//          dG/dU and X are both read MN-major.
 // MN-major operands cost nothing over K-major ones: the same bytes per stage
-// in the same 128-byte swizzle, two 8 KB boxes instead of one of 16 KB.
-// No transposed copy of anything is made.
+// in the same 128-byte swizzle, two 8 KB boxes instead of one of 16 KB.  No
+// transposed copy of anything is made.
+//
+// dX and dW run in one launch: dX's tiles are few and long (a sum over 2F),
+// dW's many and short, so the clusters that get no dX tile, or one less, take
+// dW tiles meanwhile (ffn_unit), where two launches would leave most SMs idle
+// behind dX's last wave.
 #pragma once
 
 #include <cstdint>
@@ -29,26 +33,42 @@
 
 namespace b200gemm {
 
-enum FfnKind { kGated = 0, kDx = 1, kDw = 2 };
+enum FfnKind { kGated = 0, kGrads = 1 };
 
 struct FfnOut {
   uint16_t* ptr;   // bf16 bits
   long long ld;    // row pitch in elements
 };
 
-struct FfnParams {
-  int M, N;          // rows and columns of one output matrix (kGated: N = F)
+// One set of equal tiles.
+struct FfnSet {
+  int M, N;          // rows and columns of one output matrix (gated: N = F)
   int num_kb;        // K blocks of a tile
-  int seg_kb;        // kDx: K blocks of the first product (num_kb = 2 seg_kb)
-  int tiles_m;       // tile rows of one output matrix
+  int tiles_m;       // tile rows (dW: of one of the two matrices)
   int tiles_n;       // tile columns
-  int num_tiles;     // tiles of the launch (kDw: both matrices')
+  int tiles;         // tiles in all (dW: of both matrices)
+};
+
+struct FfnParams {
+  FfnSet first;      // gated, or dX
+  FfnSet second;     // dW
+  int seg_kb;        // dX: K blocks of the first product (num_kb = 2 seg_kb)
+  int ahead;         // dW tiles that a cluster without a last dX tile takes meanwhile
   int band;          // tile rows per band of the tile order
   int act;           // kAct*
-  int save;          // kGated: G and U are written too
-  FfnOut out[3];     // kGated: H, G, U; kDx: dX; kDw: dWg, dWu
+  int save;          // gated: G and U are written too
+  FfnOut out[3];     // gated: H, G, U; gradients: dX, dWg, dWu
   unsigned int* status;
   unsigned long long timeout_ns;
+};
+
+// Tensor maps of a launch.
+struct FfnMaps {
+  CUtensorMap a0, a1;   // gated: X; dX: dG, dU (K-major)
+  CUtensorMap b0, b1;   // gated: Wg, Wu (K-major); dX: Wg, Wu (MN-major)
+  CUtensorMap w0, w1;   // dW: dG, dU (MN-major)
+  CUtensorMap x;        // dW: X (MN-major)
+  CUtensorMap c[3];     // the outputs
 };
 
 // NB = 2: 256 x 512 accumulators, a single one: two N = 256 MMAs per K step
@@ -64,13 +84,9 @@ struct FfnCfg {
   static constexpr int kKind = KIND;
   static constexpr int kNB = NB;
   static constexpr int kStages = STAGES;
-  static constexpr bool kAMn = KIND == kDw;      // A read MN-major
-  static constexpr bool kBMn = KIND != kGated;   // B read MN-major
   static constexpr int kAccCols = 256 * NB;
   static constexpr int kTileN = KIND == kGated ? 128 * NB : 256 * NB;  // output columns per tile
   static constexpr int kAccBufs = NB == 1 ? 2 : 1;
-  static constexpr uint32_t kIdesc = (1u << 4) | (1u << 7) | (1u << 10) | (kAMn ? 1u << 15 : 0u) |
-                                     (kBMn ? 1u << 16 : 0u) | ((256u >> 3) << 17) | ((256u >> 4) << 24);
   static constexpr int kEpiWarps = 4 * NB;
   static constexpr int kThreads = 64 + 32 * kEpiWarps;
   static constexpr int kWarpCols = kTileN / NB;              // output columns one epilogue warp writes
@@ -109,14 +125,53 @@ __device__ __forceinline__ uint64_t ffn_desc(uint32_t addr) {
 template <bool MN>
 constexpr uint64_t kDescStep = MN ? 128 : 2;
 
-// Tile t of the band order: bands of `band` tile rows, each swept column by
-// column, so the band's A rows and one column of B stay in L2 meanwhile.
-__device__ __forceinline__ void ffn_tile(const FfnParams& p, int tiles_m, int t, int& tm, int& tn) {
-  const int per_band = p.band * p.tiles_n;
+// Instruction descriptor: kind::f16, D f32, A and B bf16, M = 256 (pair),
+// N = 256; bits 15 and 16 say that A or B is MN-major.
+template <bool A_MN, bool B_MN>
+constexpr uint32_t kFfnIdesc = (1u << 4) | (1u << 7) | (1u << 10) | (A_MN ? 1u << 15 : 0u) | (B_MN ? 1u << 16 : 0u) |
+                               ((256u >> 3) << 17) | ((256u >> 4) << 24);
+
+// Tile t of a set in the band order: bands of `band` tile rows, each swept
+// column by column, so the band's A rows and one column of B stay in L2
+// meanwhile.
+__device__ __forceinline__ void ffn_tile(int band, int tiles_m, int tiles_n, int t, int& tm, int& tn) {
+  const int per_band = band * tiles_n;
   const int b = t / per_band, r = t - b * per_band;
-  const int rows = min(p.band, tiles_m - b * p.band);
+  const int rows = min(band, tiles_m - b * band);
   tn = r / rows;
-  tm = b * p.band + (r - tn * rows);
+  tm = b * band + (r - tn * rows);
+}
+
+// The i-th unit of cluster c of g: a tile of the first set (round robin), then
+// of the second.  Where the first set's tiles do not divide evenly, the
+// clusters that have one less take `ahead` tiles of the second set meanwhile,
+// and the rest go round all clusters.  False past the last unit.
+struct FfnUnit {
+  bool second;   // of the second set: dW
+  bool up;       // dW: a tile of dWu
+  int tm, tn;
+};
+template <int KIND>
+__device__ __forceinline__ bool ffn_unit(const FfnParams& p, int c, int g, int i, FfnUnit& u) {
+  const int q = p.first.tiles / g, r = p.first.tiles - q * g;
+  const int mine = q + (c < r ? 1 : 0);
+  u.second = u.up = false;
+  if (i < mine) {
+    ffn_tile(p.band, p.first.tiles_m, p.first.tiles_n, i * g + c, u.tm, u.tn);
+    return true;
+  }
+  if constexpr (KIND == kGated) return false;
+  const int k = i - mine, light = g - r;  // (r = 0: no cluster has more than another)
+  const int ahead = r > 0 ? p.ahead : 0;
+  int t;
+  if (c >= r && k < ahead) t = k * light + (c - r);
+  else t = ahead * light + (c >= r ? (k - ahead) * g + (c - r) : k * g + light + c);
+  if (t >= p.second.tiles) return false;
+  ffn_tile(p.band, 2 * p.second.tiles_m, p.second.tiles_n, t, u.tm, u.tn);
+  u.second = true;
+  u.up = u.tm >= p.second.tiles_m;
+  if (u.up) u.tm -= p.second.tiles_m;
+  return true;
 }
 
 // act(x) for bf16 results: e^x and the reciprocal are the fast forms, whose
@@ -218,12 +273,38 @@ __device__ __forceinline__ void ffn_store_chunk(const uint32_t (&w)[16], int col
   if (++cbuf == BUFS) cbuf = 0;
 }
 
+// The K blocks of one tile through the MMA: false when a wait ran out.
+template <class Cfg, bool A_MN, bool B_MN>
+__device__ __forceinline__ bool ffn_mma_tile(uint32_t sA, uint32_t sB, uint32_t full0, uint32_t own_empty0,
+                                             uint32_t peer_empty0, uint32_t d_tmem, int num_kb, uint32_t& stage,
+                                             uint32_t& phase, const ptx::Watchdog& wd, unsigned int unit) {
+  for (int kb = 0; kb < num_kb; ++kb) {
+    if (!ptx::mbar_wait(full0 + 8 * stage, phase, wd, kSiteMmaFull, unit)) return false;
+    ptx::tc_fence_after();
+    const uint64_t a_desc = ffn_desc<A_MN>(sA + stage * kStageBytesA);
+    const uint64_t b_desc = ffn_desc<B_MN>(sB + stage * Cfg::kStageBytesB);
+#pragma unroll
+    for (int k = 0; k < kBlockK / kMmaK; ++k) {
+#pragma unroll
+      for (int h = 0; h < Cfg::kNB; ++h) {
+        ptx::mma_bf16_cg2(d_tmem + h * 256u, a_desc + k * kDescStep<A_MN>,
+                          b_desc + (h * Cfg::kBlockBytesB >> 4) + k * kDescStep<B_MN>, kFfnIdesc<A_MN, B_MN>,
+                          (kb > 0 || k > 0) ? 1u : 0u);
+      }
+    }
+    ptx::mma_commit_cg2(own_empty0 + 8 * stage);
+    ptx::mma_commit_cg2(peer_empty0 + 8 * stage);
+    if (++stage == Cfg::kStages) {
+      stage = 0;
+      phase ^= 1u;
+    }
+  }
+  return true;
+}
+
 template <class Cfg>
 __global__ void __launch_bounds__(Cfg::kThreads, 1) __cluster_dims__(2, 1, 1)
-    ffn_gemm_sm100(const __grid_constant__ CUtensorMap map_a0, const __grid_constant__ CUtensorMap map_a1,
-                   const __grid_constant__ CUtensorMap map_b0, const __grid_constant__ CUtensorMap map_b1,
-                   const __grid_constant__ CUtensorMap map_c0, const __grid_constant__ CUtensorMap map_c1,
-                   const __grid_constant__ CUtensorMap map_c2, const FfnParams p) {
+    ffn_gemm_sm100(const __grid_constant__ FfnMaps maps, const FfnParams p) {
   constexpr int STAGES = Cfg::kStages;
   constexpr int NB = Cfg::kNB;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -234,7 +315,6 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1) __cluster_dims__(2, 1, 1)
   const bool leader = rank == 0;
   const int cluster = static_cast<int>(ptx::cluster_id_x());
   const int nclusters = static_cast<int>(ptx::num_clusters_x());
-  const int all_tiles_m = Cfg::kKind == kDw ? 2 * p.tiles_m : p.tiles_m;
 
   const uint32_t sA = base + Cfg::kA, sB = base + Cfg::kB, sC = base + Cfg::kC;
   const uint32_t full0 = base + Cfg::kFull, empty0 = base + Cfg::kEmpty;
@@ -259,9 +339,9 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1) __cluster_dims__(2, 1, 1)
     }
     ptx::mbar_init(drain, 1);
     ptx::fence_mbar_init_cluster();
-    ptx::prefetch_tensormap(&map_a0);
-    ptx::prefetch_tensormap(&map_b0);
-    ptx::prefetch_tensormap(&map_c0);
+    ptx::prefetch_tensormap(&maps.a0);
+    ptx::prefetch_tensormap(&maps.b0);
+    ptx::prefetch_tensormap(&maps.c[0]);
   }
   if (warp == 1) {
     ptx::tmem_alloc_cg2(tmem_slot, kTmemCols);
@@ -272,6 +352,10 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1) __cluster_dims__(2, 1, 1)
   ptx::tc_fence_after();
   uint32_t tmem_base;
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem_base) : "r"(tmem_slot) : "memory");
+  // The gradients are launched to overlap the kernel that makes dG and dU:
+  // the set-up above runs during its tail, and nothing global is touched
+  // before it is complete.
+  ptx::griddep_wait();
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
@@ -280,38 +364,41 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1) __cluster_dims__(2, 1, 1)
       const uint32_t full_leader0 = ptx::mapa(full0, 0);
       uint32_t stage = 0, phase = 0;
       bool ok = true;
-      for (int t = cluster; t < p.num_tiles && ok; t += nclusters) {
-        int tm, tn;
-        ffn_tile(p, all_tiles_m, t, tm, tn);
-        const bool second = Cfg::kKind == kDw && tm >= p.tiles_m;  // dWu's rows
-        if (second) tm -= p.tiles_m;
-        const int row_a = tm * kTileM + static_cast<int>(rank) * 128;
-        const int row_b = tn * Cfg::kTileN + ((Cfg::kKind == kGated && NB == 1) ? 0 : static_cast<int>(rank) * 128);
-        for (int kb = 0; kb < p.num_kb; ++kb) {
-          if (!ptx::mbar_wait(empty0 + 8 * stage, phase ^ 1u, wd, kSiteProducer, static_cast<unsigned>(t))) {
+      FfnUnit u;
+      for (int i = 0; ok && ffn_unit<Cfg::kKind>(p, cluster, nclusters, i, u); ++i) {
+        const int row_a = u.tm * kTileM + static_cast<int>(rank) * 128;
+        const int row_b = u.tn * Cfg::kTileN + ((Cfg::kKind == kGated && NB == 1) ? 0 : static_cast<int>(rank) * 128);
+        const int num_kb = u.second ? p.second.num_kb : p.first.num_kb;
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!ptx::mbar_wait(empty0 + 8 * stage, phase ^ 1u, wd, kSiteProducer, static_cast<unsigned>(i))) {
             ok = false;
             break;
           }
           if (leader) ptx::mbar_arrive_expect_tx(full0 + 8 * stage, Cfg::kTxBytes);
           const uint32_t fb = full_leader0 + 8 * stage;
-          const bool seg1 = Cfg::kKind == kDx && kb >= p.seg_kb;
-          const int k = (seg1 ? kb - p.seg_kb : kb) * kBlockK;
-          const CUtensorMap* ma = (second || seg1) ? &map_a1 : &map_a0;
           const uint32_t da = sA + stage * kStageBytesA, db = sB + stage * Cfg::kStageBytesB;
-          if constexpr (Cfg::kAMn) {
-            ptx::tma_load_2d_cg2(da, ma, fb, row_a, k, policy);
-            ptx::tma_load_2d_cg2(da + 8192, ma, fb, row_a + 64, k, policy);
-          } else {
-            ptx::tma_load_2d_cg2(da, ma, fb, k, row_a, policy);
-          }
+          if constexpr (Cfg::kKind == kGated) {
+            ptx::tma_load_2d_cg2(da, &maps.a0, fb, kb * kBlockK, row_a, policy);
 #pragma unroll
-          for (int h = 0; h < NB; ++h) {
-            const uint32_t d = db + h * Cfg::kBlockBytesB;
-            if constexpr (Cfg::kKind == kGated) {
+            for (int h = 0; h < NB; ++h) {
               const bool up = NB == 2 ? h == 1 : rank == 1;
-              ptx::tma_load_2d_cg2(d, up ? &map_b1 : &map_b0, fb, k, row_b, policy);
+              ptx::tma_load_2d_cg2(db + h * Cfg::kBlockBytesB, up ? &maps.b1 : &maps.b0, fb, kb * kBlockK, row_b,
+                                   policy);
+            }
+          } else {
+            const bool seg1 = !u.second && kb >= p.seg_kb;
+            const int k = (seg1 ? kb - p.seg_kb : kb) * kBlockK;
+            if (u.second) {
+              const CUtensorMap* ma = u.up ? &maps.w1 : &maps.w0;
+              ptx::tma_load_2d_cg2(da, ma, fb, row_a, k, policy);
+              ptx::tma_load_2d_cg2(da + 8192, ma, fb, row_a + 64, k, policy);
             } else {
-              const CUtensorMap* mb = seg1 ? &map_b1 : &map_b0;
+              ptx::tma_load_2d_cg2(da, seg1 ? &maps.a1 : &maps.a0, fb, k, row_a, policy);
+            }
+            const CUtensorMap* mb = u.second ? &maps.x : (seg1 ? &maps.b1 : &maps.b0);
+#pragma unroll
+            for (int h = 0; h < NB; ++h) {
+              const uint32_t d = db + h * Cfg::kBlockBytesB;
               ptx::tma_load_2d_cg2(d, mb, fb, row_b + h * 256, k, policy);
               ptx::tma_load_2d_cg2(d + 8192, mb, fb, row_b + h * 256 + 64, k, policy);
             }
@@ -330,34 +417,22 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1) __cluster_dims__(2, 1, 1)
       const uint32_t own_empty0 = ptx::mapa(empty0, 0), peer_empty0 = ptx::mapa(empty0, 1);
       const uint32_t own_tfull0 = ptx::mapa(tfull0, 0), peer_tfull0 = ptx::mapa(tfull0, 1);
       uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
-      bool ok = true;
-      for (int t = cluster; t < p.num_tiles && ok; t += nclusters) {
-        if (!ptx::mbar_wait(tempty0 + 8 * acc, acc_phase ^ 1u, wd, kSiteMmaTmemEmpty, static_cast<unsigned>(t))) break;
+      FfnUnit u;
+      for (int i = 0; ffn_unit<Cfg::kKind>(p, cluster, nclusters, i, u); ++i) {
+        const unsigned int unit = static_cast<unsigned int>(i);
+        if (!ptx::mbar_wait(tempty0 + 8 * acc, acc_phase ^ 1u, wd, kSiteMmaTmemEmpty, unit)) break;
         ptx::tc_fence_after();
         const uint32_t d_tmem = tmem_base + acc * 256u;
-        for (int kb = 0; kb < p.num_kb; ++kb) {
-          if (!ptx::mbar_wait(full0 + 8 * stage, phase, wd, kSiteMmaFull, static_cast<unsigned>(t))) {
-            ok = false;
-            break;
-          }
-          ptx::tc_fence_after();
-          const uint64_t a_desc = ffn_desc<Cfg::kAMn>(sA + stage * kStageBytesA);
-          const uint64_t b_desc = ffn_desc<Cfg::kBMn>(sB + stage * Cfg::kStageBytesB);
-#pragma unroll
-          for (int k = 0; k < kBlockK / kMmaK; ++k) {
-#pragma unroll
-            for (int h = 0; h < NB; ++h) {
-              ptx::mma_bf16_cg2(d_tmem + h * 256u, a_desc + k * kDescStep<Cfg::kAMn>,
-                                b_desc + (h * Cfg::kBlockBytesB >> 4) + k * kDescStep<Cfg::kBMn>, Cfg::kIdesc,
-                                (kb > 0 || k > 0) ? 1u : 0u);
-            }
-          }
-          ptx::mma_commit_cg2(own_empty0 + 8 * stage);
-          ptx::mma_commit_cg2(peer_empty0 + 8 * stage);
-          if (++stage == STAGES) {
-            stage = 0;
-            phase ^= 1u;
-          }
+        bool ok;
+        if constexpr (Cfg::kKind == kGated) {
+          ok = ffn_mma_tile<Cfg, false, false>(sA, sB, full0, own_empty0, peer_empty0, d_tmem, p.first.num_kb, stage,
+                                               phase, wd, unit);
+        } else if (u.second) {
+          ok = ffn_mma_tile<Cfg, true, true>(sA, sB, full0, own_empty0, peer_empty0, d_tmem, p.second.num_kb, stage,
+                                             phase, wd, unit);
+        } else {
+          ok = ffn_mma_tile<Cfg, false, true>(sA, sB, full0, own_empty0, peer_empty0, d_tmem, p.first.num_kb, stage,
+                                              phase, wd, unit);
         }
         if (!ok) break;
         ptx::mma_commit_cg2(own_tfull0 + 8 * acc);
@@ -383,14 +458,11 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1) __cluster_dims__(2, 1, 1)
     const uint32_t cstage0 = sC + e * Cfg::kCBufs * kCStageBytes;
     const uint32_t tempty_leader0 = ptx::mapa(tempty0, 0);
     uint32_t acc = 0, acc_phase = 0, cbuf = 0;
-    for (int t = cluster; t < p.num_tiles; t += nclusters) {
-      int tm, tn;
-      ffn_tile(p, all_tiles_m, t, tm, tn);
-      const bool second = Cfg::kKind == kDw && tm >= p.tiles_m;
-      if (second) tm -= p.tiles_m;
-      const int row = tm * kTileM + static_cast<int>(rank) * 128 + static_cast<int>(quarter) * 32;
-      const int col0 = tn * Cfg::kTileN + static_cast<int>(nblk) * Cfg::kWarpCols;
-      const bool full_ok = ptx::mbar_wait(tfull0 + 8 * acc, acc_phase, wd, kSiteEpilogue, static_cast<unsigned>(t));
+    FfnUnit u;
+    for (int i = 0; ffn_unit<Cfg::kKind>(p, cluster, nclusters, i, u); ++i) {
+      const int row = u.tm * kTileM + static_cast<int>(rank) * 128 + static_cast<int>(quarter) * 32;
+      const int col0 = u.tn * Cfg::kTileN + static_cast<int>(nblk) * Cfg::kWarpCols;
+      const bool full_ok = ptx::mbar_wait(tfull0 + 8 * acc, acc_phase, wd, kSiteEpilogue, static_cast<unsigned>(i));
       if (!__all_sync(0xFFFFFFFFu, full_ok)) break;
       ptx::tc_fence_after();
       const uint32_t t_row = tmem_base + ((quarter * 32u) << 16) + acc * 256u + nblk * Cfg::kWarpCols;
@@ -400,40 +472,87 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1) __cluster_dims__(2, 1, 1)
         if (lane == 0) ptx::mbar_arrive_cluster(tempty_leader0 + 8 * acc);
       };
       if constexpr (Cfg::kKind == kGated) {
+        const int M = p.first.M, N = p.first.N;
         constexpr uint32_t kUp = 128u * NB;  // U's columns follow G's
 #pragma unroll 1
         for (int c = 0; c < Cfg::kWarpChunks; ++c) {
-          uint32_t g[32], u[32], w[16];
+          uint32_t g[32], v[32], w[16];
           ptx::tmem_ld_32x32b_x32(t_row + c * kCBoxCols, g);
-          ptx::tmem_ld_32x32b_x32(t_row + kUp + c * kCBoxCols, u);
+          ptx::tmem_ld_32x32b_x32(t_row + kUp + c * kCBoxCols, v);
           ptx::tmem_wait_ld();
           ptx::reg_fence32(g);
-          ptx::reg_fence32(u);
+          ptx::reg_fence32(v);
           if (c == Cfg::kWarpChunks - 1) release();
           const int col = col0 + c * kCBoxCols;
-          ffn_combine(p.act, g, u, w);
-          ffn_store_chunk<Cfg::kCBufs>(w, col, row, lane, cstage0, cbuf, map_c0, p.out[0], p.M, p.N);
+          ffn_combine(p.act, g, v, w);
+          ffn_store_chunk<Cfg::kCBufs>(w, col, row, lane, cstage0, cbuf, maps.c[0], p.out[0], M, N);
           if (p.save) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) w[i] = ptx::pack_bf16x2(g[2 * i], g[2 * i + 1]);
-            ffn_store_chunk<Cfg::kCBufs>(w, col, row, lane, cstage0, cbuf, map_c1, p.out[1], p.M, p.N);
+            for (int j = 0; j < 16; ++j) w[j] = ptx::pack_bf16x2(g[2 * j], g[2 * j + 1]);
+            ffn_store_chunk<Cfg::kCBufs>(w, col, row, lane, cstage0, cbuf, maps.c[1], p.out[1], M, N);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) w[i] = ptx::pack_bf16x2(u[2 * i], u[2 * i + 1]);
-            ffn_store_chunk<Cfg::kCBufs>(w, col, row, lane, cstage0, cbuf, map_c2, p.out[2], p.M, p.N);
+            for (int j = 0; j < 16; ++j) w[j] = ptx::pack_bf16x2(v[2 * j], v[2 * j + 1]);
+            ffn_store_chunk<Cfg::kCBufs>(w, col, row, lane, cstage0, cbuf, maps.c[2], p.out[2], M, N);
           }
         }
       } else {
-#pragma unroll 1
-        for (int c = 0; c < Cfg::kWarpChunks; ++c) {
-          uint32_t v[32], w[16];
-          ptx::tmem_ld_32x32b_x32(t_row + c * kCBoxCols, v);
-          ptx::tmem_wait_ld();
-          ptx::reg_fence32(v);
-          if (c == Cfg::kWarpChunks - 1) release();
+        const int which = u.second ? (u.up ? 2 : 1) : 0;
+        const int M = u.second ? p.second.M : p.first.M, N = p.first.N;  // (N is K for all three)
+        const CUtensorMap* map = &maps.c[which];
+        constexpr int kHeld = Cfg::kWarpChunks - Cfg::kCBufs;
+        if (NB == 2 && row < M && col0 + Cfg::kWarpCols <= N) {
+          // The single accumulator holds the next tile's MMAs up until it is
+          // read: half of a warp's chunks go into its staging buffers and half
+          // into registers, then it is released, then the stores are issued.
+          if (lane == 0) ptx::bulk_wait_group_read<0>();
+          __syncwarp();
+          uint32_t held[kHeld > 0 ? kHeld : 1][16];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) w[i] = ptx::pack_bf16x2(v[2 * i], v[2 * i + 1]);
-          ffn_store_chunk<Cfg::kCBufs>(w, col0 + c * kCBoxCols, row, lane, cstage0, cbuf,
-                                       second ? map_c1 : map_c0, second ? p.out[1] : p.out[0], p.M, p.N);
+          for (int c = 0; c < Cfg::kWarpChunks; c += 2) {
+            uint32_t v0[32], v1[32];
+            ptx::tmem_ld_32x32b_x32(t_row + c * kCBoxCols, v0);
+            ptx::tmem_ld_32x32b_x32(t_row + (c + 1) * kCBoxCols, v1);
+            ptx::tmem_wait_ld();
+            ptx::reg_fence32(v0);
+            ptx::reg_fence32(v1);
+            if (c < Cfg::kCBufs) {
+              stage_chunk_row_f32(cstage0 + c * kCStageBytes, lane, v0);
+              stage_chunk_row_f32(cstage0 + (c + 1) * kCStageBytes, lane, v1);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 16; ++j) {
+                held[c - Cfg::kCBufs][j] = ptx::pack_bf16x2(v0[2 * j], v0[2 * j + 1]);
+                held[c + 1 - Cfg::kCBufs][j] = ptx::pack_bf16x2(v1[2 * j], v1[2 * j + 1]);
+              }
+            }
+          }
+          release();
+          ptx::fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+#pragma unroll
+            for (int c = 0; c < Cfg::kCBufs; ++c) {
+              ptx::tma_store_2d(map, cstage0 + c * kCStageBytes, col0 + c * kCBoxCols, row);
+              ptx::bulk_commit_group();
+            }
+          }
+          cbuf = 0;
+#pragma unroll
+          for (int c = 0; c < kHeld; ++c)
+            ffn_store_chunk<Cfg::kCBufs>(held[c], col0 + (Cfg::kCBufs + c) * kCBoxCols, row, lane, cstage0, cbuf, *map,
+                                         p.out[which], M, N);
+        } else {
+#pragma unroll 1
+          for (int c = 0; c < Cfg::kWarpChunks; ++c) {
+            uint32_t v[32], w[16];
+            ptx::tmem_ld_32x32b_x32(t_row + c * kCBoxCols, v);
+            ptx::tmem_wait_ld();
+            ptx::reg_fence32(v);
+            if (c == Cfg::kWarpChunks - 1) release();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) w[j] = ptx::pack_bf16x2(v[2 * j], v[2 * j + 1]);
+            ffn_store_chunk<Cfg::kCBufs>(w, col0 + c * kCBoxCols, row, lane, cstage0, cbuf, *map, p.out[which], M, N);
+          }
         }
       }
       if (++acc == Cfg::kAccBufs) {
@@ -468,6 +587,7 @@ struct GatedGradParams {
 
 template <int ACT>
 __global__ void __launch_bounds__(256) gated_grad_kernel(const GatedGradParams p) {
+  ptx::griddep_launch_dependents();  // the products' kernel may set itself up; it waits for this one's end
   const int col = static_cast<int>(blockIdx.x * 256u + threadIdx.x) * 8;
   if (col >= p.F) return;
   for (long long r = blockIdx.y; r < p.M; r += gridDim.y) {
