@@ -13,11 +13,12 @@
 
 #include "b200gemm.h"
 #include "ffn_sm100.cuh"
+#include "gated_decode_sm100.cuh"
 #include "gemm_decode_sm100.cuh"
 #include "gemm_sm100.cuh"
 #include "gemm_smallm1_sm100.cuh"
 #include "schedule.cuh"
-#include "skinny_sm100.cuh"
+#include "w4_sm100.cuh"
 
 namespace b200gemm {
 
@@ -460,6 +461,7 @@ struct b200gemm_handle {
   int decode_clusters[5] = {};        // [S]: co-resident clusters of the small-M pair kernel, split S
   int decode256_clusters[5] = {};     // the same for its instances covering 256 rows of A
   int smallm1_clusters[5] = {};       // [S]: the same for the single-CTA small-M kernel
+  int w4_clusters[4] = {};            // [i]: co-resident clusters of 2^i CTAs of the 4-bit product
   int ffn_clusters = 0;               // co-resident clusters of the tiled feed-forward kernels
   int tile_width = 0;         // 0 = choose per call, else one of kWidths
   int small_m = -1;           // small-M kernel: -1 or 1 = use it when eligible, 0 = never
@@ -488,7 +490,9 @@ struct b200gemm_handle {
 
 namespace b200gemm {
 int prepare_ffn_kernels(int sm_count);
-bool prepare_all_skinny_kernels();
+bool prepare_gated_decode_kernels();
+bool prepare_w4_kernels();
+int w4_clusters_fit(int sm_count, int split);
 }  // namespace b200gemm
 
 extern "C" int b200gemm_version(void) { return kVersion; }
@@ -540,7 +544,10 @@ extern "C" int b200gemm_create(b200gemm_t* out, int device) {
   const int sc2 = prepare_smallm1_kernel<SmallMCfg<2>>(sms), sc4 = prepare_smallm1_kernel<SmallMCfg<4>>(sms);
   if (sc2 <= 0 || sc4 <= 0) return B200GEMM_ERR_CUDA;
   const int fc = prepare_ffn_kernels(sms);
-  if (fc <= 0 || !prepare_all_skinny_kernels()) return B200GEMM_ERR_CUDA;
+  if (fc <= 0 || !prepare_gated_decode_kernels() || !prepare_w4_kernels()) return B200GEMM_ERR_CUDA;
+  int w4_fit[4];
+  for (int i = 0; i < 4; ++i)
+    if ((w4_fit[i] = w4_clusters_fit(sms, 1 << i)) <= 0) return B200GEMM_ERR_CUDA;
 
   auto* h = new b200gemm_handle();
   h->device = device;
@@ -555,6 +562,7 @@ extern "C" int b200gemm_create(b200gemm_t* out, int device) {
   h->smallm1_clusters[2] = sc2;
   h->smallm1_clusters[4] = sc4;
   h->ffn_clusters = fc;
+  for (int i = 0; i < 4; ++i) h->w4_clusters[i] = w4_fit[i];
   h->max_clusters = cw[0];
   for (int i = 0; i < kNumWidths; ++i) {
     h->clusters_w[i] = cw[i];

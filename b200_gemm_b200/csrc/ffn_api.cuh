@@ -1,6 +1,6 @@
 // Host side of the feed-forward entry points of include/b200gemm.h: argument
-// checks, plans and launches of the kernels in ffn_sm100.cuh and
-// skinny_sm100.cuh.  Part of b200gemm.cu's translation unit (it uses the
+// checks, plans and launches of the kernels in ffn_sm100.cuh,
+// gated_decode_sm100.cuh and w4_sm100.cuh.  Part of b200gemm.cu's translation unit (it uses the
 // handle and the helpers there).  Nothing here allocates, builds a table or
 // waits, so every call can be captured into a CUDA graph from the first one.
 #pragma once
@@ -50,26 +50,66 @@ int prepare_ffn_kernels(int sm_count) {
   return least;
 }
 
-template <class Cfg>
-bool prepare_skinny_kernel() {
-  if (cudaFuncSetAttribute(skinny_sm100<Cfg>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes) !=
-      cudaSuccess) {
-    cudaGetLastError();
-    return false;
+template <class Kernel>
+bool opt_in_smem(Kernel kernel, int bytes) {
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess) return true;
+  cudaGetLastError();
+  return false;
+}
+
+bool prepare_gated_decode_kernels() {
+  return opt_in_smem(gated_decode_sm100<GatedDecodeCfg<1>>, GatedDecodeCfg<1>::kSmemBytes) &&
+         opt_in_smem(gated_decode_sm100<GatedDecodeCfg<2>>, GatedDecodeCfg<2>::kSmemBytes) &&
+         opt_in_smem(gated_decode_sm100<GatedDecodeCfg<4>>, GatedDecodeCfg<4>::kSmemBytes);
+}
+
+// Instances of the 4-bit product: 16-row tiles of W per warp (MT) that its
+// registers and ring allow next to NT tiles of X's rows.
+template <int NT>
+constexpr int kW4MaxMT = NT == 1 ? 7 : (NT == 2 ? 5 : 3);
+
+template <bool GATED, bool G32, int NT, int MT = kW4MaxMT<NT>>
+bool prepare_w4_instances() {
+  if constexpr (MT == 0) {
+    return true;
+  } else {
+    using Cfg = W4NtCfg<GATED, G32, MT, NT>;
+    return opt_in_smem(w4_nt_sm100<Cfg>, Cfg::kSmemBytes) && prepare_w4_instances<GATED, G32, NT, MT - 1>();
   }
-  return true;
 }
 
-template <bool W4, bool GATED, bool G32>
-bool prepare_skinny_kernels() {
-  return prepare_skinny_kernel<SkinnyCfg<W4, GATED, 1, G32>>() && prepare_skinny_kernel<SkinnyCfg<W4, GATED, 2, G32>>() &&
-         prepare_skinny_kernel<SkinnyCfg<W4, GATED, 4, G32>>();
+template <bool GATED, bool G32>
+bool prepare_w4_nt() {
+  return prepare_w4_instances<GATED, G32, 1>() && prepare_w4_instances<GATED, G32, 2>() &&
+         prepare_w4_instances<GATED, G32, 4>();
 }
 
-bool prepare_all_skinny_kernels() {
-  return prepare_skinny_kernels<false, true, false>() && prepare_skinny_kernels<true, false, false>() &&
-         prepare_skinny_kernels<true, false, true>() && prepare_skinny_kernels<true, true, false>() &&
-         prepare_skinny_kernels<true, true, true>();
+bool prepare_w4_kernels() {
+  return prepare_w4_nt<false, false>() && prepare_w4_nt<false, true>() && prepare_w4_nt<true, false>() &&
+         prepare_w4_nt<true, true>();
+}
+
+// How many clusters of `split` CTAs of the 4-bit product, which fill an SM
+// each, fit on the device at once.
+int w4_clusters_fit(int sm_count, int split) {
+  using Cfg = W4NtCfg<false, false, 7, 1>;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(split);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3(static_cast<unsigned>(split), static_cast<unsigned>(sm_count / split), 1);
+  cfg.blockDim = dim3(Cfg::kThreads, 1, 1);
+  cfg.dynamicSmemBytes = Cfg::kSmemBytes;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int clusters = 0;
+  if (cudaOccupancyMaxActiveClusters(&clusters, w4_nt_sm100<Cfg>, &cfg) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  return clusters;
 }
 
 template <class Cfg>
@@ -89,18 +129,20 @@ cudaError_t launch_ffn(int clusters, cudaStream_t stream, const FfnMaps& m, cons
   return cudaLaunchKernelEx(&cfg, ffn_gemm_sm100<Cfg>, m, p);
 }
 
-template <class Cfg>
-cudaError_t launch_skinny(int split, int rows, int token_blocks, cudaStream_t stream, const CUtensorMap& w0,
-                          const CUtensorMap& w1, const CUtensorMap& x, const SkinnyParams& p) {
+// Launch of a few-rows kernel: `split` CTAs a cluster, which share K.
+template <class Kernel, class Params>
+cudaError_t launch_rows(Kernel kernel, int threads, int smem, int split, int blocks, int token_blocks,
+                        cudaStream_t stream, const CUtensorMap& w0, const CUtensorMap& w1, const CUtensorMap& x,
+                        const Params& p) {
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = static_cast<unsigned>(split);
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
-  cfg.gridDim = dim3(static_cast<unsigned>(split), static_cast<unsigned>(rows), static_cast<unsigned>(token_blocks));
-  cfg.blockDim = dim3(Cfg::kThreads, 1, 1);
-  cfg.dynamicSmemBytes = Cfg::kSmemBytes;
+  cfg.gridDim = dim3(static_cast<unsigned>(split), static_cast<unsigned>(blocks), static_cast<unsigned>(token_blocks));
+  cfg.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
@@ -109,7 +151,7 @@ cudaError_t launch_skinny(int split, int rows, int token_blocks, cudaStream_t st
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.numAttrs = 2;
   }
-  return cudaLaunchKernelEx(&cfg, skinny_sm100<Cfg>, w0, w1, x, p);
+  return cudaLaunchKernelEx(&cfg, kernel, w0, w1, x, p);
 }
 
 // One matrix of a call, for the overlap check: rows of `width` bytes every
@@ -206,39 +248,30 @@ bool encode_out(CUtensorMap* m, void* ptr, int cols, int rows, long long ld) {
                    kCBoxCols, kCBoxRows, CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
-// K ranges (CTAs of a cluster) of a skinny product: the smallest power of two
-// up to 8 that gives every SM a CTA, while each keeps at least two stages.
-int skinny_split(const b200gemm_handle* h, long long row_blocks, int num_stages) {
+// K ranges (CTAs of a cluster) of the gated block's decode kernel: the smallest
+// power of two up to 8 that gives every SM a CTA, while each CTA's warps keep
+// a stage or two.
+int gated_decode_split(const b200gemm_handle* h, long long blocks, int num_stages) {
   int split = 1;
-  while (split < 8 && row_blocks * split < h->sm_count && num_stages >= 4 * split) split *= 2;
+  while (split < 8 && blocks * split < h->sm_count && num_stages >= 16 * split) split *= 2;
   return split;
 }
 
-template <bool W4, bool GATED, bool G32 = false>
-int run_skinny(b200gemm_t h, const void* w0, const void* w1, long long ldw, const void* X, long long ldx,
-               SkinnyParams p, cudaStream_t stream) {
+int run_gated_decode(b200gemm_t h, const void* Wg, const void* Wu, long long ldw, const void* X, long long ldx,
+                     GatedDecodeParams p, cudaStream_t stream) {
   const int nt = p.M > 16 ? 4 : (p.M > 8 ? 2 : 1);
-  const int cols = GATED ? 32 : 64;
-  const long long row_blocks = (static_cast<long long>(p.N) + cols - 1) / cols;
-  const long long token_blocks = (static_cast<long long>(p.M) + 31) / 32;
-  if (row_blocks > 65535 || token_blocks > 65535) return B200GEMM_ERR_TOO_LARGE;
-  CUtensorMap mw0, mw1, mx;
-  const auto encode_w = [&](CUtensorMap* m, const void* w) {
-    return W4 ? encode_2d(m, w, static_cast<uint64_t>(p.K) / 2, static_cast<uint64_t>(p.N),
-                          static_cast<uint64_t>(p.K) / 2, 128, static_cast<uint32_t>(cols), CU_TENSOR_MAP_SWIZZLE_128B,
-                          CU_TENSOR_MAP_DATA_TYPE_UINT8)
-              : encode_2d(m, w, static_cast<uint64_t>(p.K), static_cast<uint64_t>(p.N),
-                          static_cast<uint64_t>(ldw) * 2, 64, static_cast<uint32_t>(cols), CU_TENSOR_MAP_SWIZZLE_128B);
+  const long long blocks = (static_cast<long long>(p.F) + 31) / 32;
+  if (blocks > 65535) return B200GEMM_ERR_TOO_LARGE;
+  CUtensorMap mg, mu, mx;
+  const auto encode = [&](CUtensorMap* m, const void* ptr, int rows, long long ld, uint32_t box_rows) {
+    return encode_2d(m, ptr, static_cast<uint64_t>(p.K), static_cast<uint64_t>(rows), static_cast<uint64_t>(ld) * 2, 64,
+                     box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
   };
-  if (!encode_w(&mw0, w0) || (GATED && !encode_w(&mw1, w1)) ||
-      !encode_2d(&mx, X, static_cast<uint64_t>(p.K), static_cast<uint64_t>(p.M), static_cast<uint64_t>(ldx) * 2, 64,
-                 static_cast<uint32_t>(8 * nt), CU_TENSOR_MAP_SWIZZLE_128B)) {
+  if (!encode(&mg, Wg, p.F, ldw, 32) || !encode(&mu, Wu, p.F, ldw, 32) ||
+      !encode(&mx, X, p.M, ldx, static_cast<uint32_t>(8 * nt)))
     return B200GEMM_ERR_CUDA;
-  }
-  if (!GATED) mw1 = mw0;
-  const int stage_k = SkinnyCfg<W4, GATED, 1>::kStageK;
-  p.num_stages = (p.K + stage_k - 1) / stage_k;
-  const int split = skinny_split(h, row_blocks * token_blocks, p.num_stages);
+  p.num_stages = (p.K + 63) / 64;
+  const int split = gated_decode_split(h, blocks, p.num_stages);
   p.stages_per_cta = (p.num_stages + split - 1) / split;
   {
     std::lock_guard<std::mutex> lock(h->mu);
@@ -246,11 +279,103 @@ int run_skinny(b200gemm_t h, const void* w0, const void* w1, long long ldw, cons
     p.pdl = h->pdl;
   }
   p.status = h->status_dev;
-  const int rb = static_cast<int>(row_blocks), tb = static_cast<int>(token_blocks);
+  const auto go = [&](auto kernel, int threads, int smem) {
+    return launch_rows(kernel, threads, smem, split, static_cast<int>(blocks), 1, stream, mg, mu, mx, p);
+  };
   const cudaError_t e =
-      nt == 1   ? launch_skinny<SkinnyCfg<W4, GATED, 1, G32>>(split, rb, tb, stream, mw0, mw1, mx, p)
-      : nt == 2 ? launch_skinny<SkinnyCfg<W4, GATED, 2, G32>>(split, rb, tb, stream, mw0, mw1, mx, p)
-                : launch_skinny<SkinnyCfg<W4, GATED, 4, G32>>(split, rb, tb, stream, mw0, mw1, mx, p);
+      nt == 1   ? go(gated_decode_sm100<GatedDecodeCfg<1>>, GatedDecodeCfg<1>::kThreads, GatedDecodeCfg<1>::kSmemBytes)
+      : nt == 2 ? go(gated_decode_sm100<GatedDecodeCfg<2>>, GatedDecodeCfg<2>::kThreads, GatedDecodeCfg<2>::kSmemBytes)
+                : go(gated_decode_sm100<GatedDecodeCfg<4>>, GatedDecodeCfg<4>::kThreads, GatedDecodeCfg<4>::kSmemBytes);
+  return e == cudaSuccess ? B200GEMM_OK : B200GEMM_ERR_CUDA;
+}
+
+// Rows of W per CTA, 16-row tiles per warp and K ranges of a 4-bit product: of
+// the splits of K over clusters of 1, 2, 4 and 8 CTAs, the one with the least
+// estimated time.  Rows are divided evenly over the clusters that fit at once
+// (a second wave only where a CTA's registers and ring cannot hold its share).
+struct W4Plan {
+  int rows = 0, mt = 0, split = 1;
+};
+W4Plan w4_plan(const b200gemm_handle* h, int N, int token_blocks, int num_stages, int max_mt, bool gated) {
+  const int tiles = gated ? 1 : 2;  // 16-row tiles of output per unit of mt
+  W4Plan best;
+  double best_cost = 1e300;
+  for (int i = 0, split = 1; i < 4; ++i, split *= 2) {
+    if (split > 1 && num_stages < 2 * split) break;
+    const int fit = h->w4_clusters[i] / token_blocks > 0 ? h->w4_clusters[i] / token_blocks : 1;
+    const long long per_wave = 16ll * max_mt * tiles * fit;
+    const long long waves = (N + per_wave - 1) / per_wave;
+    const int rows = static_cast<int>((N + waves * fit - 1) / (waves * fit));
+    const int mt = (rows + 16 * tiles - 1) / (16 * tiles);
+    const int stages = (num_stages + split - 1) / split;
+    const double cost = static_cast<double>(waves) * (stages * (mt + 1.0) + (split > 1 ? 10.0 : 6.0));
+    if (cost < best_cost) {
+      best_cost = cost;
+      best.rows = rows;
+      best.mt = mt;
+      best.split = split;
+    }
+  }
+  return best;
+}
+
+struct W4Launch {
+  W4Plan plan;
+  int blocks, token_blocks;
+  cudaStream_t stream;
+  CUtensorMap w0, w1, x;
+};
+
+template <bool GATED, bool G32, int NT, int MT = kW4MaxMT<NT>>
+cudaError_t launch_w4(const W4Launch& l, const W4NtParams& p) {
+  if constexpr (MT == 0) {
+    return cudaErrorInvalidValue;
+  } else {
+    using Cfg = W4NtCfg<GATED, G32, MT, NT>;
+    if (l.plan.mt != MT) return launch_w4<GATED, G32, NT, MT - 1>(l, p);
+    return launch_rows(w4_nt_sm100<Cfg>, Cfg::kThreads, Cfg::kSmemBytes, l.plan.split, l.blocks, l.token_blocks,
+                       l.stream, l.w0, l.w1, l.x, p);
+  }
+}
+
+template <bool GATED>
+int run_w4(b200gemm_t h, const void* w0, const void* w1, const void* X, long long ldx, W4NtParams p,
+           cudaStream_t stream) {
+  const int nt = p.M > 16 ? 4 : (p.M > 8 ? 2 : 1);
+  const long long token_blocks = (static_cast<long long>(p.M) + 31) / 32;
+  if (token_blocks > 65535) return B200GEMM_ERR_TOO_LARGE;
+  p.num_stages = static_cast<int>((static_cast<long long>(p.K) + 511) / 512);
+  W4Launch l;
+  l.token_blocks = static_cast<int>(token_blocks);
+  l.stream = stream;
+  l.plan = w4_plan(h, p.N, l.token_blocks, p.num_stages, nt == 1 ? kW4MaxMT<1> : (nt == 2 ? kW4MaxMT<2> : kW4MaxMT<4>),
+                   GATED);
+  l.blocks = (p.N + l.plan.rows - 1) / l.plan.rows;
+  if (l.blocks > 65535) return B200GEMM_ERR_TOO_LARGE;
+  p.rows = l.plan.rows;
+  p.stages_per_cta = (p.num_stages + l.plan.split - 1) / l.plan.split;
+  const auto encode_w = [&](CUtensorMap* map, const void* w) {
+    return encode_2d(map, w, static_cast<uint64_t>(p.K) / 2, static_cast<uint64_t>(p.N), static_cast<uint64_t>(p.K) / 2,
+                     128, static_cast<uint32_t>((GATED ? 16 : 32) * l.plan.mt), CU_TENSOR_MAP_SWIZZLE_128B,
+                     CU_TENSOR_MAP_DATA_TYPE_UINT8);
+  };
+  if (!encode_w(&l.w0, w0) || (GATED && !encode_w(&l.w1, w1)) ||
+      !encode_2d(&l.x, X, static_cast<uint64_t>(p.K), static_cast<uint64_t>(p.M), static_cast<uint64_t>(ldx) * 2, 256,
+                 static_cast<uint32_t>(8 * nt), CU_TENSOR_MAP_SWIZZLE_NONE)) {
+    return B200GEMM_ERR_CUDA;
+  }
+  if (!GATED) l.w1 = l.w0;
+  {
+    std::lock_guard<std::mutex> lock(h->mu);
+    p.timeout_ns = h->timeout_ns;
+    p.pdl = h->pdl;
+  }
+  p.status = h->status_dev;
+  cudaError_t e;
+  if (p.group_shift == 5)
+    e = nt == 1 ? launch_w4<GATED, true, 1>(l, p) : nt == 2 ? launch_w4<GATED, true, 2>(l, p) : launch_w4<GATED, true, 4>(l, p);
+  else
+    e = nt == 1 ? launch_w4<GATED, false, 1>(l, p) : nt == 2 ? launch_w4<GATED, false, 2>(l, p) : launch_w4<GATED, false, 4>(l, p);
   return e == cudaSuccess ? B200GEMM_OK : B200GEMM_ERR_CUDA;
 }
 
@@ -320,15 +445,14 @@ extern "C" int b200gemm_bf16_gated(b200gemm_t h, int M, int F, int K, const void
     nb = ffn_gated_nb(h, (M + kTileM - 1) / kTileM, F, num_kb);
   }
   if (small) {
-    SkinnyParams p{};
+    GatedDecodeParams p{};
     p.M = M;
-    p.N = F;
+    p.F = F;
     p.K = K;
     p.act = activation;
-    p.out_type = kOutBf16;
-    p.out = H;
+    p.out = static_cast<uint16_t*>(H);
     p.ldo = ldh;
-    return run_skinny<false, true>(h, Wg, Wu, ldw, X, ldx, p, stream);
+    return run_gated_decode(h, Wg, Wu, ldw, X, ldx, p, stream);
   }
   FfnMaps m;
   if (!encode_kmajor(&m.a0, X, K, M, ldx) || !encode_kmajor(&m.b0, Wg, K, F, ldw) ||
@@ -525,7 +649,7 @@ extern "C" int b200gemm_w4_nt(b200gemm_t h, int M, int N, int K, const void* A, 
   if (M == 0 || N == 0) return B200GEMM_OK;
   if (K == 0) return B200GEMM_ERR_UNSUPPORTED;
   if (A == nullptr || codes == nullptr || scales == nullptr || C == nullptr) return B200GEMM_ERR_INVALID_ARG;
-  SkinnyParams p{};
+  W4NtParams p{};
   const int rc = w4_product_check(K, group, lda, A, &p.group_shift);
   if (rc != B200GEMM_OK) return rc;
   const int esize = out_type == B200GEMM_OUT_F32 ? 4 : 2;
@@ -547,9 +671,7 @@ extern "C" int b200gemm_w4_nt(b200gemm_t h, int M, int N, int K, const void* A, 
   p.scales0 = static_cast<const uint16_t*>(scales);
   p.out = C;
   p.ldo = ldc;
-  const cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
-  return group == 32 ? run_skinny<true, false, true>(h, codes, nullptr, 0, A, lda, p, stream)
-                     : run_skinny<true, false>(h, codes, nullptr, 0, A, lda, p, stream);
+  return run_w4<false>(h, codes, nullptr, A, lda, p, static_cast<cudaStream_t>(stream_ptr));
 }
 
 extern "C" int b200gemm_w4_gated(b200gemm_t h, int M, int F, int K, const void* X, long long ldx,
@@ -562,7 +684,7 @@ extern "C" int b200gemm_w4_gated(b200gemm_t h, int M, int F, int K, const void* 
   if (X == nullptr || gate_codes == nullptr || gate_scales == nullptr || up_codes == nullptr || up_scales == nullptr ||
       H == nullptr)
     return B200GEMM_ERR_INVALID_ARG;
-  SkinnyParams p{};
+  W4NtParams p{};
   const int rc = w4_product_check(K, group, ldx, X, &p.group_shift);
   if (rc != B200GEMM_OK) return rc;
   if (ldh < F || !aligned16(gate_codes) || !aligned16(up_codes) || !aligned2(gate_scales) || !aligned2(up_scales) ||
@@ -585,7 +707,5 @@ extern "C" int b200gemm_w4_gated(b200gemm_t h, int M, int F, int K, const void* 
   p.scales1 = static_cast<const uint16_t*>(up_scales);
   p.out = H;
   p.ldo = ldh;
-  const cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
-  return group == 32 ? run_skinny<true, true, true>(h, gate_codes, up_codes, 0, X, ldx, p, stream)
-                     : run_skinny<true, true>(h, gate_codes, up_codes, 0, X, ldx, p, stream);
+  return run_w4<true>(h, gate_codes, up_codes, X, ldx, p, static_cast<cudaStream_t>(stream_ptr));
 }
