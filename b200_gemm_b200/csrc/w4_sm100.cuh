@@ -69,6 +69,10 @@ struct W4NtCfg {
   static constexpr int kMT = MT;
   static constexpr int kNT = NT;
   static constexpr int kTok = 8 * NT;
+  // Whether the 136 too much come off the sum (see above) or, with 17 to 32
+  // rows of X, off the weights: there the registers and the products that the
+  // sum's start takes outweigh eight subtractions per row tile.
+  static constexpr bool kFromSum = NT < 4;
   static constexpr int kHalf = 16 * MT;                // weight rows of one half of the warps
   static constexpr int kWarps = 16;
   static constexpr int kThreads = 32 * kWarps;
@@ -123,6 +127,12 @@ __device__ __forceinline__ void w4_expand(uint32_t w, const W4Const& k, uint32_t
   for (int j = 0; j < 4; ++j)
     asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(v[j]) : "r"(w >> (4 * j)), "r"(k.mask), "r"(k.magic));
 }
+// A pair of 128 + q less 136: exact.
+__device__ __forceinline__ uint32_t w4_less_136(uint32_t v) {
+  const __nv_bfloat162 offset = __halves2bfloat162(__ushort_as_bfloat16(0x4308), __ushort_as_bfloat16(0x4308));
+  const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), offset);
+  return *reinterpret_cast<const uint32_t*>(&d);
+}
 constexpr uint32_t kMinus136 = 0xC308C308u;  // a bf16 pair of -136
 
 template <class Cfg>
@@ -169,26 +179,27 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
 
   const uint32_t half = warp >> 3, part = warp & 7u;  // rows, and k's 64 part .. of every stage
   // Scales of this warp's rows for its k's of the next stage (one or two
-  // groups), loaded one stage ahead: lane l holds rows l, l + 32, ..  (Rows
-  // past N take the last row's: their sums are not written.)  The first ones
-  // are asked for before the ring's copies, which would keep them waiting for
-  // microseconds.
+  // groups), loaded one stage ahead: lane l holds rows l, l + 32, ..  The
+  // first ones are asked for before the ring's copies, which would keep them
+  // waiting for microseconds.
   constexpr int kHold = (Cfg::kHalf + 31) / 32, kSets = Cfg::kG32 ? 2 : 1;
   uint32_t next_sc[kSets][kHold] = {};
-  const uint16_t* scales = (Cfg::kGatedOut && half == 1) ? p.scales1 : p.scales0;
   const int row0 = n0 + (Cfg::kGatedOut ? 0 : static_cast<int>(half) * Cfg::kHalf) + static_cast<int>(lane);
-  auto load_scales = [&](int it) {
+  const uint16_t* scales = ((Cfg::kGatedOut && half == 1) ? p.scales1 : p.scales0) + row0;
+  int k_next = s_begin * Cfg::kStageK + static_cast<int>(part) * 64;
+  const int k_end = min(p.K, (s_begin + count) * Cfg::kStageK);  // past it: scale 0 (past K X is 0)
+  auto load_scales = [&]() {
 #pragma unroll
     for (int e = 0; e < kSets; ++e) {
-      const int k = (s_begin + it) * Cfg::kStageK + static_cast<int>(part) * 64 + 32 * e;
-      const bool in_k = it < count && k < p.K;  // past K: scale 0 (X is 0 there)
-      const uint16_t* src = scales + static_cast<long long>(k >> p.group_shift) * p.N;
+      const bool in_k = k_next + 32 * e < k_end;
+      const uint16_t* src = scales + static_cast<long long>((k_next + 32 * e) >> p.group_shift) * p.N;
 #pragma unroll
-      for (int r = 0; r < kHold; ++r) next_sc[e][r] = in_k ? __ldg(src + min(row0 + 32 * r, p.N - 1)) : 0;
+      for (int r = 0; r < kHold; ++r) next_sc[e][r] = in_k && row0 + 32 * r < p.N ? __ldg(src + 32 * r) : 0;
     }
+    k_next += Cfg::kStageK;
   };
   if (p.pdl != kPdlWeightsEarly) ptx::griddep_wait();
-  load_scales(0);
+  load_scales();
   if (threadIdx.x == 0) {
     asm volatile("st.shared.u32 [%0], 0;" ::"r"(wd.abort_flag) : "memory");
     for (int s = 0; s < RING; ++s) {
@@ -247,57 +258,92 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
         const uint32_t s = next_sc[e][r];
         sc[e][r] = __uint_as_float((s & 0x7F80u) == 0x7F80u ? 0x7FC00000u : s << 16);
       }
-    load_scales(it + 1);
+    load_scales();
     const bool got = ptx::mbar_wait_cta(full0 + 8 * stage, phase, wd, kSiteEpilogue, blockIdx.y);
     if (!__all_sync(0xFFFFFFFFu, got)) break;
     if ((s_begin + it) * Cfg::kStageK + static_cast<int>(part) * 64 < p.K) {
       const uint32_t aw = ring + stage * Cfg::kStageBytes + off_w;
       const uint32_t ax = ring + stage * Cfg::kStageBytes + off_x;
-      // X's 8 k's of this lane in both 32-k chunks, for every tile of tokens,
-      // as pairs (k_j, k_j+4) like the weights'; and -136 times their sum.
-      uint32_t x[2][NT][4];
-      float start[kSets][NT][4];
+      // X's 8 k's of this lane in chunk e of 32, as pairs (k_j, k_j+4) like the
+      // weights'.
+      auto load_x = [&](int e, uint32_t (&x)[NT][4]) {
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
+        for (int j = 0; j < NT; ++j) {
           uint32_t x0, x1, x2, x3;
           ptx::ld_shared_v4(ax + 64u * e + j * 4096u, x0, x1, x2, x3);
-          x[e][j][0] = __byte_perm(x0, x2, 0x5410);
-          x[e][j][1] = __byte_perm(x0, x2, 0x7632);
-          x[e][j][2] = __byte_perm(x1, x3, 0x5410);
-          x[e][j][3] = __byte_perm(x1, x3, 0x7632);
-          float (&s)[4] = start[e % kSets][j];
-          if (e < kSets) s[0] = s[1] = s[2] = s[3] = 0.0f;
-          mma_m16n8k16(s, kMinus136, kMinus136, kMinus136, kMinus136, x[e][j][0], x[e][j][1]);
-          mma_m16n8k16(s, kMinus136, kMinus136, kMinus136, kMinus136, x[e][j][2], x[e][j][3]);
+          x[j][0] = __byte_perm(x0, x2, 0x5410);
+          x[j][1] = __byte_perm(x0, x2, 0x7632);
+          x[j][2] = __byte_perm(x1, x3, 0x5410);
+          x[j][3] = __byte_perm(x1, x3, 0x7632);
         }
-      }
+      };
+      // acc += scale * sum for row tile i.
+      auto add_scaled = [&](int i, int set, const float (&sum)[NT][4]) {
+        const float v = sc[set][i >> 1];
+        const float s0 = __shfl_sync(0xFFFFFFFFu, v, (i & 1) * 16 + tokg);
+        const float s1 = __shfl_sync(0xFFFFFFFFu, v, (i & 1) * 16 + 8 + tokg);
 #pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        float sum[NT][4];
+        for (int j = 0; j < NT; ++j) {
+          acc[i][j][0] = fmaf(s0, sum[j][0], acc[i][j][0]);
+          acc[i][j][1] = fmaf(s0, sum[j][1], acc[i][j][1]);
+          acc[i][j][2] = fmaf(s1, sum[j][2], acc[i][j][2]);
+          acc[i][j][3] = fmaf(s1, sum[j][3], acc[i][j][3]);
+        }
+      };
+      if constexpr (Cfg::kFromSum) {
+        uint32_t x[2][NT][4];
+        float start[kSets][NT][4];  // -136 sum(x)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          uint32_t lo[4], hi[4];
-          w4_expand(ld_shared_u32((aw ^ (16u * e)) + i * 2048u), w4c, lo);
-          w4_expand(ld_shared_u32((aw ^ (16u * e)) + i * 2048u + 1024u), w4c, hi);
+          load_x(e, x[e]);
 #pragma unroll
           for (int j = 0; j < NT; ++j) {
-            if (e < kSets) mma_m16n8k16_onto(sum[j], start[e][j], lo[0], hi[0], lo[1], hi[1], x[e][j][0], x[e][j][1]);
-            else mma_m16n8k16(sum[j], lo[0], hi[0], lo[1], hi[1], x[e][j][0], x[e][j][1]);
-            mma_m16n8k16(sum[j], lo[2], hi[2], lo[3], hi[3], x[e][j][2], x[e][j][3]);
+            float (&s)[4] = start[e % kSets][j];
+            if (e < kSets) s[0] = s[1] = s[2] = s[3] = 0.0f;
+            mma_m16n8k16(s, kMinus136, kMinus136, kMinus136, kMinus136, x[e][j][0], x[e][j][1]);
+            mma_m16n8k16(s, kMinus136, kMinus136, kMinus136, kMinus136, x[e][j][2], x[e][j][3]);
           }
-          if (e == 1 || Cfg::kG32) {
-            const float v = sc[e % kSets][i >> 1];
-            const float s0 = __shfl_sync(0xFFFFFFFFu, v, (i & 1) * 16 + tokg);
-            const float s1 = __shfl_sync(0xFFFFFFFFu, v, (i & 1) * 16 + 8 + tokg);
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          float sum[NT][4];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            uint32_t lo[4], hi[4];
+            w4_expand(ld_shared_u32((aw ^ (16u * e)) + i * 2048u), w4c, lo);
+            w4_expand(ld_shared_u32((aw ^ (16u * e)) + i * 2048u + 1024u), w4c, hi);
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
-              acc[i][j][0] = fmaf(s0, sum[j][0], acc[i][j][0]);
-              acc[i][j][1] = fmaf(s0, sum[j][1], acc[i][j][1]);
-              acc[i][j][2] = fmaf(s1, sum[j][2], acc[i][j][2]);
-              acc[i][j][3] = fmaf(s1, sum[j][3], acc[i][j][3]);
+              if (e < kSets) mma_m16n8k16_onto(sum[j], start[e][j], lo[0], hi[0], lo[1], hi[1], x[e][j][0], x[e][j][1]);
+              else mma_m16n8k16(sum[j], lo[0], hi[0], lo[1], hi[1], x[e][j][0], x[e][j][1]);
+              mma_m16n8k16(sum[j], lo[2], hi[2], lo[3], hi[3], x[e][j][2], x[e][j][3]);
             }
+            if (e == 1 || Cfg::kG32) add_scaled(i, e % kSets, sum);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          uint32_t x[NT][4];
+          load_x(e, x);
+#pragma unroll
+          for (int i = 0; i < MT; ++i) {
+            uint32_t lo[4], hi[4];
+            w4_expand(ld_shared_u32((aw ^ (16u * e)) + i * 2048u), w4c, lo);
+            w4_expand(ld_shared_u32((aw ^ (16u * e)) + i * 2048u + 1024u), w4c, hi);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              lo[q] = w4_less_136(lo[q]);
+              hi[q] = w4_less_136(hi[q]);
+            }
+            const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            float sum[NT][4];
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+              mma_m16n8k16_onto(sum[j], zero, lo[0], hi[0], lo[1], hi[1], x[j][0], x[j][1]);
+              mma_m16n8k16(sum[j], lo[2], hi[2], lo[3], hi[3], x[j][2], x[j][3]);
+            }
+            add_scaled(i, e % kSets, sum);
           }
         }
       }
@@ -499,7 +545,6 @@ __global__ void __launch_bounds__(256) w4_dequantize_kernel(const W4Params p) {
   __syncthreads();
   if (k >= p.K) return;
   const W4Const c = w4_const();
-  const __nv_bfloat162 offset = __halves2bfloat162(__ushort_as_bfloat16(0x4308), __ushort_as_bfloat16(0x4308));
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int n = n0 + warp + 8 * i;
@@ -510,8 +555,8 @@ __global__ void __launch_bounds__(256) w4_dequantize_kernel(const W4Params p) {
     w4_expand(w[i], c, v);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const __nv_bfloat162 q = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v[j]), offset);
-      const __nv_bfloat162 d = __hmul2(q, s2);
+      v[j] = w4_less_136(v[j]);
+      const __nv_bfloat162 d = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&v[j]), s2);
       v[j] = *reinterpret_cast<const uint32_t*>(&d);
     }
     // pairs (k_j, k_j+4) back into order
