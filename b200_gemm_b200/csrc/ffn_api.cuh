@@ -8,11 +8,14 @@
 namespace b200gemm {
 
 // Stages fill shared memory next to the staging buffers: 3 x 48 KB + 64 KB,
-// or 6 x 32 KB + 16 KB.
-using FfnGated2 = FfnCfg<kGated, 2, 3>;
-using FfnGated1 = FfnCfg<kGated, 1, 6>;
-using FfnGrads2 = FfnCfg<kGrads, 2, 3>;
-using FfnGrads1 = FfnCfg<kGrads, 1, 6>;
+// or 6 x 32 KB, 7 x 28 KB, 8 x 24 KB + 16 KB.
+using FfnGated512 = FfnCfg<kGated, 2, 3>;
+using FfnGated256 = FfnCfg<kGated, 1, 6>;
+using FfnGated192 = FfnCfg<kGated, 1, 7, 192>;
+using FfnGated128 = FfnCfg<kGated, 1, 8, 128>;
+using FfnGrads512 = FfnCfg<kGrads, 2, 3>;
+using FfnGrads256 = FfnCfg<kGrads, 1, 6>;
+using FfnGrads128 = FfnCfg<kGrads, 1, 8, 128>;
 
 template <class Cfg>
 int prepare_ffn_kernel(int sm_count) {
@@ -43,8 +46,10 @@ int prepare_ffn_kernel(int sm_count) {
 // Smallest number of clusters that fit over all instances of the tiled
 // feed-forward kernel (they differ only in registers), or 0 on failure.
 int prepare_ffn_kernels(int sm_count) {
-  const int c[4] = {prepare_ffn_kernel<FfnGated2>(sm_count), prepare_ffn_kernel<FfnGated1>(sm_count),
-                    prepare_ffn_kernel<FfnGrads2>(sm_count), prepare_ffn_kernel<FfnGrads1>(sm_count)};
+  const int c[] = {prepare_ffn_kernel<FfnGated512>(sm_count), prepare_ffn_kernel<FfnGated256>(sm_count),
+                   prepare_ffn_kernel<FfnGated192>(sm_count), prepare_ffn_kernel<FfnGated128>(sm_count),
+                   prepare_ffn_kernel<FfnGrads512>(sm_count), prepare_ffn_kernel<FfnGrads256>(sm_count),
+                   prepare_ffn_kernel<FfnGrads128>(sm_count)};
   int least = c[0];
   for (int v : c) least = v < least ? v : least;
   return least;
@@ -57,10 +62,13 @@ bool opt_in_smem(Kernel kernel, int bytes) {
   return false;
 }
 
+template <int NT>
+bool prepare_gated_decode() {
+  return opt_in_smem(gated_decode_sm100<GatedDecodeCfg<NT, false>>, GatedDecodeCfg<NT, false>::kSmemBytes) &&
+         opt_in_smem(gated_decode_sm100<GatedDecodeCfg<NT, true>>, GatedDecodeCfg<NT, true>::kSmemBytes);
+}
 bool prepare_gated_decode_kernels() {
-  return opt_in_smem(gated_decode_sm100<GatedDecodeCfg<1>>, GatedDecodeCfg<1>::kSmemBytes) &&
-         opt_in_smem(gated_decode_sm100<GatedDecodeCfg<2>>, GatedDecodeCfg<2>::kSmemBytes) &&
-         opt_in_smem(gated_decode_sm100<GatedDecodeCfg<4>>, GatedDecodeCfg<4>::kSmemBytes);
+  return prepare_gated_decode<1>() && prepare_gated_decode<2>() && prepare_gated_decode<4>();
 }
 
 // Instances of the 4-bit product: 16-row tiles of W per warp (MT) that its
@@ -196,48 +204,63 @@ bool group_shift_of(int group, int* shift) {
 
 constexpr int kMaxExtent = 0x7FFFFFFF - 4096;  // rows, columns: tile coordinates stay inside an int
 
-// Time of one tile of num_kb K blocks in the units of tile_plan_cost: a 256 x
-// 256 tile (NB = 1, its epilogue hidden) or a 256 x 512 one (NB = 2) whose
-// epilogue costs `epi` more than the plain one.
-double ffn_tile_time(int nb, int num_kb, double epi) {
-  return nb == 2 ? (2.0 * num_kb + 13.0) * 0.8545 / 0.85 + epi : num_kb / 0.85 + 4.0;
+// Time of one tile with `width` accumulator columns and num_kb K blocks, in
+// the units and by the fit of tile_plan_cost; a 512-wide tile's epilogue is
+// not hidden and costs `epi` more than the plain one.
+double ffn_tile_time(int width, int num_kb, double epi) {
+  if (width == 512) return (2.0 * num_kb + 13.0) * 0.8545 / 0.85 + epi;
+  const double feed = (16384.0 + 64.0 * width) / 32768.0;
+  return num_kb * (0.08 + 0.92 * feed) / 0.85 + 4.0;
 }
 
-// The gated block's NB: by waves of tiles.  A forced tile width of 512 or 448
-// asks for 2, any other for 1.
-int ffn_gated_nb(const b200gemm_handle* h, int tiles_m, int F, int num_kb) {
-  if (h->tile_width != 0) return h->tile_width >= 448 ? 2 : 1;
-  double cost[3];
-  for (int nb = 1; nb <= 2; ++nb) {
-    const long long tiles = static_cast<long long>(tiles_m) * ((F + 128ll * nb - 1) / (128 * nb));
-    cost[nb] = static_cast<double>((tiles + h->ffn_clusters - 1) / h->ffn_clusters) *
-               ffn_tile_time(nb, num_kb, 12.0);
+// Accumulator columns of the gated block's tiles (twice H's): by waves of
+// tiles.  A forced tile width asks for the nearest one there is.
+int ffn_gated_width(const b200gemm_handle* h, int tiles_m, int F, int num_kb) {
+  if (h->tile_width != 0) return h->tile_width >= 448 ? 512 : (h->tile_width >= 224 ? 256 : h->tile_width);
+  int best = 0;
+  double best_cost = 1e300;
+  for (int width : {512, 256, 192, 128}) {
+    const long long tiles = static_cast<long long>(tiles_m) * ((F + width / 2 - 1ll) / (width / 2));
+    const double cost = static_cast<double>((tiles + h->ffn_clusters - 1) / h->ffn_clusters) *
+                        ffn_tile_time(width, num_kb, 12.0);
+    if (cost < best_cost) {
+      best_cost = cost;
+      best = width;
+    }
   }
-  return cost[2] < cost[1] ? 2 : 1;
+  return best;
 }
 
 // The same for the gradients, whose tiles fill the clusters' time together:
 // the mean load and half a dW tile, or what the dX tiles alone take.
-int ffn_grads_nb(const b200gemm_handle* h, int m, int f, int k, bool dx, bool dw) {
-  if (h->tile_width != 0) return h->tile_width >= 448 ? 2 : 1;
-  double cost[3];
+int ffn_grads_width(const b200gemm_handle* h, int m, int f, int k, bool dx, bool dw) {
+  if (h->tile_width != 0) return h->tile_width >= 448 ? 512 : (h->tile_width >= 192 ? 256 : 128);
+  int best = 0;
+  double best_cost = 1e300;
   const double g = h->ffn_clusters;
-  for (int nb = 1; nb <= 2; ++nb) {
-    const double tn = (k + 256ll * nb - 1) / (256 * nb);
+  for (int width : {512, 256, 128}) {
+    const double tn = static_cast<double>((k + width - 1ll) / width);
     const double n1 = dx ? tn * ((m + 255ll) / 256) : 0.0, n2 = dw ? 2.0 * tn * ((f + 255ll) / 256) : 0.0;
-    const double t1 = ffn_tile_time(nb, 2 * ((f + 63) / 64), 0.0), t2 = ffn_tile_time(nb, (m + 63) / 64, 0.0);
+    const double t1 = ffn_tile_time(width, 2 * ((f + 63) / 64), 0.0), t2 = ffn_tile_time(width, (m + 63) / 64, 0.0);
     const double mean = (n1 * t1 + n2 * t2) / g + (n2 > 0.0 ? 0.5 * t2 : 0.0);
-    const double alone = static_cast<double>(static_cast<long long>((n1 + g - 1.0) / g)) * t1;
-    cost[nb] = mean > alone ? mean : alone;
+    const double dx_alone = static_cast<double>(static_cast<long long>((n1 + g - 1.0) / g)) * t1;
+    const double dw_alone = n1 > 0.0 ? t2 : static_cast<double>(static_cast<long long>((n2 + g - 1.0) / g)) * t2;
+    double cost = mean > dx_alone ? mean : dx_alone;
+    if (n2 > 0.0 && dw_alone > cost) cost = dw_alone;
+    if (cost < best_cost) {
+      best_cost = cost;
+      best = width;
+    }
   }
-  return cost[2] < cost[1] ? 2 : 1;
+  return best;
 }
 
-// bf16 operand maps of the tiled kernel: K-major boxes of 64 k x 128 rows,
+// bf16 operand maps of the tiled kernel: K-major boxes of 64 k x 128 rows (or
+// as many as one CTA loads),
 // MN-major boxes of 64 columns x 64 k, both one 128-byte swizzle row wide.
-bool encode_kmajor(CUtensorMap* m, const void* ptr, int k, int rows, long long ld) {
+bool encode_kmajor(CUtensorMap* m, const void* ptr, int k, int rows, long long ld, int box_rows = 128) {
   return encode_2d(m, ptr, static_cast<uint64_t>(k), static_cast<uint64_t>(rows), static_cast<uint64_t>(ld) * 2,
-                   kBlockK, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+                   kBlockK, static_cast<uint32_t>(box_rows), CU_TENSOR_MAP_SWIZZLE_128B);
 }
 bool encode_mnmajor(CUtensorMap* m, const void* ptr, int mn, int k, long long ld) {
   return encode_2d(m, ptr, static_cast<uint64_t>(mn), static_cast<uint64_t>(k), static_cast<uint64_t>(ld) * 2, 64, 64,
@@ -248,30 +271,57 @@ bool encode_out(CUtensorMap* m, void* ptr, int cols, int rows, long long ld) {
                    kCBoxCols, kCBoxRows, CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
-// K ranges (CTAs of a cluster) of the gated block's decode kernel: the smallest
-// power of two up to 8 that gives every SM a CTA, while each CTA's warps keep
-// a stage or two.
-int gated_decode_split(const b200gemm_handle* h, long long blocks, int num_stages) {
+// Whether the gated block runs on the decode kernel, which reads the weights
+// once per 32 rows of X: always up to 32 rows, and as far as 128 where that is
+// estimated to beat the tiled kernel, whose few tiles of a small block leave
+// most SMs idle.  In microseconds, measured on B200: 0.315 per unit of
+// ffn_tile_time; the weights at 5 TB/s with 32 rows of X; 4 of either launch.
+bool gated_uses_decode(const b200gemm_handle* h, int M, int F, int K) {
+  if (h->small_m == 0 || h->tile_width != 0 || M > 128) return false;
+  if (M <= 32) return true;
+  const int num_kb = (K + kBlockK - 1) / kBlockK;
+  const int width = ffn_gated_width(h, 1, F, num_kb);
+  const long long tiles = (F + width / 2 - 1ll) / (width / 2);
+  const double tiled = 0.315 * static_cast<double>((tiles + h->ffn_clusters - 1) / h->ffn_clusters) *
+                       ffn_tile_time(width, num_kb, 12.0);
+  return (M + 31) / 32 * (4e-6 / 5.0 * F * static_cast<double>(K)) < tiled;
+}
+
+// K ranges (CTAs of a cluster) of the decode kernel: the smallest power of two
+// up to 8 that gives every SM a CTA, while each CTA's warps keep a few stages.
+int gated_decode_split(const b200gemm_handle* h, long long ctas, int num_stages) {
   int split = 1;
-  while (split < 8 && blocks * split < h->sm_count && num_stages >= 16 * split) split *= 2;
+  while (split < 8 && ctas * split < h->sm_count && num_stages >= 16 * split) split *= 2;
   return split;
+}
+
+template <int NT>
+cudaError_t launch_gated_decode(const b200gemm_handle* h, int split, int blocks, int token_blocks, cudaStream_t stream,
+                                const CUtensorMap& mg, const CUtensorMap& mu, const CUtensorMap& mx,
+                                const GatedDecodeParams& p) {
+  using Deep = GatedDecodeCfg<NT, true>;
+  using Small = GatedDecodeCfg<NT, false>;
+  if (static_cast<long long>(split) * blocks * token_blocks <= static_cast<long long>(Deep::kCtas) * h->sm_count)
+    return launch_rows(gated_decode_sm100<Deep>, Deep::kThreads, Deep::kSmemBytes, split, blocks, token_blocks, stream,
+                       mg, mu, mx, p);
+  return launch_rows(gated_decode_sm100<Small>, Small::kThreads, Small::kSmemBytes, split, blocks, token_blocks, stream,
+                     mg, mu, mx, p);
 }
 
 int run_gated_decode(b200gemm_t h, const void* Wg, const void* Wu, long long ldw, const void* X, long long ldx,
                      GatedDecodeParams p, cudaStream_t stream) {
   const int nt = p.M > 16 ? 4 : (p.M > 8 ? 2 : 1);
   const long long blocks = (static_cast<long long>(p.F) + 31) / 32;
+  const int token_blocks = (p.M + 31) / 32;
   if (blocks > 65535) return B200GEMM_ERR_TOO_LARGE;
   CUtensorMap mg, mu, mx;
-  const auto encode = [&](CUtensorMap* m, const void* ptr, int rows, long long ld, uint32_t box_rows) {
-    return encode_2d(m, ptr, static_cast<uint64_t>(p.K), static_cast<uint64_t>(rows), static_cast<uint64_t>(ld) * 2, 64,
-                     box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
+  const auto encode = [&](CUtensorMap* m, const void* ptr, int rows, long long ld, int box_rows) {
+    return encode_kmajor(m, ptr, p.K, rows, ld, box_rows);
   };
-  if (!encode(&mg, Wg, p.F, ldw, 32) || !encode(&mu, Wu, p.F, ldw, 32) ||
-      !encode(&mx, X, p.M, ldx, static_cast<uint32_t>(8 * nt)))
+  if (!encode(&mg, Wg, p.F, ldw, 32) || !encode(&mu, Wu, p.F, ldw, 32) || !encode(&mx, X, p.M, ldx, 8 * nt))
     return B200GEMM_ERR_CUDA;
   p.num_stages = (p.K + 63) / 64;
-  const int split = gated_decode_split(h, blocks, p.num_stages);
+  const int split = gated_decode_split(h, blocks * token_blocks, p.num_stages);
   p.stages_per_cta = (p.num_stages + split - 1) / split;
   {
     std::lock_guard<std::mutex> lock(h->mu);
@@ -279,13 +329,10 @@ int run_gated_decode(b200gemm_t h, const void* Wg, const void* Wu, long long ldw
     p.pdl = h->pdl;
   }
   p.status = h->status_dev;
-  const auto go = [&](auto kernel, int threads, int smem) {
-    return launch_rows(kernel, threads, smem, split, static_cast<int>(blocks), 1, stream, mg, mu, mx, p);
-  };
-  const cudaError_t e =
-      nt == 1   ? go(gated_decode_sm100<GatedDecodeCfg<1>>, GatedDecodeCfg<1>::kThreads, GatedDecodeCfg<1>::kSmemBytes)
-      : nt == 2 ? go(gated_decode_sm100<GatedDecodeCfg<2>>, GatedDecodeCfg<2>::kThreads, GatedDecodeCfg<2>::kSmemBytes)
-                : go(gated_decode_sm100<GatedDecodeCfg<4>>, GatedDecodeCfg<4>::kThreads, GatedDecodeCfg<4>::kSmemBytes);
+  const int b = static_cast<int>(blocks);
+  const cudaError_t e = nt == 1   ? launch_gated_decode<1>(h, split, b, token_blocks, stream, mg, mu, mx, p)
+                        : nt == 2 ? launch_gated_decode<2>(h, split, b, token_blocks, stream, mg, mu, mx, p)
+                                  : launch_gated_decode<4>(h, split, b, token_blocks, stream, mg, mu, mx, p);
   return e == cudaSuccess ? B200GEMM_OK : B200GEMM_ERR_CUDA;
 }
 
@@ -437,12 +484,12 @@ extern "C" int b200gemm_bf16_gated(b200gemm_t h, int M, int F, int K, const void
   if (!guard.ok()) return B200GEMM_ERR_CUDA;
 
   bool small;
-  int nb;
+  int width;
   const int num_kb = (K + kBlockK - 1) / kBlockK;
   {
     std::lock_guard<std::mutex> lock(h->mu);
-    small = M <= 32 && G == nullptr && h->small_m != 0 && h->tile_width == 0;
-    nb = ffn_gated_nb(h, (M + kTileM - 1) / kTileM, F, num_kb);
+    small = G == nullptr && gated_uses_decode(h, M, F, K);
+    width = ffn_gated_width(h, (M + kTileM - 1) / kTileM, F, num_kb);
   }
   if (small) {
     GatedDecodeParams p{};
@@ -455,8 +502,9 @@ extern "C" int b200gemm_bf16_gated(b200gemm_t h, int M, int F, int K, const void
     return run_gated_decode(h, Wg, Wu, ldw, X, ldx, p, stream);
   }
   FfnMaps m;
-  if (!encode_kmajor(&m.a0, X, K, M, ldx) || !encode_kmajor(&m.b0, Wg, K, F, ldw) ||
-      !encode_kmajor(&m.b1, Wu, K, F, ldw) || !encode_out(&m.c[0], H, F, M, ldh)) {
+  const int box_rows = width == 512 ? 128 : width / 2;
+  if (!encode_kmajor(&m.a0, X, K, M, ldx) || !encode_kmajor(&m.b0, Wg, K, F, ldw, box_rows) ||
+      !encode_kmajor(&m.b1, Wu, K, F, ldw, box_rows) || !encode_out(&m.c[0], H, F, M, ldh)) {
     return B200GEMM_ERR_CUDA;
   }
   m.a1 = m.w0 = m.w1 = m.x = m.a0;  // (not read)
@@ -464,13 +512,18 @@ extern "C" int b200gemm_bf16_gated(b200gemm_t h, int M, int F, int K, const void
   if (G != nullptr && (!encode_out(&m.c[1], G, F, M, ldgu) || !encode_out(&m.c[2], U, F, M, ldgu)))
     return B200GEMM_ERR_CUDA;
   FfnParams p{};
-  p.first = ffn_set(M, F, num_kb, 128 * nb, 1);
+  p.first = ffn_set(M, F, num_kb, width / 2, 1);
   p.act = activation;
   p.save = G != nullptr ? 1 : 0;
   p.out[0] = {static_cast<uint16_t*>(H), ldh};
   p.out[1] = {static_cast<uint16_t*>(G), ldgu};
   p.out[2] = {static_cast<uint16_t*>(U), ldgu};
-  return nb == 2 ? run_ffn<FfnGated2>(h, m, p, stream, false) : run_ffn<FfnGated1>(h, m, p, stream, false);
+  switch (width) {
+    case 512: return run_ffn<FfnGated512>(h, m, p, stream, false);
+    case 192: return run_ffn<FfnGated192>(h, m, p, stream, false);
+    case 128: return run_ffn<FfnGated128>(h, m, p, stream, false);
+    default: return run_ffn<FfnGated256>(h, m, p, stream, false);
+  }
 }
 
 extern "C" unsigned long long b200gemm_gated_backward_workspace(int M, int F) {
@@ -557,20 +610,25 @@ extern "C" int b200gemm_bf16_gated_backward(b200gemm_t h, int M, int F, int K, c
     return B200GEMM_ERR_CUDA;
   if (dX == nullptr) m.c[0] = m.c[1];  // (not written)
   if (dWg == nullptr) m.c[1] = m.c[2] = m.c[0];
-  int nb;
+  int width;
   {
     std::lock_guard<std::mutex> lock(h->mu);
-    nb = ffn_grads_nb(h, M, F, K, dX != nullptr, dWg != nullptr);
+    width = ffn_grads_width(h, M, F, K, dX != nullptr, dWg != nullptr);
   }
   FfnParams p{};
   p.seg_kb = (F + kBlockK - 1) / kBlockK;
-  p.first = ffn_set(M, K, 2 * p.seg_kb, 256 * nb, dX != nullptr ? 1 : 0);
-  p.second = ffn_set(F, K, (M + kBlockK - 1) / kBlockK, 256 * nb, dWg != nullptr ? 2 : 0);
-  p.ahead = static_cast<int>(ffn_tile_time(nb, p.first.num_kb, 0.0) / ffn_tile_time(nb, p.second.num_kb, 0.0) + 0.5);
+  p.first = ffn_set(M, K, 2 * p.seg_kb, width, dX != nullptr ? 1 : 0);
+  p.second = ffn_set(F, K, (M + kBlockK - 1) / kBlockK, width, dWg != nullptr ? 2 : 0);
+  p.ahead =
+      static_cast<int>(ffn_tile_time(width, p.first.num_kb, 0.0) / ffn_tile_time(width, p.second.num_kb, 0.0) + 0.5);
   p.out[0] = {static_cast<uint16_t*>(dX), lddx};
   p.out[1] = {static_cast<uint16_t*>(dWg), lddw};
   p.out[2] = {static_cast<uint16_t*>(dWu), lddw};
-  return nb == 2 ? run_ffn<FfnGrads2>(h, m, p, stream, true) : run_ffn<FfnGrads1>(h, m, p, stream, true);
+  switch (width) {
+    case 512: return run_ffn<FfnGrads512>(h, m, p, stream, true);
+    case 128: return run_ffn<FfnGrads128>(h, m, p, stream, true);
+    default: return run_ffn<FfnGrads256>(h, m, p, stream, true);
+  }
 }
 
 namespace {

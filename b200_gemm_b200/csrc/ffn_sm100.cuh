@@ -78,21 +78,25 @@ struct FfnMaps {
 //         overlaps the next tile's MMAs.  kGated: the N = 256 MMA takes its
 //         first 128 B rows from the even CTA and the others from the odd one,
 //         so the even CTA loads rows of Wg and the odd one the same rows of
-//         Wu (128 columns of H per tile).
-template <int KIND, int NB, int STAGES>
+//         Wu (128 columns of H per tile).  MN = 192 (gated only) and 128 are
+//         the same with narrower MMAs, for sizes that 256 cuts into a mostly
+//         idle last wave, or into fewer tiles than there are clusters.
+template <int KIND, int NB, int STAGES, int MN = 256>
 struct FfnCfg {
+  static_assert(MN == 256 || (NB == 1 && (MN == 128 || (MN == 192 && KIND == kGated))), "MMA width");
   static constexpr int kKind = KIND;
   static constexpr int kNB = NB;
   static constexpr int kStages = STAGES;
-  static constexpr int kAccCols = 256 * NB;
-  static constexpr int kTileN = KIND == kGated ? 128 * NB : 256 * NB;  // output columns per tile
+  static constexpr int kMmaN = MN;
+  static constexpr int kTileN = KIND == kGated ? MN / 2 * NB : MN * NB;  // output columns per tile
   static constexpr int kAccBufs = NB == 1 ? 2 : 1;
   static constexpr int kEpiWarps = 4 * NB;
   static constexpr int kThreads = 64 + 32 * kEpiWarps;
   static constexpr int kWarpCols = kTileN / NB;              // output columns one epilogue warp writes
   static constexpr int kWarpChunks = kWarpCols / kCBoxCols;
   static constexpr int kCBufs = NB == 2 ? 4 : 2;
-  static constexpr int kBlockBytesB = 128 * kBlockK * 2;     // one CTA's half of one N = 256 block
+  static constexpr int kBRows = MN / 2;                      // one CTA's half of one MMA's B rows
+  static constexpr int kBlockBytesB = kBRows * kBlockK * 2;
   static constexpr int kStageBytesB = NB * kBlockBytesB;
   static constexpr uint32_t kTxBytes = 2 * (kStageBytesA + kStageBytesB);
   static constexpr int kA = 0;
@@ -126,10 +130,10 @@ template <bool MN>
 constexpr uint64_t kDescStep = MN ? 128 : 2;
 
 // Instruction descriptor: kind::f16, D f32, A and B bf16, M = 256 (pair),
-// N = 256; bits 15 and 16 say that A or B is MN-major.
-template <bool A_MN, bool B_MN>
+// N = MN; bits 15 and 16 say that A or B is MN-major.
+template <int MN, bool A_MN, bool B_MN>
 constexpr uint32_t kFfnIdesc = (1u << 4) | (1u << 7) | (1u << 10) | (A_MN ? 1u << 15 : 0u) | (B_MN ? 1u << 16 : 0u) |
-                               ((256u >> 3) << 17) | ((256u >> 4) << 24);
+                               (static_cast<uint32_t>(MN >> 3) << 17) | ((256u >> 4) << 24);
 
 // Tile t of a set in the band order: bands of `band` tile rows, each swept
 // column by column, so the band's A rows and one column of B stay in L2
@@ -288,7 +292,7 @@ __device__ __forceinline__ bool ffn_mma_tile(uint32_t sA, uint32_t sB, uint32_t 
 #pragma unroll
       for (int h = 0; h < Cfg::kNB; ++h) {
         ptx::mma_bf16_cg2(d_tmem + h * 256u, a_desc + k * kDescStep<A_MN>,
-                          b_desc + (h * Cfg::kBlockBytesB >> 4) + k * kDescStep<B_MN>, kFfnIdesc<A_MN, B_MN>,
+                          b_desc + (h * Cfg::kBlockBytesB >> 4) + k * kDescStep<B_MN>, kFfnIdesc<Cfg::kMmaN, A_MN, B_MN>,
                           (kb > 0 || k > 0) ? 1u : 0u);
       }
     }
@@ -367,7 +371,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1) __cluster_dims__(2, 1, 1)
       FfnUnit u;
       for (int i = 0; ok && ffn_unit<Cfg::kKind>(p, cluster, nclusters, i, u); ++i) {
         const int row_a = u.tm * kTileM + static_cast<int>(rank) * 128;
-        const int row_b = u.tn * Cfg::kTileN + ((Cfg::kKind == kGated && NB == 1) ? 0 : static_cast<int>(rank) * 128);
+        const int row_b = u.tn * Cfg::kTileN + ((Cfg::kKind == kGated && NB == 1) ? 0 : static_cast<int>(rank) * Cfg::kBRows);
         const int num_kb = u.second ? p.second.num_kb : p.first.num_kb;
         for (int kb = 0; kb < num_kb; ++kb) {
           if (!ptx::mbar_wait(empty0 + 8 * stage, phase ^ 1u, wd, kSiteProducer, static_cast<unsigned>(i))) {
@@ -399,8 +403,9 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1) __cluster_dims__(2, 1, 1)
 #pragma unroll
             for (int h = 0; h < NB; ++h) {
               const uint32_t d = db + h * Cfg::kBlockBytesB;
-              ptx::tma_load_2d_cg2(d, mb, fb, row_b + h * 256, k, policy);
-              ptx::tma_load_2d_cg2(d + 8192, mb, fb, row_b + h * 256 + 64, k, policy);
+#pragma unroll
+              for (int c = 0; c < Cfg::kBRows / 64; ++c)
+                ptx::tma_load_2d_cg2(d + c * 8192, mb, fb, row_b + h * 256 + c * 64, k, policy);
             }
           }
           if (++stage == STAGES) {
@@ -473,7 +478,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1) __cluster_dims__(2, 1, 1)
       };
       if constexpr (Cfg::kKind == kGated) {
         const int M = p.first.M, N = p.first.N;
-        constexpr uint32_t kUp = 128u * NB;  // U's columns follow G's
+        constexpr uint32_t kUp = Cfg::kMmaN / 2 * NB;  // U's columns follow G's
 #pragma unroll 1
         for (int c = 0; c < Cfg::kWarpChunks; ++c) {
           uint32_t g[32], v[32], w[16];

@@ -1,7 +1,7 @@
 // Gated block for a few rows of activations (decode) on sm_100a, where reading
 // the weights once from HBM is the whole cost:
 //   H = act(X Wg^T) * (X Wu^T)     X [M,K], Wg, Wu [F,K] bf16
-// at most 32 rows of X.
+// at most 32 rows of X per CTA (blocks of 32 rows of X beyond that).
 //
 // Rows of the weights are the M side of mma.sync m16n8k16 (its rate is far
 // from its limit here, and the sums stay in registers), rows of X its N side.
@@ -38,7 +38,10 @@ struct GatedDecodeParams {
   int pdl;
 };
 
-template <int NT>
+// DEEP: twice the ring (or more) at half the CTAs per SM, for launches that
+// do not fill the SMs otherwise: an SM needs some 64 KB of copies in flight
+// to draw its share of HBM's bandwidth.
+template <int NT, bool DEEP>
 struct GatedDecodeCfg {
   static constexpr int kNT = NT;                       // tiles of 8 rows of X
   static constexpr int kTok = 8 * NT;
@@ -52,11 +55,11 @@ struct GatedDecodeCfg {
   static constexpr int kStageBytes = kStageW + kStageX;
   // CTAs per SM and a ring that fits that often: small CTAs, so that all of
   // a launch's are resident at once and share HBM evenly.
-  static constexpr int kCtas = NT == 4 ? 2 : 4;
+  static constexpr int kCtas = (NT == 4 ? 2 : 4) / (DEEP ? 2 : 1);
   // A multiple of the warps, so that a stage has the same reader every time
   // around and that reader waits for its fillings in order: a wait by parity
   // for the filling after next would be satisfied before the next arrived.
-  static constexpr int kStages = (NT == 4 ? 98304 : 53248) / kStageBytes / kWarps * kWarps;
+  static constexpr int kStages = (233472 / kCtas - 1024 - 1024 - 256) / kStageBytes / kWarps * kWarps;
   static constexpr int kX = kStages * kStageW;
   static constexpr int kFull = kX + kStages * kStageX;
   static constexpr int kAbort = kFull + 8 * kStages;
@@ -117,6 +120,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, Cfg::kCtas)
   const int split = static_cast<int>(gridDim.x);   // CTAs of this cluster: K ranges
   const int rank = static_cast<int>(blockIdx.x);
   const int n0 = static_cast<int>(blockIdx.y) * Cfg::kOutCols;
+  const int m0 = static_cast<int>(blockIdx.z) * 32;
   const int s_begin = rank * p.stages_per_cta;
   const int count = max(0, min(p.num_stages, s_begin + p.stages_per_cta) - s_begin);
 
@@ -126,7 +130,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, Cfg::kCtas)
   wd.status = p.status;
   wd.timeout_ns = p.timeout_ns;
 
-  const uint64_t policy_w = ptx::policy_evict_first();  // read once
+  const uint64_t policy_w = ptx::policy_evict_first();  // read once (per 32 rows of X)
   const uint64_t policy_x = ptx::policy_evict_last();   // read by every CTA
   auto load_w = [&](int it, int s) {
     const uint32_t bar = full0 + 8 * s, dst = base + s * Cfg::kStageW;
@@ -135,7 +139,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, Cfg::kCtas)
     ptx::tma_load_2d(dst + 32 * 128, &map_u, bar, (s_begin + it) * Cfg::kStageK, n0, policy_w);
   };
   auto load_x = [&](int it, int s) {
-    ptx::tma_load_2d(base + Cfg::kX + s * Cfg::kStageX, &map_x, full0 + 8 * s, (s_begin + it) * Cfg::kStageK, 0,
+    ptx::tma_load_2d(base + Cfg::kX + s * Cfg::kStageX, &map_x, full0 + 8 * s, (s_begin + it) * Cfg::kStageK, m0,
                      policy_x);
   };
   if (threadIdx.x == 0) {
@@ -253,10 +257,10 @@ __global__ void __launch_bounds__(Cfg::kThreads, Cfg::kCtas)
     for (int idx = static_cast<int>(threadIdx.x) + Cfg::kThreads * rank; idx < Cfg::kTok * kCols;
          idx += Cfg::kThreads * split) {
       const int tok = idx / kCols, c = idx % kCols;
-      if (tok >= p.M || n0 + c >= p.F) continue;
+      if (m0 + tok >= p.M || n0 + c >= p.F) continue;
       const float gate = total(tok * Cfg::kPitch + c), up = total(tok * Cfg::kPitch + 32 + c);
       const float v = gated_value(p.act, gate, up);
-      p.out[static_cast<long long>(tok) * p.ldo + n0 + c] = __bfloat16_as_ushort(__float2bfloat16_rn(v));
+      p.out[static_cast<long long>(m0 + tok) * p.ldo + n0 + c] = __bfloat16_as_ushort(__float2bfloat16_rn(v));
     }
   }
   if (threadIdx.x == 0 && ptx::aborted(wd)) ptx::sleep_ns_bounded(200000ull);

@@ -46,18 +46,19 @@ def test_gated(gpu_handle, M, F, K, kind):
     _check_gated(gpu_handle, M, F, K, kind, save=False, seed=M + F)
 
 
-@pytest.mark.parametrize("M,F,K", [(1, 14000, 4096), (8, 5001, 2056), (12, 3001, 4096), (32, 6000, 2048), (1, 40, 8192)])
+@pytest.mark.parametrize("M,F,K", [(1, 14000, 4096), (8, 5001, 2056), (12, 3001, 4096), (32, 6000, 2048), (1, 40, 8192),
+                                   (100, 300, 4104), (65, 70, 2048), (20, 9500, 520)])
 def test_gated_few_rows_long(gpu_handle, M, F, K):
     """Few rows against many and long weights: every ring goes around many
     times, every SM holds several blocks; and a width that splits K."""
     _check_gated(gpu_handle, M, F, K, "silu", save=False, seed=M)
 
 
-@pytest.mark.parametrize("width", [512, 256])
+@pytest.mark.parametrize("width", [512, 256, 192, 128])
 @pytest.mark.parametrize("save", [False, True])
 @pytest.mark.parametrize("M,F,K", [(1, 7, 8), (300, 1001, 520), (2, 128, 64)])
 def test_gated_tiled(gpu_handle, M, F, K, width, save):
-    """Both tile widths of the tiled kernel, whatever the rule would pick."""
+    """Every tile width of the tiled kernel, whatever the rule would pick."""
     gpu_handle.set_tile_width(width)
     try:
         _check_gated(gpu_handle, M, F, K, "silu", save, pad=24, seed=K)
@@ -150,7 +151,7 @@ def test_backward(gpu_handle, M, F, K, kind):
     _check_backward(gpu_handle, M, F, K, kind, seed=M + F)
 
 
-@pytest.mark.parametrize("width", [512, 256])
+@pytest.mark.parametrize("width", [512, 256, 128])
 @pytest.mark.parametrize("M,F,K", [(130, 70, 136), (700, 1030, 1160)])
 def test_backward_tiled(gpu_handle, M, F, K, width):
     gpu_handle.set_tile_width(width)
