@@ -78,10 +78,10 @@ SIGNATURES = {
     "b200gemm_bf16_nt_noalloc": (_c_int, [_c_int, _c_int, _c_int, _vp, _vp, _vp, _c_int, _vp]),
     "b200gemm_bf16_gated": (_c_int, [_vp, _c_int, _c_int, _c_int, _vp, _c_ll, _vp, _vp, _c_ll, _c_int,
                                      _vp, _c_ll, _vp, _vp, _c_ll, _vp]),
-    "b200gemm_gated_backward_workspace": (_c_ull, [_c_int, _c_int]),
+    "b200gemm_gated_backward_workspace": (_c_ull, [_vp, _c_int, _c_int, _c_int]),
     "b200gemm_bf16_gated_backward": (_c_int, [_vp, _c_int, _c_int, _c_int, _vp, _c_ll, _vp, _c_ll, _vp, _vp,
                                               _c_ll, _vp, _vp, _c_ll, _c_int, _vp, _c_ll, _vp, _vp, _c_ll,
-                                              _vp, _vp]),
+                                              _vp, _c_ull, _vp]),
     "b200gemm_w4_quantize": (_c_int, [_vp, _c_int, _c_int, _vp, _c_ll, _c_int, _vp, _vp, _vp]),
     "b200gemm_w4_dequantize": (_c_int, [_vp, _c_int, _c_int, _vp, _vp, _c_int, _vp, _c_ll, _vp]),
     "b200gemm_w4_nt": (_c_int, [_vp, _c_int, _c_int, _c_int, _vp, _c_ll, _vp, _vp, _c_int, _vp, _c_ll, _c_int,

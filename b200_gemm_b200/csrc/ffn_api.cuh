@@ -232,27 +232,50 @@ int ffn_gated_width(const b200gemm_handle* h, int tiles_m, int F, int num_kb) {
 }
 
 // The same for the gradients, whose tiles fill the clusters' time together:
-// the mean load and half a dW tile, or what the dX tiles alone take.
-int ffn_grads_width(const b200gemm_handle* h, int m, int f, int k, bool dx, bool dw) {
-  if (h->tile_width != 0) return h->tile_width >= 448 ? 512 : (h->tile_width >= 192 ? 256 : 128);
-  int best = 0;
+// the mean load and half a dW tile, or what the dX tiles take by themselves.
+// Where dX has too few tiles for the clusters, its sum is split into up to 16
+// ranges of at least 8 K blocks (another launch, and their partial sums, cost
+// about 10 units).
+struct GradsPlan {
+  int width = 256, split = 1, slice_kb = 0;
+};
+GradsPlan grads_plan(const b200gemm_handle* h, int m, int f, int k, bool dx, bool dw, bool may_split) {
+  GradsPlan best;
   double best_cost = 1e300;
   const double g = h->ffn_clusters;
+  const int kb = 2 * ((f + 63) / 64);
   for (int width : {512, 256, 128}) {
+    if (h->tile_width != 0 && width != (h->tile_width >= 448 ? 512 : (h->tile_width >= 192 ? 256 : 128))) continue;
     const double tn = static_cast<double>((k + width - 1ll) / width);
     const double n1 = dx ? tn * ((m + 255ll) / 256) : 0.0, n2 = dw ? 2.0 * tn * ((f + 255ll) / 256) : 0.0;
-    const double t1 = ffn_tile_time(width, 2 * ((f + 63) / 64), 0.0), t2 = ffn_tile_time(width, (m + 63) / 64, 0.0);
-    const double mean = (n1 * t1 + n2 * t2) / g + (n2 > 0.0 ? 0.5 * t2 : 0.0);
-    const double dx_alone = static_cast<double>(static_cast<long long>((n1 + g - 1.0) / g)) * t1;
-    const double dw_alone = n1 > 0.0 ? t2 : static_cast<double>(static_cast<long long>((n2 + g - 1.0) / g)) * t2;
-    double cost = mean > dx_alone ? mean : dx_alone;
-    if (n2 > 0.0 && dw_alone > cost) cost = dw_alone;
-    if (cost < best_cost) {
-      best_cost = cost;
-      best = width;
+    const double t2 = ffn_tile_time(width, (m + 63) / 64, 0.0);
+    for (int want = 1; want <= (dx && may_split ? 16 : 1); want *= 2) {
+      const int slice = (kb + want - 1) / want, split = (kb + slice - 1) / slice;
+      if (split > 1 && (slice < 8 || n1 * split > 2.0 * g)) break;
+      const double t1 = ffn_tile_time(width, slice, 0.0);
+      const double mean = (n1 * split * t1 + n2 * t2) / g + (n2 > 0.0 ? 0.5 * t2 : 0.0);
+      double cost = static_cast<double>(static_cast<long long>((n1 * split + g - 1.0) / g)) * t1;
+      if (mean > cost) cost = mean;
+      const double dw_alone = n1 > 0.0 ? t2 : static_cast<double>(static_cast<long long>((n2 + g - 1.0) / g)) * t2;
+      if (n2 > 0.0 && dw_alone > cost) cost = dw_alone;
+      if (split > 1) cost += 10.0;
+      if (cost < best_cost) {
+        best_cost = cost;
+        best.width = width;
+        best.split = split;
+        best.slice_kb = slice;
+      }
     }
   }
   return best;
+}
+
+// Workspace of the gated block's gradients: dG, dU, and dX's partial sums.
+unsigned long long grads_base_bytes(int M, int F) {
+  return 4ull * static_cast<unsigned long long>(M) * ((static_cast<unsigned long long>(F) + 7) / 8 * 8);
+}
+unsigned long long grads_partial_bytes(int M, int K, int split) {
+  return split > 1 ? 4ull * static_cast<unsigned long long>(split) * M * K : 0;
 }
 
 // bf16 operand maps of the tiled kernel: K-major boxes of 64 k x 128 rows (or
@@ -526,17 +549,23 @@ extern "C" int b200gemm_bf16_gated(b200gemm_t h, int M, int F, int K, const void
   }
 }
 
-extern "C" unsigned long long b200gemm_gated_backward_workspace(int M, int F) {
-  if (M <= 0 || F <= 0) return 0;
-  const unsigned long long pitch = (static_cast<unsigned long long>(F) + 7) / 8 * 8;
-  return 4ull * static_cast<unsigned long long>(M) * pitch;
+extern "C" unsigned long long b200gemm_gated_backward_workspace(b200gemm_t h, int M, int F, int K) {
+  if (h == nullptr || M <= 0 || F <= 0 || K <= 0 || M > kMaxExtent || F > kMaxExtent || K > kMaxExtent) return 0;
+  std::lock_guard<std::mutex> lock(h->mu);
+  int split = 1;
+  for (bool dw : {false, true}) {
+    const int s = grads_plan(h, M, F, K, true, dw, true).split;
+    split = s > split ? s : split;
+  }
+  return (grads_base_bytes(M, F) + 15) / 16 * 16 + grads_partial_bytes(M, K, split);
 }
 
 extern "C" int b200gemm_bf16_gated_backward(b200gemm_t h, int M, int F, int K, const void* dH, long long lddh,
                                             const void* X, long long ldx, const void* Wg, const void* Wu,
                                             long long ldw, const void* G, const void* U, long long ldgu,
                                             int activation, void* dX, long long lddx, void* dWg, void* dWu,
-                                            long long lddw, void* workspace, void* stream_ptr) {
+                                            long long lddw, void* workspace, unsigned long long workspace_bytes,
+                                            void* stream_ptr) {
   if (h == nullptr || M < 0 || F < 0 || K < 0 || !valid_activation(activation)) return B200GEMM_ERR_INVALID_ARG;
   if ((dWg == nullptr) != (dWu == nullptr)) return B200GEMM_ERR_INVALID_ARG;
   if (K == 0 || (dX == nullptr && dWg == nullptr)) return B200GEMM_OK;
@@ -566,7 +595,9 @@ extern "C" int b200gemm_bf16_gated_backward(b200gemm_t h, int M, int F, int K, c
   for (const void* q : {dH, X, Wg, Wu, G, U, static_cast<const void*>(workspace)})
     if (!aligned16(q)) return B200GEMM_ERR_UNSUPPORTED;
   const long long f8 = (static_cast<long long>(F) + 7) / 8 * 8;
-  const Extent e[] = {{workspace, 2ll * M, 2 * f8, 2 * f8},
+  const unsigned long long base_bytes = grads_base_bytes(M, F);
+  if (workspace_bytes < base_bytes) return B200GEMM_ERR_UNSUPPORTED;
+  const Extent e[] = {{workspace, 1, static_cast<long long>(workspace_bytes), 0},
                       {dX, M, 2ll * K, 2 * lddx},
                       {dWg, F, 2ll * K, 2 * lddw},
                       {dWu, F, 2ll * K, 2 * lddw},
@@ -610,25 +641,34 @@ extern "C" int b200gemm_bf16_gated_backward(b200gemm_t h, int M, int F, int K, c
     return B200GEMM_ERR_CUDA;
   if (dX == nullptr) m.c[0] = m.c[1];  // (not written)
   if (dWg == nullptr) m.c[1] = m.c[2] = m.c[0];
-  int width;
+  GradsPlan plan;
   {
     std::lock_guard<std::mutex> lock(h->mu);
-    width = ffn_grads_width(h, M, F, K, dX != nullptr, dWg != nullptr);
+    plan = grads_plan(h, M, F, K, dX != nullptr, dWg != nullptr, true);
+    if (plan.split > 1 && workspace_bytes < base_bytes + grads_partial_bytes(M, K, plan.split))
+      plan = grads_plan(h, M, F, K, dX != nullptr, dWg != nullptr, false);
   }
+  const int width = plan.width;
   FfnParams p{};
   p.seg_kb = (F + kBlockK - 1) / kBlockK;
-  p.first = ffn_set(M, K, 2 * p.seg_kb, width, dX != nullptr ? 1 : 0);
+  p.split = plan.split;
+  p.slice_kb = plan.slice_kb;
+  p.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + base_bytes);  // (a multiple of 32 bytes in)
+  p.first = ffn_set(M, K, 2 * p.seg_kb, width, dX != nullptr ? plan.split : 0);
   p.second = ffn_set(F, K, (M + kBlockK - 1) / kBlockK, width, dWg != nullptr ? 2 : 0);
-  p.ahead =
-      static_cast<int>(ffn_tile_time(width, p.first.num_kb, 0.0) / ffn_tile_time(width, p.second.num_kb, 0.0) + 0.5);
+  p.ahead = static_cast<int>(ffn_tile_time(width, plan.split > 1 ? plan.slice_kb : p.first.num_kb, 0.0) /
+                                 ffn_tile_time(width, p.second.num_kb, 0.0) + 0.5);
   p.out[0] = {static_cast<uint16_t*>(dX), lddx};
   p.out[1] = {static_cast<uint16_t*>(dWg), lddw};
   p.out[2] = {static_cast<uint16_t*>(dWu), lddw};
-  switch (width) {
-    case 512: return run_ffn<FfnGrads512>(h, m, p, stream, true);
-    case 128: return run_ffn<FfnGrads128>(h, m, p, stream, true);
-    default: return run_ffn<FfnGrads256>(h, m, p, stream, true);
-  }
+  const int rc = width == 512   ? run_ffn<FfnGrads512>(h, m, p, stream, true)
+                 : width == 128 ? run_ffn<FfnGrads128>(h, m, p, stream, true)
+                                : run_ffn<FfnGrads256>(h, m, p, stream, true);
+  if (rc != B200GEMM_OK || dX == nullptr || plan.split == 1) return rc;
+  const long long groups = static_cast<long long>(M) * (K / 8);
+  dx_sum_kernel<<<static_cast<unsigned>((groups + 255) / 256), 256, 0, stream>>>(
+      p.partials, plan.split, M, K, static_cast<uint16_t*>(dX), lddx);
+  return cudaGetLastError() == cudaSuccess ? B200GEMM_OK : B200GEMM_ERR_CUDA;
 }
 
 namespace {

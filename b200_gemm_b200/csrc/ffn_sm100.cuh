@@ -46,13 +46,18 @@ struct FfnSet {
   int num_kb;        // K blocks of a tile
   int tiles_m;       // tile rows (dW: of one of the two matrices)
   int tiles_n;       // tile columns
-  int tiles;         // tiles in all (dW: of both matrices)
+  int tiles;         // tiles in all (dW: of both matrices; dX: of every K range)
 };
 
 struct FfnParams {
   FfnSet first;      // gated, or dX
   FfnSet second;     // dW
   int seg_kb;        // dX: K blocks of the first product (num_kb = 2 seg_kb)
+  // dX split over its sum, where it has too few tiles for the clusters: range
+  // s of `split` covers K blocks [s slice_kb, ..) and writes fp32 partial sums
+  // to partials[s][M][N] (dX_sum_kernel adds them); split = 1: none of that.
+  int split, slice_kb;
+  float* partials;
   int ahead;         // dW tiles that a cluster without a last dX tile takes meanwhile
   int band;          // tile rows per band of the tile order
   int act;           // kAct*
@@ -153,6 +158,7 @@ __device__ __forceinline__ void ffn_tile(int band, int tiles_m, int tiles_n, int
 struct FfnUnit {
   bool second;   // of the second set: dW
   bool up;       // dW: a tile of dWu
+  int slice;     // dX: its K range
   int tm, tn;
 };
 template <int KIND>
@@ -160,8 +166,15 @@ __device__ __forceinline__ bool ffn_unit(const FfnParams& p, int c, int g, int i
   const int q = p.first.tiles / g, r = p.first.tiles - q * g;
   const int mine = q + (c < r ? 1 : 0);
   u.second = u.up = false;
+  u.slice = 0;
   if (i < mine) {
-    ffn_tile(p.band, p.first.tiles_m, p.first.tiles_n, i * g + c, u.tm, u.tn);
+    int t = i * g + c;
+    if (KIND == kGrads && p.split > 1) {  // a range's tiles follow one another
+      const int cells = p.first.tiles_m * p.first.tiles_n;
+      u.slice = t / cells;
+      t -= u.slice * cells;
+    }
+    ffn_tile(p.band, p.first.tiles_m, p.first.tiles_n, t, u.tm, u.tn);
     return true;
   }
   if constexpr (KIND == kGated) return false;
@@ -277,6 +290,17 @@ __device__ __forceinline__ void ffn_store_chunk(const uint32_t (&w)[16], int col
   if (++cbuf == BUFS) cbuf = 0;
 }
 
+// K blocks [first, end) of a unit.
+template <int KIND>
+__device__ __forceinline__ void ffn_range(const FfnParams& p, const FfnUnit& u, int& first, int& end) {
+  first = 0;
+  end = u.second ? p.second.num_kb : p.first.num_kb;
+  if (KIND == kGrads && !u.second && p.split > 1) {
+    first = u.slice * p.slice_kb;
+    end = min(end, first + p.slice_kb);
+  }
+}
+
 // The K blocks of one tile through the MMA: false when a wait ran out.
 template <class Cfg, bool A_MN, bool B_MN>
 __device__ __forceinline__ bool ffn_mma_tile(uint32_t sA, uint32_t sB, uint32_t full0, uint32_t own_empty0,
@@ -372,8 +396,9 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1) __cluster_dims__(2, 1, 1)
       for (int i = 0; ok && ffn_unit<Cfg::kKind>(p, cluster, nclusters, i, u); ++i) {
         const int row_a = u.tm * kTileM + static_cast<int>(rank) * 128;
         const int row_b = u.tn * Cfg::kTileN + ((Cfg::kKind == kGated && NB == 1) ? 0 : static_cast<int>(rank) * Cfg::kBRows);
-        const int num_kb = u.second ? p.second.num_kb : p.first.num_kb;
-        for (int kb = 0; kb < num_kb; ++kb) {
+        int kb_first, kb_end;
+        ffn_range<Cfg::kKind>(p, u, kb_first, kb_end);
+        for (int kb = kb_first; kb < kb_end; ++kb) {
           if (!ptx::mbar_wait(empty0 + 8 * stage, phase ^ 1u, wd, kSiteProducer, static_cast<unsigned>(i))) {
             ok = false;
             break;
@@ -429,15 +454,18 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1) __cluster_dims__(2, 1, 1)
         ptx::tc_fence_after();
         const uint32_t d_tmem = tmem_base + acc * 256u;
         bool ok;
+        int kb_first, kb_end;
+        ffn_range<Cfg::kKind>(p, u, kb_first, kb_end);
+        const int num_kb = kb_end - kb_first;
         if constexpr (Cfg::kKind == kGated) {
-          ok = ffn_mma_tile<Cfg, false, false>(sA, sB, full0, own_empty0, peer_empty0, d_tmem, p.first.num_kb, stage,
-                                               phase, wd, unit);
+          ok = ffn_mma_tile<Cfg, false, false>(sA, sB, full0, own_empty0, peer_empty0, d_tmem, num_kb, stage, phase,
+                                               wd, unit);
         } else if (u.second) {
-          ok = ffn_mma_tile<Cfg, true, true>(sA, sB, full0, own_empty0, peer_empty0, d_tmem, p.second.num_kb, stage,
-                                             phase, wd, unit);
+          ok = ffn_mma_tile<Cfg, true, true>(sA, sB, full0, own_empty0, peer_empty0, d_tmem, num_kb, stage, phase, wd,
+                                             unit);
         } else {
-          ok = ffn_mma_tile<Cfg, false, true>(sA, sB, full0, own_empty0, peer_empty0, d_tmem, p.first.num_kb, stage,
-                                              phase, wd, unit);
+          ok = ffn_mma_tile<Cfg, false, true>(sA, sB, full0, own_empty0, peer_empty0, d_tmem, num_kb, stage, phase, wd,
+                                              unit);
         }
         if (!ok) break;
         ptx::mma_commit_cg2(own_tfull0 + 8 * acc);
@@ -505,7 +533,24 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1) __cluster_dims__(2, 1, 1)
         const int M = u.second ? p.second.M : p.first.M, N = p.first.N;  // (N is K for all three)
         const CUtensorMap* map = &maps.c[which];
         constexpr int kHeld = Cfg::kWarpChunks - Cfg::kCBufs;
-        if (NB == 2 && row < M && col0 + Cfg::kWarpCols <= N) {
+        if (!u.second && p.split > 1) {
+          // fp32 partial sums of this K range, straight from the registers (a
+          // lane's row, 16 bytes at a time; N % 8 == 0).
+          const int r = row + static_cast<int>(lane);
+          float* dst = p.partials + (static_cast<long long>(u.slice) * M + r) * N;
+#pragma unroll 1
+          for (int c = 0; c < Cfg::kWarpChunks; ++c) {
+            uint32_t v[32];
+            ptx::tmem_ld_32x32b_x32(t_row + c * kCBoxCols, v);
+            ptx::tmem_wait_ld();
+            ptx::reg_fence32(v);
+            if (c == Cfg::kWarpChunks - 1) release();
+            const int col = col0 + c * kCBoxCols;
+#pragma unroll
+            for (int j = 0; j < 32; j += 4)
+              if (r < M && col + j < N) ptx::st_global_v4(dst + col + j, v[j], v[j + 1], v[j + 2], v[j + 3]);
+          }
+        } else if (NB == 2 && row < M && col0 + Cfg::kWarpCols <= N) {
           // The single accumulator holds the next tile's MMAs up until it is
           // read: half of a warp's chunks go into its staging buffers and half
           // into registers, then it is released, then the stores are issued.
@@ -613,6 +658,32 @@ __global__ void __launch_bounds__(256) gated_grad_kernel(const GatedGradParams p
     ptx::st_global_v4(p.dg + r * p.ldo + col, dg[0], dg[1], dg[2], dg[3]);
     ptx::st_global_v4(p.du + r * p.ldo + col, du[0], du[1], du[2], du[3]);
   }
+}
+
+// dX from its K ranges' partial sums, added in range order and rounded once;
+// a thread takes 8 columns.
+__global__ void __launch_bounds__(256) dx_sum_kernel(const float* partials, int split, int M, int N, uint16_t* dx,
+                                                     long long ld) {
+  const int groups = N / 8;
+  const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+  const long long r = i / groups;
+  if (r >= M) return;
+  const int col = static_cast<int>(i - r * groups) * 8;
+  float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f), b = a;
+  for (int s = 0; s < split; ++s) {
+    const auto* src = reinterpret_cast<const float4*>(partials + (s * static_cast<long long>(M) + r) * N + col);
+    const float4 x = src[0], y = src[1];
+    a.x += x.x;
+    a.y += x.y;
+    a.z += x.z;
+    a.w += x.w;
+    b.x += y.x;
+    b.y += y.y;
+    b.z += y.z;
+    b.w += y.w;
+  }
+  auto pack = [](float lo, float hi) { return ptx::pack_bf16x2(__float_as_uint(lo), __float_as_uint(hi)); };
+  ptx::st_global_v4(dx + r * ld + col, pack(a.x, a.y), pack(a.z, a.w), pack(b.x, b.y), pack(b.z, b.w));
 }
 
 }  // namespace b200gemm

@@ -146,13 +146,13 @@ class FfnOps:
                 dWu, lddw = self._empty(F, K, bf16)
             # Freed when this returns: the allocator hands it on in the order of
             # the stream that it was allocated for, which is the call's.
-            ws = torch.empty(max(16, self._lib.b200gemm_gated_backward_workspace(M, F)), dtype=torch.uint8,
-                             device=torch.device("cuda", self.device))
+            ws_bytes = self._lib.b200gemm_gated_backward_workspace(self._h, M, F, K)
+            ws = torch.empty(ws_bytes + 16, dtype=torch.uint8, device=torch.device("cuda", self.device))
             rc = self._lib.b200gemm_bf16_gated_backward(
                 self._h, M, F, K, dH.data_ptr(), lddh, X.data_ptr(), ldx, Wg.data_ptr(), Wu.data_ptr(), ldw,
                 G.data_ptr(), U.data_ptr(), ldgu, act, None if dX is None else dX.data_ptr(), lddx,
                 None if dWg is None else dWg.data_ptr(), None if dWu is None else dWu.data_ptr(), lddw,
-                ws.data_ptr(), ptr)
+                ws.data_ptr(), ws_bytes, ptr)
         _lib.check(rc, "b200gemm_bf16_gated_backward")
         return dX, dWg, dWu
 

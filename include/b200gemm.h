@@ -320,9 +320,11 @@ int b200gemm_bf16_gated(b200gemm_t handle, int M, int F, int K, const void* X, l
                         const void* Wg, const void* Wu, long long ldw, int activation, void* H,
                         long long ldh, void* G, void* U, long long ldgu, void* stream);
 
-/* Bytes of workspace a b200gemm_bf16_gated_backward call of this size needs
- * (dG and dU in bf16; 0 for an empty one). */
-unsigned long long b200gemm_gated_backward_workspace(int M, int F);
+/* Bytes of workspace for b200gemm_bf16_gated_backward calls of this size on
+ * this handle (0 for an empty one or a null handle): dG and dU in bf16, 4 M F'
+ * bytes with F' = F rounded up to 8, and, where dX has too few tiles to occupy
+ * the device, room for fp32 partial sums of it. */
+unsigned long long b200gemm_gated_backward_workspace(b200gemm_t handle, int M, int F, int K);
 
 /* Gradients of the gated block from dH [M,F], given X, Wg, Wu and the saved
  * G and U (the bf16 values are taken as they are):
@@ -333,14 +335,16 @@ unsigned long long b200gemm_gated_backward_workspace(int M, int F);
  * may dWg and dWu together: those are then not computed.  With M == 0 the
  * weight gradients are zeros, with F == 0 dX is.  act'(0) of relu is 0.
  * workspace: 16-byte aligned, its contents before and after mean nothing; it
- * is in use until the call's work on `stream` is done.  The same rules as
+ * is in use until the call's work on `stream` is done.  With less than the
+ * size above the call does without partial sums; less than 4 M F' bytes is
+ * B200GEMM_ERR_UNSUPPORTED.  The same rules as
  * b200gemm_bf16_gated otherwise. */
 int b200gemm_bf16_gated_backward(b200gemm_t handle, int M, int F, int K, const void* dH,
                                  long long lddh, const void* X, long long ldx, const void* Wg,
                                  const void* Wu, long long ldw, const void* G, const void* U,
                                  long long ldgu, int activation, void* dX, long long lddx,
                                  void* dWg, void* dWu, long long lddw, void* workspace,
-                                 void* stream);
+                                 unsigned long long workspace_bytes, void* stream);
 
 /* 4-bit weights: W[n][k] = scales[k / group][n] * (q[n][k] - 8), q in 0..15.
  *   codes   [N][K / 2] bytes, contiguous, 16-byte aligned: byte b of a row

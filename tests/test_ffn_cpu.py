@@ -50,9 +50,9 @@ def test_column_slices_of_one_matrix_are_apart():
 
 
 def _backward(handle=H, M=4, F=16, K=64, dH=_at(0), lddh=16, X=_at(1), ldx=64, Wg=_at(2), Wu=_at(3), ldw=64, G=_at(4),
-              U=_at(5), ldgu=16, act=4, dX=_at(6), lddx=64, dWg=_at(7), dWu=_at(8), lddw=64, ws=_at(9)):
+              U=_at(5), ldgu=16, act=4, dX=_at(6), lddx=64, dWg=_at(7), dWu=_at(8), lddw=64, ws=_at(9), ws_bytes=4 * 4 * 16):
     return _lib.load().b200gemm_bf16_gated_backward(handle, M, F, K, dH, lddh, X, ldx, Wg, Wu, ldw, G, U, ldgu, act, dX,
-                                                    lddx, dWg, dWu, lddw, ws, None)
+                                                    lddx, dWg, dWu, lddw, ws, ws_bytes, None)
 
 
 @pytest.mark.parametrize("change,code", [
@@ -63,17 +63,16 @@ def _backward(handle=H, M=4, F=16, K=64, dH=_at(0), lddh=16, X=_at(1), ldx=64, W
     (dict(ws=_at(9) + 4), UNSUPPORTED), (dict(dH=None), INVALID), (dict(G=None), INVALID), (dict(ws=None), INVALID),
     (dict(K=2 ** 31 - 8), UNSUPPORTED), (dict(dX=_at(1)), INVALID), (dict(dX=_at(0)), INVALID),
     (dict(dWg=_at(2)), INVALID), (dict(dWg=_at(7), dWu=_at(7)), INVALID), (dict(ws=_at(6)), INVALID),
-    (dict(ws=_at(4)), INVALID),
+    (dict(ws=_at(4)), INVALID), (dict(ws_bytes=4 * 4 * 16 - 1), UNSUPPORTED),
+    (dict(ws=_at(6) - 4096, ws_bytes=4097), INVALID), (dict(F=9, ws_bytes=4 * 4 * 16 - 1), UNSUPPORTED),
 ])
 def test_backward(change, code):
     assert _backward(**change) == code
 
 
-def test_workspace_size():
+def test_workspace_size_of_nothing():
     size = _lib.load().b200gemm_gated_backward_workspace
-    assert size(0, 5) == 0 and size(5, 0) == 0 and size(-1, 4) == 0
-    assert size(3, 9) == 2 * 3 * 16 * 2
-    assert size(1 << 20, 1 << 15) == 4 << 35  # past 32 bits
+    assert size(H, 0, 5, 8) == 0 and size(H, 5, 0, 8) == 0 and size(H, -1, 4, 8) == 0 and size(None, 4, 4, 8) == 0
 
 
 def _nt(handle=H, M=2, N=64, K=128, A=_at(0), lda=128, codes=_at(1), scales=_at(2), group=32, C=_at(3), ldc=64, out=0):

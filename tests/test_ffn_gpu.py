@@ -113,23 +113,26 @@ def _backward_raw(h, dh, x, wg, wu, g, u, kind, workspace, dx, dwg, dwu):
         h._h, M, F, K, dh.data_ptr(), dh.stride(0), x.data_ptr(), x.stride(0), wg.data_ptr(), wu.data_ptr(),
         wg.stride(0), g.data_ptr(), u.data_ptr(), g.stride(0),
         {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}[kind], dx.data_ptr(), dx.stride(0),
-        dwg.data_ptr(), dwu.data_ptr(), dwg.stride(0), workspace.data_ptr(),
+        dwg.data_ptr(), dwu.data_ptr(), dwg.stride(0), workspace.data_ptr(), workspace.numel(),
         torch.cuda.current_stream().cuda_stream)
     assert rc == 0
     assert h.last_device_status()[0] == 0
 
 
-def _check_backward(h, M, F, K, kind, pad=0, seed=0):
+def _check_backward(h, M, F, K, kind, pad=0, seed=0, small_workspace=False):
     dh = plain.rows(M, F, seed, 0.1, pad=pad)
     g, u = (plain.rows(M, F, seed + i, 1.5, pad=pad) for i in (1, 2))
     x = plain.rows(M, K, seed + 3, pad=pad)
     wg, wu = (plain.rows(F, K, seed + i, K ** -0.5, pad=pad) for i in (4, 5))
     f8 = 8 * ((F + 7) // 8)
-    ws = torch.full((2, M, f8), float("nan"), dtype=BF, device="cuda")  # its contents mean nothing
-    assert _lib.load().b200gemm_gated_backward_workspace(M, F) == 2 * ws.numel()
+    base = 4 * M * f8
+    size = _lib.load().b200gemm_gated_backward_workspace(h._h, M, F, K)
+    assert size >= base
+    buf = torch.full((base if small_workspace else size,), 255, dtype=torch.uint8, device="cuda")  # NaN, as it happens
+    ws = buf[:base].view(BF).view(2, M, f8)
     outs = [torch.full((r + 2, K + 8), 7.0, dtype=BF, device="cuda") for r in (M, F, F)]
     dx, dwg, dwu = (b[:r, :K] for b, r in zip(outs, (M, F, F)))
-    _backward_raw(h, dh, x, wg, wu, g, u, kind, ws, dx, dwg, dwu)
+    _backward_raw(h, dh, x, wg, wu, g, u, kind, buf, dx, dwg, dwu)
     # dG and dU element by element, then the products of what they were rounded to
     rdg, edg, rdu, edu = plain.grads(dh, g, u, kind)
     dg, du = ws[0, :, :F].double(), ws[1, :, :F].double()
@@ -159,6 +162,16 @@ def test_backward_tiled(gpu_handle, M, F, K, width):
         _check_backward(gpu_handle, M, F, K, "silu", pad=16, seed=3)
     finally:
         gpu_handle.set_tile_width(0)
+
+
+@pytest.mark.parametrize("M,F,K", [(1, 5003, 2056), (40, 9000, 264), (300, 4100, 520), (17, 1100, 72)])
+@pytest.mark.parametrize("small_workspace", [False, True])
+def test_backward_split(gpu_handle, M, F, K, small_workspace):
+    """dX of few tiles: its sum in ranges, with partial sums in the workspace;
+    and without, when the workspace has no room for them."""
+    size = _lib.load().b200gemm_gated_backward_workspace(gpu_handle._h, M, F, K)
+    assert size > 4 * M * 8 * ((F + 7) // 8)  # a case that is split
+    _check_backward(gpu_handle, M, F, K, "silu", seed=M, small_workspace=small_workspace)
 
 
 def test_backward_many_tiles(gpu_handle):
@@ -197,9 +210,10 @@ def test_backward_extreme_gates(gpu_handle, kind):
     g[0], g[1], g[2], g[3] = 1e4, -1e4, 3e38, -3e38
     one = torch.ones(M, F, dtype=BF, device="cuda")
     x, w = torch.ones(M, K, dtype=BF, device="cuda"), torch.full((F, K), 2.0 ** -130, dtype=BF, device="cuda")
-    ws = torch.empty(2, M, F, dtype=BF, device="cuda")
+    buf = torch.empty(4 * M * F, dtype=torch.uint8, device="cuda")
+    ws = buf.view(BF).view(2, M, F)
     dx, dwg, dwu = (torch.empty(r, K, dtype=BF, device="cuda") for r in (M, F, F))
-    _backward_raw(gpu_handle, one, x, w, w, g, one, kind, ws, dx, dwg, dwu)
+    _backward_raw(gpu_handle, one, x, w, w, g, one, kind, buf, dx, dwg, dwu)
     assert torch.equal(ws[0, :, 0].float().cpu(), torch.tensor([1.0, 0.0, 1.0, 0.0]))
     assert (ws[1, 1] == 0).all() and (ws[1, 3] == 0).all()
     assert torch.equal(ws[1, 0], g[0]) and torch.equal(ws[1, 2], g[2])
