@@ -213,6 +213,15 @@ double ffn_tile_time(int width, int num_kb, double epi) {
   return num_kb * (0.08 + 0.92 * feed) / 0.85 + 4.0;
 }
 
+// The same for a dW tile, which takes at least as long as its stores do: with
+// one K block (dW of a few rows of X, 14336 x 4096) tiles of 512, 256 and 128
+// columns took about 6.5, 4.5 and 3 us next to dX's.
+double dw_tile_time(int width, int num_kb) {
+  const double t = ffn_tile_time(width, num_kb, 0.0);
+  const double stores = width == 512 ? 20.0 : (width == 256 ? 14.0 : 10.0);
+  return t > stores ? t : stores;
+}
+
 // Accumulator columns of the gated block's tiles (twice H's): by waves of
 // tiles.  A forced tile width asks for the nearest one there is.
 int ffn_gated_width(const b200gemm_handle* h, int tiles_m, int F, int num_kb) {
@@ -248,7 +257,7 @@ GradsPlan grads_plan(const b200gemm_handle* h, int m, int f, int k, bool dx, boo
     if (h->tile_width != 0 && width != (h->tile_width >= 448 ? 512 : (h->tile_width >= 192 ? 256 : 128))) continue;
     const double tn = static_cast<double>((k + width - 1ll) / width);
     const double n1 = dx ? tn * ((m + 255ll) / 256) : 0.0, n2 = dw ? 2.0 * tn * ((f + 255ll) / 256) : 0.0;
-    const double t2 = ffn_tile_time(width, (m + 63) / 64, 0.0);
+    const double t2 = dw_tile_time(width, (m + 63) / 64);
     for (int want = 1; want <= (dx && may_split ? 16 : 1); want *= 2) {
       const int slice = (kb + want - 1) / want, split = (kb + slice - 1) / slice;
       if (split > 1 && (slice < 8 || n1 * split > 2.0 * g)) break;
@@ -511,7 +520,7 @@ extern "C" int b200gemm_bf16_gated(b200gemm_t h, int M, int F, int K, const void
   const int num_kb = (K + kBlockK - 1) / kBlockK;
   {
     std::lock_guard<std::mutex> lock(h->mu);
-    small = G == nullptr && gated_uses_decode(h, M, F, K);
+    small = gated_uses_decode(h, M, F, K);
     width = ffn_gated_width(h, (M + kTileM - 1) / kTileM, F, num_kb);
   }
   if (small) {
@@ -522,6 +531,9 @@ extern "C" int b200gemm_bf16_gated(b200gemm_t h, int M, int F, int K, const void
     p.act = activation;
     p.out = static_cast<uint16_t*>(H);
     p.ldo = ldh;
+    p.gate = static_cast<uint16_t*>(G);
+    p.up = static_cast<uint16_t*>(U);
+    p.ldgu = ldgu;
     return run_gated_decode(h, Wg, Wu, ldw, X, ldx, p, stream);
   }
   FfnMaps m;
@@ -657,7 +669,7 @@ extern "C" int b200gemm_bf16_gated_backward(b200gemm_t h, int M, int F, int K, c
   p.first = ffn_set(M, K, 2 * p.seg_kb, width, dX != nullptr ? plan.split : 0);
   p.second = ffn_set(F, K, (M + kBlockK - 1) / kBlockK, width, dWg != nullptr ? 2 : 0);
   p.ahead = static_cast<int>(ffn_tile_time(width, plan.split > 1 ? plan.slice_kb : p.first.num_kb, 0.0) /
-                                 ffn_tile_time(width, p.second.num_kb, 0.0) + 0.5);
+                                 dw_tile_time(width, p.second.num_kb) + 0.5);
   p.out[0] = {static_cast<uint16_t*>(dX), lddx};
   p.out[1] = {static_cast<uint16_t*>(dWg), lddw};
   p.out[2] = {static_cast<uint16_t*>(dWu), lddw};

@@ -33,6 +33,8 @@ struct GatedDecodeParams {
   int act;                 // kAct*
   uint16_t* out;           // H, bf16 bits
   long long ldo;           // elements
+  uint16_t *gate, *up;     // G and U, or null
+  long long ldgu;
   unsigned int* status;
   unsigned long long timeout_ns;
   int pdl;
@@ -259,8 +261,13 @@ __global__ void __launch_bounds__(Cfg::kThreads, Cfg::kCtas)
       const int tok = idx / kCols, c = idx % kCols;
       if (m0 + tok >= p.M || n0 + c >= p.F) continue;
       const float gate = total(tok * Cfg::kPitch + c), up = total(tok * Cfg::kPitch + 32 + c);
-      const float v = gated_value(p.act, gate, up);
-      p.out[static_cast<long long>(m0 + tok) * p.ldo + n0 + c] = __bfloat16_as_ushort(__float2bfloat16_rn(v));
+      const long long r = m0 + tok;
+      auto bits = [](float v) { return __bfloat16_as_ushort(__float2bfloat16_rn(v)); };
+      p.out[r * p.ldo + n0 + c] = bits(gated_value(p.act, gate, up));
+      if (p.gate != nullptr) {
+        p.gate[r * p.ldgu + n0 + c] = bits(gate);
+        p.up[r * p.ldgu + n0 + c] = bits(up);
+      }
     }
   }
   if (threadIdx.x == 0 && ptx::aborted(wd)) ptx::sleep_ns_bounded(200000ull);

@@ -9,14 +9,22 @@ torch stream or a raw pointer; default: the current stream of the handle's
 device); tensors that it allocates are allocated for that stream."""
 from __future__ import annotations
 
-import contextlib
-
 from . import _lib
 
 ACTIVATIONS = {"none": _lib.ACT_NONE, "relu": _lib.ACT_RELU, "gelu": _lib.ACT_GELU,
                "gelu_tanh": _lib.ACT_GELU_TANH, "silu": _lib.ACT_SILU}
 W4_GROUPS = (32, 64, 128, 256)
-_NO_CONTEXT = contextlib.nullcontext()
+class _NoContext:
+    """contextlib.nullcontext without its cost."""
+
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return None
+
+
+_NO_CONTEXT = _NoContext()
 _torch_module = None
 
 
@@ -69,12 +77,12 @@ class FfnOps:
             raise ValueError(f"stream must belong to cuda:{self.device}")
         return int(stream.cuda_stream), torch.cuda.stream(stream)
 
-    def _empty(self, rows: int, cols: int, dtype):
-        """A [rows, cols] matrix whose rows start on 16-byte boundaries, and its
-        row pitch."""
-        torch = _torch()
-        pitch = 8 * ((cols + 7) // 8)
-        t = torch.empty((rows, pitch), dtype=dtype, device=torch.device("cuda", self.device))
+    @staticmethod
+    def _empty(like, rows: int, cols: int, dtype=None):
+        """A [rows, cols] matrix on `like`'s device (of its type, or `dtype`)
+        whose rows start on 16-byte boundaries, and its row pitch."""
+        pitch = cols + -cols % 8
+        t = like.new_empty((rows, pitch)) if dtype is None else like.new_empty((rows, pitch), dtype=dtype)
         return (t if pitch == cols else t[:, :cols]), pitch
 
     # ------------------------------------------------------------ gated block
@@ -99,12 +107,12 @@ class FfnOps:
         ptr, where = self._where(stream)
         ldgu = 0
         with where:
-            H, ldh = self._empty(M, F, bf16) if out is None else (out, self._check(out, "out", bf16, M, F))
+            H, ldh = self._empty(X, M, F) if out is None else (out, self._check(out, "out", bf16, M, F))
             G = U = None
             if save or gate_out is not None or up_out is not None:
-                G, ldgu = (self._empty(M, F, bf16) if gate_out is None
+                G, ldgu = (self._empty(X, M, F) if gate_out is None
                            else (gate_out, self._check(gate_out, "gate_out", bf16, M, F)))
-                U, ldu = (self._empty(M, F, bf16) if up_out is None
+                U, ldu = (self._empty(X, M, F) if up_out is None
                           else (up_out, self._check(up_out, "up_out", bf16, M, F)))
                 if ldu != ldgu:
                     raise ValueError("gate_out and up_out must have the same row stride")
@@ -140,14 +148,14 @@ class FfnOps:
             dX = dWg = dWu = None
             lddx = lddw = 0
             if input_grad:
-                dX, lddx = self._empty(M, K, bf16)
+                dX, lddx = self._empty(X, M, K)
             if weight_grad:
-                dWg, lddw = self._empty(F, K, bf16)
-                dWu, lddw = self._empty(F, K, bf16)
+                dWg, lddw = self._empty(X, F, K)
+                dWu, lddw = self._empty(X, F, K)
             # Freed when this returns: the allocator hands it on in the order of
             # the stream that it was allocated for, which is the call's.
             ws_bytes = self._lib.b200gemm_gated_backward_workspace(self._h, M, F, K)
-            ws = torch.empty(ws_bytes + 16, dtype=torch.uint8, device=torch.device("cuda", self.device))
+            ws = X.new_empty(ws_bytes + 16, dtype=torch.uint8)
             rc = self._lib.b200gemm_bf16_gated_backward(
                 self._h, M, F, K, dH.data_ptr(), lddh, X.data_ptr(), ldx, Wg.data_ptr(), Wu.data_ptr(), ldw,
                 G.data_ptr(), U.data_ptr(), ldgu, act, None if dX is None else dX.data_ptr(), lddx,
@@ -204,7 +212,7 @@ class FfnOps:
         ptr, where = self._where(stream)
         with where:
             bf16 = torch.bfloat16
-            W, ldw = self._empty(N, K, bf16) if out is None else (out, self._check(out, "out", bf16, N, K))
+            W, ldw = self._empty(scales, N, K) if out is None else (out, self._check(out, "out", bf16, N, K))
             rc = self._lib.b200gemm_w4_dequantize(self._h, N, K, codes.data_ptr(), scales.data_ptr(), group,
                                                   W.data_ptr(), ldw, ptr)
         _lib.check(rc, "b200gemm_w4_dequantize")
@@ -224,7 +232,7 @@ class FfnOps:
             raise TypeError("out_dtype must be torch.bfloat16 or torch.float32")
         ptr, where = self._where(stream)
         with where:
-            C, ldc = (self._empty(M, N, out_dtype) if out is None
+            C, ldc = (self._empty(A, M, N, None if out_dtype is A.dtype else out_dtype) if out is None
                       else (out, self._check(out, "out", out_dtype, M, N)))
             rc = self._lib.b200gemm_w4_nt(self._h, M, N, K, A.data_ptr(), lda, codes.data_ptr(), scales.data_ptr(),
                                           group, C.data_ptr(), ldc,
@@ -245,7 +253,7 @@ class FfnOps:
         ptr, where = self._where(stream)
         with where:
             bf16 = torch.bfloat16
-            H, ldh = self._empty(M, F, bf16) if out is None else (out, self._check(out, "out", bf16, M, F))
+            H, ldh = self._empty(X, M, F) if out is None else (out, self._check(out, "out", bf16, M, F))
             rc = self._lib.b200gemm_w4_gated(self._h, M, F, K, X.data_ptr(), ldx, gate_codes.data_ptr(),
                                              gate_scales.data_ptr(), up_codes.data_ptr(), up_scales.data_ptr(), group,
                                              act, H.data_ptr(), ldh, ptr)

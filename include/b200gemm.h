@@ -314,8 +314,9 @@ int b200gemm_bf16_nt_noalloc(int M, int N, int K, const void* A, const void* B, 
  * G and U, both or neither, receive the two products rounded to bf16 (one
  * pitch ldgu): what b200gemm_bf16_gated_backward needs.  Any M and F;
  * K % 8 == 0, K > 0; pitches % 8 == 0; every pointer 16-byte aligned.
- * Up to 32 rows (without G and U) the weights are streamed by every SM; an
- * element's sum then runs in another order than in the tiled kernel. */
+ * Up to 32 rows (up to 128 where the tiled kernel would leave most SMs idle)
+ * run on a kernel whose every SM streams the weights; an element's sum then
+ * runs in another order than in the tiled kernel. */
 int b200gemm_bf16_gated(b200gemm_t handle, int M, int F, int K, const void* X, long long ldx,
                         const void* Wg, const void* Wu, long long ldw, int activation, void* H,
                         long long ldh, void* G, void* U, long long ldgu, void* stream);

@@ -43,7 +43,7 @@ def _check_gated(h, M, F, K, kind, save, pad=0, seed=0):
 @pytest.mark.parametrize("M,F,K", [(1, 64, 64), (3, 1, 8), (8, 33, 136), (9, 257, 512), (17, 130, 1032), (32, 300, 264),
                                    (33, 131, 200), (129, 255, 64), (257, 520, 328)])
 def test_gated(gpu_handle, M, F, K, kind):
-    _check_gated(gpu_handle, M, F, K, kind, save=False, seed=M + F)
+    _check_gated(gpu_handle, M, F, K, kind, save=kind == "gelu", seed=M + F)
 
 
 @pytest.mark.parametrize("M,F,K", [(1, 14000, 4096), (8, 5001, 2056), (12, 3001, 4096), (32, 6000, 2048), (1, 40, 8192),
@@ -51,7 +51,7 @@ def test_gated(gpu_handle, M, F, K, kind):
 def test_gated_few_rows_long(gpu_handle, M, F, K):
     """Few rows against many and long weights: every ring goes around many
     times, every SM holds several blocks; and a width that splits K."""
-    _check_gated(gpu_handle, M, F, K, "silu", save=False, seed=M)
+    _check_gated(gpu_handle, M, F, K, "silu", save=M % 2 == 0, seed=M)
 
 
 @pytest.mark.parametrize("width", [512, 256, 192, 128])
