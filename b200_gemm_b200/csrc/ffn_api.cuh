@@ -203,6 +203,7 @@ bool group_shift_of(int group, int* shift) {
 }
 
 constexpr int kMaxExtent = 0x7FFFFFFF - 4096;  // rows, columns: tile coordinates stay inside an int
+constexpr long long kMaxPitch = 1ll << 38;     // elements: tensor maps take pitches below 2^40 bytes
 
 // Time of one tile with `width` accumulator columns and num_kb K blocks, in
 // the units and by the fit of tile_plan_cost; a 512-wide tile's epilogue is
@@ -507,7 +508,9 @@ extern "C" int b200gemm_bf16_gated(b200gemm_t h, int M, int F, int K, const void
   if (G != nullptr && (ldgu < F || (ldgu % 8) != 0)) return B200GEMM_ERR_UNSUPPORTED;
   for (const void* q : {X, Wg, Wu, static_cast<const void*>(H), static_cast<const void*>(G), static_cast<const void*>(U)})
     if (!aligned16(q)) return B200GEMM_ERR_UNSUPPORTED;
-  if (M > kMaxExtent || F > kMaxExtent || K > kMaxExtent) return B200GEMM_ERR_TOO_LARGE;
+  if (M > kMaxExtent || F > kMaxExtent || K > kMaxExtent || ldx > kMaxPitch || ldw > kMaxPitch || ldh > kMaxPitch ||
+      (G != nullptr && ldgu > kMaxPitch))
+    return B200GEMM_ERR_TOO_LARGE;
   const Extent e[] = {{H, M, 2ll * F, 2 * ldh}, {G, M, 2ll * F, 2 * ldgu}, {U, M, 2ll * F, 2 * ldgu},
                       {X, M, 2ll * K, 2 * ldx}, {Wg, F, 2ll * K, 2 * ldw}, {Wu, F, 2ll * K, 2 * ldw}};
   if (!outputs_distinct(e, 3, 6)) return B200GEMM_ERR_INVALID_ARG;
@@ -586,7 +589,9 @@ extern "C" int b200gemm_bf16_gated_backward(b200gemm_t h, int M, int F, int K, c
   if (dX != nullptr && (lddx < K || (lddx % 8) != 0 || !aligned16(dX))) return B200GEMM_ERR_UNSUPPORTED;
   if (dWg != nullptr && (lddw < K || (lddw % 8) != 0 || !aligned16(dWg) || !aligned16(dWu)))
     return B200GEMM_ERR_UNSUPPORTED;
-  if (M > kMaxExtent || F > kMaxExtent || K > kMaxExtent) return B200GEMM_ERR_TOO_LARGE;
+  if (M > kMaxExtent || F > kMaxExtent || K > kMaxExtent || (dX != nullptr && lddx > kMaxPitch) ||
+      (dWg != nullptr && lddw > kMaxPitch))
+    return B200GEMM_ERR_TOO_LARGE;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
   if (M == 0 || F == 0) {  // empty sums
     DeviceGuard guard(h->device);
@@ -606,6 +611,7 @@ extern "C" int b200gemm_bf16_gated_backward(b200gemm_t h, int M, int F, int K, c
     return B200GEMM_ERR_UNSUPPORTED;
   for (const void* q : {dH, X, Wg, Wu, G, U, static_cast<const void*>(workspace)})
     if (!aligned16(q)) return B200GEMM_ERR_UNSUPPORTED;
+  if (lddh > kMaxPitch || ldx > kMaxPitch || ldw > kMaxPitch || ldgu > kMaxPitch) return B200GEMM_ERR_TOO_LARGE;
   const long long f8 = (static_cast<long long>(F) + 7) / 8 * 8;
   const unsigned long long base_bytes = grads_base_bytes(M, F);
   if (workspace_bytes < base_bytes) return B200GEMM_ERR_UNSUPPORTED;
@@ -702,7 +708,7 @@ int w4_convert_check(b200gemm_t h, int N, int K, const void* W, long long ldw, i
   if (W == nullptr || codes == nullptr || scales == nullptr) return B200GEMM_ERR_INVALID_ARG;
   if (ldw < K || (ldw % 8) != 0 || !aligned16(W) || !aligned16(codes) || !aligned2(scales))
     return B200GEMM_ERR_UNSUPPORTED;
-  if ((static_cast<long long>(N) + 31) / 32 > 65535 || K > kMaxExtent) return B200GEMM_ERR_TOO_LARGE;
+  if ((static_cast<long long>(N) + 31) / 32 > 65535 || K > kMaxExtent || ldw > kMaxPitch) return B200GEMM_ERR_TOO_LARGE;
   return B200GEMM_OK;
 }
 
@@ -766,7 +772,8 @@ extern "C" int b200gemm_w4_nt(b200gemm_t h, int M, int N, int K, const void* A, 
   if (ldc < N || !aligned16(codes) || !aligned2(scales) ||
       (reinterpret_cast<uintptr_t>(C) & static_cast<uintptr_t>(esize - 1)) != 0)
     return B200GEMM_ERR_UNSUPPORTED;
-  if (M > kMaxExtent || N > kMaxExtent || K > kMaxExtent) return B200GEMM_ERR_TOO_LARGE;
+  if (M > kMaxExtent || N > kMaxExtent || K > kMaxExtent || lda > kMaxPitch || ldc > kMaxPitch)
+    return B200GEMM_ERR_TOO_LARGE;
   const Extent e[] = {{C, M, static_cast<long long>(esize) * N, esize * ldc},
                       {A, M, 2ll * K, 2 * lda},
                       {codes, 1, static_cast<long long>(N) * (K / 2), 0},
@@ -800,7 +807,8 @@ extern "C" int b200gemm_w4_gated(b200gemm_t h, int M, int F, int K, const void* 
   if (ldh < F || !aligned16(gate_codes) || !aligned16(up_codes) || !aligned2(gate_scales) || !aligned2(up_scales) ||
       !aligned2(H))
     return B200GEMM_ERR_UNSUPPORTED;
-  if (M > kMaxExtent || F > kMaxExtent || K > kMaxExtent) return B200GEMM_ERR_TOO_LARGE;
+  if (M > kMaxExtent || F > kMaxExtent || K > kMaxExtent || ldx > kMaxPitch || ldh > kMaxPitch)
+    return B200GEMM_ERR_TOO_LARGE;
   const long long code_bytes = static_cast<long long>(F) * (K / 2), scale_bytes = 2ll * F * (K / group);
   const Extent e[] = {{H, M, 2ll * F, 2 * ldh},       {X, M, 2ll * K, 2 * ldx},
                       {gate_codes, 1, code_bytes, 0}, {gate_scales, 1, scale_bytes, 0},

@@ -306,6 +306,9 @@ int b200gemm_bf16_nt_noalloc(int M, int N, int K, const void* A, const void* B, 
  * allocates nothing, waits for nothing and can be captured into a CUDA graph.
  * No output may overlap an input or another output (column slices of one
  * wide matrix do not count as overlapping): B200GEMM_ERR_INVALID_ARG.
+ * Launch overlap (b200gemm_set_pdl) applies to the kernels for few rows: with
+ * B200GEMM_PDL_WEIGHTS_EARLY the weights, codes and scales count as B, which
+ * the previous kernel must not write.
  * ------------------------------------------------------------------- */
 
 /* Gated block, one kernel:  G = X Wg^T,  U = X Wu^T,  H = act(G) * U

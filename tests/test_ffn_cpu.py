@@ -28,7 +28,8 @@ def _gated(handle=H, M=4, F=16, K=64, X=_at(0), ldx=64, Wg=_at(1), Wu=_at(2), ld
     (dict(M=0), OK), (dict(F=0), OK), (dict(K=0), UNSUPPORTED), (dict(K=60), UNSUPPORTED),
     (dict(ldx=56), UNSUPPORTED), (dict(ldx=68), UNSUPPORTED), (dict(ldw=60), UNSUPPORTED), (dict(ldh=12), UNSUPPORTED),
     (dict(ldh=20), UNSUPPORTED), (dict(G=_at(4), U=_at(5), ldgu=8), UNSUPPORTED), (dict(X=_at(0) + 8), UNSUPPORTED),
-    (dict(out=_at(3) + 2), UNSUPPORTED), (dict(M=2 ** 31 - 1), TOO_LARGE),
+    (dict(out=_at(3) + 2), UNSUPPORTED), (dict(M=2 ** 31 - 1), TOO_LARGE), (dict(ldx=2 ** 62), TOO_LARGE),
+    (dict(ldw=2 ** 39), TOO_LARGE), (dict(ldh=2 ** 39), TOO_LARGE),
     (dict(out=_at(0)), INVALID), (dict(out=_at(1) + 15 * 128), INVALID), (dict(G=_at(3), U=_at(5)), INVALID),
     (dict(G=_at(4), U=_at(4)), INVALID), (dict(G=_at(4), U=_at(4) + 16, ldgu=24), INVALID),
 ])
@@ -61,7 +62,8 @@ def _backward(handle=H, M=4, F=16, K=64, dH=_at(0), lddh=16, X=_at(1), ldx=64, W
     (dict(K=12), UNSUPPORTED), (dict(lddx=60), UNSUPPORTED), (dict(lddw=8), UNSUPPORTED), (dict(lddh=8), UNSUPPORTED),
     (dict(ldgu=17), UNSUPPORTED), (dict(ldx=65), UNSUPPORTED), (dict(dX=_at(6) + 2), UNSUPPORTED),
     (dict(ws=_at(9) + 4), UNSUPPORTED), (dict(dH=None), INVALID), (dict(G=None), INVALID), (dict(ws=None), INVALID),
-    (dict(K=2 ** 31 - 8), UNSUPPORTED), (dict(dX=_at(1)), INVALID), (dict(dX=_at(0)), INVALID),
+    (dict(K=2 ** 31 - 8), UNSUPPORTED), (dict(lddx=2 ** 62), TOO_LARGE), (dict(ldgu=2 ** 39), TOO_LARGE),
+    (dict(dX=_at(1)), INVALID), (dict(dX=_at(0)), INVALID),
     (dict(dWg=_at(2)), INVALID), (dict(dWg=_at(7), dWu=_at(7)), INVALID), (dict(ws=_at(6)), INVALID),
     (dict(ws=_at(4)), INVALID), (dict(ws_bytes=4 * 4 * 16 - 1), UNSUPPORTED),
     (dict(ws=_at(6) - 4096, ws_bytes=4097), INVALID), (dict(F=9, ws_bytes=4 * 4 * 16 - 1), UNSUPPORTED),
@@ -86,7 +88,7 @@ def _nt(handle=H, M=2, N=64, K=128, A=_at(0), lda=128, codes=_at(1), scales=_at(
     (dict(group=512), UNSUPPORTED), (dict(K=96, group=64), UNSUPPORTED), (dict(lda=120), UNSUPPORTED),
     (dict(lda=132), UNSUPPORTED), (dict(ldc=63), UNSUPPORTED), (dict(A=_at(0) + 2), UNSUPPORTED),
     (dict(codes=_at(1) + 8), UNSUPPORTED), (dict(scales=_at(2) + 1), UNSUPPORTED), (dict(C=_at(3) + 1), UNSUPPORTED),
-    (dict(C=_at(3) + 2, out=1), UNSUPPORTED), (dict(N=2 ** 31 - 1, ldc=2 ** 31), TOO_LARGE),
+    (dict(C=_at(3) + 2, out=1), UNSUPPORTED), (dict(N=2 ** 31 - 1, ldc=2 ** 31), TOO_LARGE), (dict(lda=2 ** 40), TOO_LARGE), (dict(ldc=2 ** 62), TOO_LARGE),
     (dict(C=_at(0)), INVALID), (dict(C=_at(1) + 64 * 64 - 2), INVALID), (dict(C=_at(2)), INVALID),
 ])
 def test_w4_nt(change, code):
