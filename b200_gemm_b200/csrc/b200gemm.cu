@@ -18,6 +18,7 @@
 #include "gemm_sm100.cuh"
 #include "gemm_smallm1_sm100.cuh"
 #include "schedule.cuh"
+#include "w4_mma_sm100.cuh"
 #include "w4_sm100.cuh"
 
 namespace b200gemm {

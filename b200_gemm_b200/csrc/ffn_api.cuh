@@ -74,7 +74,9 @@ bool prepare_gated_decode_kernels() {
 // Instances of the 4-bit product: 16-row tiles of W per warp (MT) that its
 // registers and ring allow next to NT tiles of X's rows.
 template <int NT>
-constexpr int kW4MaxMT = NT == 1 ? 7 : (NT == 2 ? 5 : 3);
+constexpr int kW4MaxMT = NT == 1 ? 7 : 5;
+// Rows of X up to which a 4-bit product runs on mma.sync.
+constexpr int kW4MaxSyncRows = 16;
 
 template <bool GATED, bool G32, int NT, int MT = kW4MaxMT<NT>>
 bool prepare_w4_instances() {
@@ -88,12 +90,19 @@ bool prepare_w4_instances() {
 
 template <bool GATED, bool G32>
 bool prepare_w4_nt() {
-  return prepare_w4_instances<GATED, G32, 1>() && prepare_w4_instances<GATED, G32, 2>() &&
-         prepare_w4_instances<GATED, G32, 4>();
+  return prepare_w4_instances<GATED, G32, 1>() && prepare_w4_instances<GATED, G32, 2>();
+}
+
+template <bool GATED, int H>
+bool prepare_w4_mma() {
+  return opt_in_smem(w4_mma_sm100<W4MmaCfg<GATED, H, 1>>, W4MmaCfg<GATED, H, 1>::kSmemBytes) &&
+         opt_in_smem(w4_mma_sm100<W4MmaCfg<GATED, H, 2>>, W4MmaCfg<GATED, H, 2>::kSmemBytes) &&
+         opt_in_smem(w4_mma_sm100<W4MmaCfg<GATED, H, 4>>, W4MmaCfg<GATED, H, 4>::kSmemBytes);
 }
 
 bool prepare_w4_kernels() {
-  return prepare_w4_nt<false, false>() && prepare_w4_nt<false, true>() && prepare_w4_nt<true, false>() &&
+  return prepare_w4_mma<false, 1>() && prepare_w4_mma<false, 2>() && prepare_w4_mma<true, 2>() &&
+         prepare_w4_nt<false, false>() && prepare_w4_nt<false, true>() && prepare_w4_nt<true, false>() &&
          prepare_w4_nt<true, true>();
 }
 
@@ -418,30 +427,76 @@ cudaError_t launch_w4(const W4Launch& l, const W4NtParams& p) {
   }
 }
 
+// The same for the tcgen05 kernel, whose CTA holds 128 rows of W or 256 (128
+// of Wg and of Wu); plan.mt = 128-row blocks.  A stage of 256 k's takes some
+// 1200 cycles with one block and 2100 with two, however few of their rows are
+// there (the MMAs' time; DRAM's share of 256 rows is 1400), and a CTA some 6000
+// besides, 700 more in a cluster.
+W4Plan w4_mma_plan(const b200gemm_handle* h, int N, int token_blocks, int num_stages, bool gated) {
+  W4Plan best;
+  double best_cost = 1e300;
+  for (int i = 0, split = 1; i < 4 && split <= num_stages; ++i, split *= 2) {
+    const int fit = h->w4_clusters[i] / token_blocks > 0 ? h->w4_clusters[i] / token_blocks : 1;
+    const long long max_rows = gated ? 128 : 256;
+    const long long waves = (N + max_rows * fit - 1) / (max_rows * fit);
+    const int rows = static_cast<int>((N + waves * fit - 1) / (waves * fit));
+    const int blocks = gated || rows > 128 ? 2 : 1;
+    const int stages = (num_stages + split - 1) / split;
+    const double cost = static_cast<double>(waves) * (stages * (blocks == 2 ? 2100.0 : 1200.0) + (split > 1 ? 6700.0 : 6000.0));
+    if (cost < best_cost) {
+      best_cost = cost;
+      best.rows = rows;
+      best.mt = blocks;
+      best.split = split;
+    }
+  }
+  return best;
+}
+
+template <bool GATED, int H>
+cudaError_t launch_w4_mma(const W4Launch& l, const W4NtParams& p) {
+  const auto go = [&](auto kernel, int threads, int smem) {
+    return launch_rows(kernel, threads, smem, l.plan.split, l.blocks, l.token_blocks, l.stream, l.w0, l.w1, l.x, p);
+  };
+  using C1 = W4MmaCfg<GATED, H, 1>;
+  using C2 = W4MmaCfg<GATED, H, 2>;
+  using C4 = W4MmaCfg<GATED, H, 4>;
+  if (p.group_shift == 5) return go(w4_mma_sm100<C4>, C4::kThreads, C4::kSmemBytes);
+  if (p.group_shift == 6) return go(w4_mma_sm100<C2>, C2::kThreads, C2::kSmemBytes);
+  return go(w4_mma_sm100<C1>, C1::kThreads, C1::kSmemBytes);
+}
+
 template <bool GATED>
 int run_w4(b200gemm_t h, const void* w0, const void* w1, const void* X, long long ldx, W4NtParams p,
            cudaStream_t stream) {
-  const int nt = p.M > 16 ? 4 : (p.M > 8 ? 2 : 1);
   const long long token_blocks = (static_cast<long long>(p.M) + 31) / 32;
   if (token_blocks > 65535) return B200GEMM_ERR_TOO_LARGE;
-  p.num_stages = static_cast<int>((static_cast<long long>(p.K) + 511) / 512);
+  // 16 rows of X and fewer: mma.sync, whose cost grows with them.
+  const bool mma = p.M > kW4MaxSyncRows;
+  const int nt = p.M > 8 ? 2 : 1;
+  const int stage_k = mma ? 256 : 512;
+  p.num_stages = static_cast<int>((static_cast<long long>(p.K) + stage_k - 1) / stage_k);
   W4Launch l;
   l.token_blocks = static_cast<int>(token_blocks);
   l.stream = stream;
-  l.plan = w4_plan(h, p.N, l.token_blocks, p.num_stages, nt == 1 ? kW4MaxMT<1> : (nt == 2 ? kW4MaxMT<2> : kW4MaxMT<4>),
-                   GATED);
+  l.plan = mma ? w4_mma_plan(h, p.N, l.token_blocks, p.num_stages, GATED)
+               : w4_plan(h, p.N, l.token_blocks, p.num_stages, nt == 1 ? kW4MaxMT<1> : kW4MaxMT<2>, GATED);
   l.blocks = (p.N + l.plan.rows - 1) / l.plan.rows;
   if (l.blocks > 65535) return B200GEMM_ERR_TOO_LARGE;
   p.rows = l.plan.rows;
   p.stages_per_cta = (p.num_stages + l.plan.split - 1) / l.plan.split;
+  // Codes: boxes of 256 k's (128 swizzled bytes a row); X: 256 k's plain, or
+  // 64 swizzled as the MMA reads them.
+  const uint32_t box_rows = mma ? 128u : static_cast<uint32_t>((GATED ? 16 : 32) * l.plan.mt);
   const auto encode_w = [&](CUtensorMap* map, const void* w) {
     return encode_2d(map, w, static_cast<uint64_t>(p.K) / 2, static_cast<uint64_t>(p.N), static_cast<uint64_t>(p.K) / 2,
-                     128, static_cast<uint32_t>((GATED ? 16 : 32) * l.plan.mt), CU_TENSOR_MAP_SWIZZLE_128B,
+                     128, box_rows, CU_TENSOR_MAP_SWIZZLE_128B,
                      CU_TENSOR_MAP_DATA_TYPE_UINT8);
   };
   if (!encode_w(&l.w0, w0) || (GATED && !encode_w(&l.w1, w1)) ||
-      !encode_2d(&l.x, X, static_cast<uint64_t>(p.K), static_cast<uint64_t>(p.M), static_cast<uint64_t>(ldx) * 2, 256,
-                 static_cast<uint32_t>(8 * nt), CU_TENSOR_MAP_SWIZZLE_NONE)) {
+      !encode_2d(&l.x, X, static_cast<uint64_t>(p.K), static_cast<uint64_t>(p.M), static_cast<uint64_t>(ldx) * 2,
+                 mma ? 64 : 256, mma ? 32u : static_cast<uint32_t>(8 * nt),
+                 mma ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE)) {
     return B200GEMM_ERR_CUDA;
   }
   if (!GATED) l.w1 = l.w0;
@@ -452,10 +507,14 @@ int run_w4(b200gemm_t h, const void* w0, const void* w1, const void* X, long lon
   }
   p.status = h->status_dev;
   cudaError_t e;
-  if (p.group_shift == 5)
-    e = nt == 1 ? launch_w4<GATED, true, 1>(l, p) : nt == 2 ? launch_w4<GATED, true, 2>(l, p) : launch_w4<GATED, true, 4>(l, p);
-  else
-    e = nt == 1 ? launch_w4<GATED, false, 1>(l, p) : nt == 2 ? launch_w4<GATED, false, 2>(l, p) : launch_w4<GATED, false, 4>(l, p);
+  if (mma) {
+    if constexpr (GATED) e = launch_w4_mma<true, 2>(l, p);
+    else e = l.plan.mt == 2 ? launch_w4_mma<false, 2>(l, p) : launch_w4_mma<false, 1>(l, p);
+  } else if (p.group_shift == 5) {
+    e = nt == 1 ? launch_w4<GATED, true, 1>(l, p) : launch_w4<GATED, true, 2>(l, p);
+  } else {
+    e = nt == 1 ? launch_w4<GATED, false, 1>(l, p) : launch_w4<GATED, false, 2>(l, p);
+  }
   return e == cudaSuccess ? B200GEMM_OK : B200GEMM_ERR_CUDA;
 }
 

@@ -3,13 +3,16 @@
 //   Y = X W^T,   H = act(X Wg^T) * (X Wu^T)
 //   W[n,k] = s[k / group, n] * (q[n,k] - 8), q in 0..15, two to a byte (even k
 //   in the low four bits), s bf16
-// X [M,K] bf16, at most 32 rows per CTA (blocks of 32 rows of X beyond that).
+// X [M,K] bf16, at most 16 rows (more: w4_mma_sm100.cuh).
 //
 // Rows of W are the M side of mma.sync m16n8k16, rows of X its N side, fp32
 // sums.  mma.sync, not tcgen05: the codes are expanded in registers, which
-// mma.sync reads directly where tcgen05 would want them written back to
-// shared memory first.  What bounds the kernel, next to HBM, is the number of
-// instructions issued per weight, so everything else is arranged around them:
+// mma.sync reads directly, and a tcgen05.mma takes the same time for 8 rows of
+// X as for 32.  Both measured at 8 rows (us, this kernel and that one): 8192^2
+// in groups of 128 13.7 and 16.7, of 32 14 and 23, 4096 x 14336 12.9 and 16.6;
+// at 9 .. 16 rows 16.3 and 17.7, 17.7 and 22.5, 15.3 and 14.4.  What bounds
+// the kernel, next to HBM, is the number of instructions issued per weight, so
+// everything else is arranged around them:
 //   * 0x4300 is 128 in bf16 with a spacing of 1: a code or-ed in gives 128 + q,
 //     seven instructions for eight weights.  The 136 too much are not
 //     subtracted from the weights but from the sum: the accumulator starts
@@ -69,10 +72,6 @@ struct W4NtCfg {
   static constexpr int kMT = MT;
   static constexpr int kNT = NT;
   static constexpr int kTok = 8 * NT;
-  // Whether the 136 too much come off the sum (see above) or, with 17 to 32
-  // rows of X, off the weights: there the registers and the products that the
-  // sum's start takes outweigh eight subtractions per row tile.
-  static constexpr bool kFromSum = NT < 4;
   static constexpr int kHalf = 16 * MT;                // weight rows of one half of the warps
   static constexpr int kWarps = 16;
   static constexpr int kThreads = 32 * kWarps;
@@ -158,7 +157,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
   wd.status = p.status;
   wd.timeout_ns = p.timeout_ns;
 
-  const uint64_t policy_w = ptx::policy_evict_first();  // read once (per 32 rows of X)
+  const uint64_t policy_w = ptx::policy_evict_first();  // read once
   const uint64_t policy_x = ptx::policy_evict_last();   // read by every CTA
   auto load_w = [&](int it, int s) {
     const uint32_t bar = full0 + 8 * s, dst = ring + s * Cfg::kStageBytes;
@@ -290,61 +289,34 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
           acc[i][j][3] = fmaf(s1, sum[j][3], acc[i][j][3]);
         }
       };
-      if constexpr (Cfg::kFromSum) {
-        uint32_t x[2][NT][4];
-        float start[kSets][NT][4];  // -136 sum(x)
+      uint32_t x[2][NT][4];
+      float start[kSets][NT][4];  // -136 sum(x)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        load_x(e, x[e]);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          float (&s)[4] = start[e % kSets][j];
+          if (e < kSets) s[0] = s[1] = s[2] = s[3] = 0.0f;
+          mma_m16n8k16(s, kMinus136, kMinus136, kMinus136, kMinus136, x[e][j][0], x[e][j][1]);
+          mma_m16n8k16(s, kMinus136, kMinus136, kMinus136, kMinus136, x[e][j][2], x[e][j][3]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        float sum[NT][4];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          load_x(e, x[e]);
+          uint32_t lo[4], hi[4];
+          w4_expand(ld_shared_u32((aw ^ (16u * e)) + i * 2048u), w4c, lo);
+          w4_expand(ld_shared_u32((aw ^ (16u * e)) + i * 2048u + 1024u), w4c, hi);
 #pragma unroll
           for (int j = 0; j < NT; ++j) {
-            float (&s)[4] = start[e % kSets][j];
-            if (e < kSets) s[0] = s[1] = s[2] = s[3] = 0.0f;
-            mma_m16n8k16(s, kMinus136, kMinus136, kMinus136, kMinus136, x[e][j][0], x[e][j][1]);
-            mma_m16n8k16(s, kMinus136, kMinus136, kMinus136, kMinus136, x[e][j][2], x[e][j][3]);
+            if (e < kSets) mma_m16n8k16_onto(sum[j], start[e][j], lo[0], hi[0], lo[1], hi[1], x[e][j][0], x[e][j][1]);
+            else mma_m16n8k16(sum[j], lo[0], hi[0], lo[1], hi[1], x[e][j][0], x[e][j][1]);
+            mma_m16n8k16(sum[j], lo[2], hi[2], lo[3], hi[3], x[e][j][2], x[e][j][3]);
           }
-        }
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          float sum[NT][4];
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            uint32_t lo[4], hi[4];
-            w4_expand(ld_shared_u32((aw ^ (16u * e)) + i * 2048u), w4c, lo);
-            w4_expand(ld_shared_u32((aw ^ (16u * e)) + i * 2048u + 1024u), w4c, hi);
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-              if (e < kSets) mma_m16n8k16_onto(sum[j], start[e][j], lo[0], hi[0], lo[1], hi[1], x[e][j][0], x[e][j][1]);
-              else mma_m16n8k16(sum[j], lo[0], hi[0], lo[1], hi[1], x[e][j][0], x[e][j][1]);
-              mma_m16n8k16(sum[j], lo[2], hi[2], lo[3], hi[3], x[e][j][2], x[e][j][3]);
-            }
-            if (e == 1 || Cfg::kG32) add_scaled(i, e % kSets, sum);
-          }
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          uint32_t x[NT][4];
-          load_x(e, x);
-#pragma unroll
-          for (int i = 0; i < MT; ++i) {
-            uint32_t lo[4], hi[4];
-            w4_expand(ld_shared_u32((aw ^ (16u * e)) + i * 2048u), w4c, lo);
-            w4_expand(ld_shared_u32((aw ^ (16u * e)) + i * 2048u + 1024u), w4c, hi);
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              lo[q] = w4_less_136(lo[q]);
-              hi[q] = w4_less_136(hi[q]);
-            }
-            const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            float sum[NT][4];
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-              mma_m16n8k16_onto(sum[j], zero, lo[0], hi[0], lo[1], hi[1], x[j][0], x[j][1]);
-              mma_m16n8k16(sum[j], lo[2], hi[2], lo[3], hi[3], x[j][2], x[j][3]);
-            }
-            add_scaled(i, e % kSets, sum);
-          }
+          if (e == 1 || Cfg::kG32) add_scaled(i, e % kSets, sum);
         }
       }
     }

@@ -20,7 +20,9 @@ def _w4_product(x, codes, scales):
     with at most 8 steps of 16 products (4 for the start): each rounds or
     truncates a value of at most (136 + 143) sum|x|, so a scaled sum is off by
     at most 8 * 2^-22 * 279 s sum|x|.  Then one fp32 multiply-add per such sum
-    (at least 32 k's), a few more over the warps and the cluster."""
+    (at least 32 k's), a few more over the warps and the cluster.  With more
+    than 16 rows of X it sums (q - 8) x itself, in the same steps: within the
+    same bound."""
     w = plain.w4_values(codes, scales)
     x = x.double()
     s = scales.double().t().repeat_interleave(x.shape[1] // scales.shape[0], dim=1)
@@ -232,3 +234,60 @@ def test_refusals(gpu_handle):
     assert err.value.code == _lib.ERR_INVALID_ARG
     assert h.w4_nt(e(0, 128), codes, scales).shape == (0, 64)
     assert h.w4_dequantize(e(0, 64, t=torch.uint8), e(4, 0)).shape == (0, 128)
+
+
+@pytest.mark.parametrize("group", [32, 64, 256])
+@pytest.mark.parametrize("M,N,K", [(17, 1, 256), (32, 129, 768), (25, 8192, 1024), (40, 30000, 512), (33, 400, 8448),
+                                   (300, 130, 256)])
+def test_nt_more_rows(gpu_handle, M, N, K, group):
+    """17 rows and more: blocks of 128 rows of weights that end anywhere, one
+    and two of them per CTA, K split over clusters, several blocks of rows of X."""
+    _check_nt(gpu_handle, M, N, K, group, seed=N, pad=8)
+
+
+@pytest.mark.parametrize("M,F,K,group", [(17, 1, 32, 32), (32, 130, 4096, 64), (31, 14000, 256, 128), (50, 300, 8192, 32)])
+def test_gated_more_rows(gpu_handle, M, F, K, group):
+    x = plain.rows(M, K, 1)
+    gate, up = plain.w4_random(F, K, group, 2), plain.w4_random(F, K, group, 3)
+    out = gpu_handle.w4_gated(x, *gate, *up, activation="gelu")
+    assert gpu_handle.last_device_status()[0] == 0
+    plain.close(out, *plain.gated(*_w4_product(x, *gate), *_w4_product(x, *up), "gelu"))
+
+
+def test_more_rows_bad_values(gpu_handle):
+    """The same as with a few rows: a bad row of X or group of W reaches its own results only."""
+    x = plain.rows(40, 256, 1)
+    codes, scales = plain.w4_random(300, 256, 64, 2)
+    ref = gpu_handle.w4_nt(x, codes, scales)
+    y = x.clone()
+    y[2, 9] = float("nan")
+    y[35, 0] = float("inf")
+    got = gpu_handle.w4_nt(y, codes, scales)
+    keep = [i for i in range(40) if i not in (2, 35)]
+    assert torch.equal(got[keep], ref[keep]) and got[2].isnan().all() and not got[35].isfinite().any()
+    bad = scales.clone()
+    bad[3, 7], bad[0, 299], bad[1, 140] = float("nan"), float("inf"), float("-inf")
+    got = gpu_handle.w4_nt(x, codes, bad)
+    keep = [n for n in range(300) if n not in (7, 299, 140)]
+    assert torch.equal(got[:, keep], ref[:, keep]) and got[:, [7, 299, 140]].isnan().all()
+
+
+@pytest.mark.parametrize("M", [3, 20])
+def test_scales_of_any_size(gpu_handle, M):
+    """Scales and activations that are powers of two shift the results by their
+    exponents and nothing else: 2^120 * 2^-110 as 1 * 1, and 2^-100 * 2^90."""
+    x = plain.rows(M, 512, 1)
+    codes, scales = plain.w4_random(70, 512, 128, 2)
+    ref = gpu_handle.w4_nt(x, codes, scales)
+    for s, v in ((110, -100), (-100, 90)):
+        got = gpu_handle.w4_nt(x * 2.0 ** v, codes, scales * 2.0 ** s)
+        assert torch.equal(got.float() * 2.0 ** -(s + v), ref.float())
+
+
+def test_more_rows_repeat_exactly(gpu_handle):
+    """No atomics: the same call gives the same bits."""
+    x = plain.rows(70, 8192, 1)
+    codes, scales = plain.w4_random(900, 8192, 32, 2)
+    ref = gpu_handle.w4_nt(x, codes, scales, out_dtype=torch.float32)
+    for _ in range(5):
+        assert torch.equal(gpu_handle.w4_nt(x, codes, scales, out_dtype=torch.float32), ref)
