@@ -90,12 +90,10 @@ struct W4MmaCfg {
 };
 
 // Eight codes (k in order, the lowest in the lowest four bits) to four bf16
-// pairs of (q - 8) / 64, exactly.  The codes at even k masked out in place,
-// and those at odd k, 16 q; a byte permutation makes 16-bit halves 0x00bb of
-// adjacent bytes.  As bf16 such a half is b 2^-133, with or without the lowest
-// bit of the exponent, so a product with 2^127 (even k) or 2^123 (odd k) less
-// 1/8 is the result: six bit operations and four products for eight codes.
-// The epilogue's sums are 64 times too small, to be put right at their end.
+// pairs of (q - 8) / 64, as in w4_sm100.cuh but adjacent k's to a pair.  The
+// codes at even k are masked out in place, and those at odd k, 16 q; a byte
+// permutation puts adjacent bytes into 16-bit halves.  Six bit operations and
+// four multiply-adds.
 struct W4PairConst {
   uint32_t even, odd, scale, offset;
 };
@@ -112,7 +110,7 @@ __device__ __forceinline__ void w4_expand_pairs(uint32_t w, const W4PairConst& c
     // bytes: e_i, its sign (0), o_i, the sign of e_i
     uint32_t d;
     asm("prmt.b32 %0, %1, %2, %3;" : "=r"(d) : "r"(e), "r"(o), "r"(0x8480u + i * 0x1111u));
-    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(v[i]) : "r"(d), "r"(c.scale), "r"(c.offset));
+    v[i] = fma_bf16x2(d, c.scale, c.offset);
   }
 }
 

@@ -13,13 +13,13 @@
 // at 9 .. 16 rows 16.3 and 17.7, 17.7 and 22.5, 15.3 and 14.4.  What bounds
 // the kernel, next to HBM, is the number of instructions issued per weight, so
 // everything else is arranged around them:
-//   * 0x4300 is 128 in bf16 with a spacing of 1: a code or-ed in gives 128 + q,
-//     seven instructions for eight weights.  The 136 too much are not
-//     subtracted from the weights but from the sum: the accumulator starts
-//     from -136 sum(x), one product of X with a constant for all rows of W.
-//     A sum of 32 or 64 products, exact but for its fp32 additions, whose
-//     magnitude is up to 35 times that of the (q - 8) x, loses at most
-//     4 or 8 additions * 2^-22 * 279 sum|x|; no weight is rounded.
+//   * Four bits masked out in place, b = q or 16 q in a 16-bit half, are
+//     b 2^-133 as bf16 (the lowest bit of the exponent counts on like one of
+//     the mantissa), so a multiply-add by 2^127 or 2^123 and -1/8 makes them
+//     (q - 8) / 64, exactly: five bit operations and four multiply-adds for
+//     eight weights.  The last 6 bits come back with the row's finished sums.
+//     (128 + q, or-ed together, costs seven bit operations and no multiply-add
+//     but a sum that starts from -136 sum(x): 3 to 8% slower.)
 //   * The sum of a group (of half of one, ..) is multiplied by its scale in
 //     fp32 and added to the row's.
 //   * One CTA of 16 warps per SM takes a range of rows of W (gated: the same
@@ -109,30 +109,30 @@ __device__ __forceinline__ void mma_m16n8k16_onto(float (&d)[4], const float (&c
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
 
-// Eight codes of a word -> four bf16 pairs of 128 + q: pair j holds codes j and
-// j + 4.  And-or is one instruction on the logic pipe when mask and magic
-// number come from registers (W4Const: opaque to the compiler, which
-// otherwise keeps them as immediates and takes two).
+// Eight codes of a word -> four bf16 pairs of (q - 8) / 64: pair j holds codes
+// j and j + 4.  (Constants come from registers: opaque to the compiler, which
+// otherwise keeps them as immediates.)
 struct W4Const {
-  uint32_t mask, magic;
+  uint32_t mask, mask16, scale, scale16, offset;
 };
 __device__ __forceinline__ W4Const w4_const() {
   W4Const c;
-  asm volatile("mov.u32 %0, 0x000F000F;\n\tmov.u32 %1, 0x43004300;" : "=r"(c.mask), "=r"(c.magic));
+  asm volatile("mov.u32 %0, 0x000F000F;\n\tmov.u32 %1, 0x00F000F0;" : "=r"(c.mask), "=r"(c.mask16));
+  asm volatile("mov.u32 %0, 0x7F007F00;\n\tmov.u32 %1, 0x7D007D00;\n\tmov.u32 %2, 0xBE00BE00;"
+               : "=r"(c.scale), "=r"(c.scale16), "=r"(c.offset));
   return c;
 }
+__device__ __forceinline__ uint32_t fma_bf16x2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
 __device__ __forceinline__ void w4_expand(uint32_t w, const W4Const& k, uint32_t (&v)[4]) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(v[j]) : "r"(w >> (4 * j)), "r"(k.mask), "r"(k.magic));
+  v[0] = fma_bf16x2(w & k.mask, k.scale, k.offset);
+  v[1] = fma_bf16x2(w & k.mask16, k.scale16, k.offset);
+  v[2] = fma_bf16x2((w >> 8) & k.mask, k.scale, k.offset);
+  v[3] = fma_bf16x2((w >> 8) & k.mask16, k.scale16, k.offset);
 }
-// A pair of 128 + q less 136: exact.
-__device__ __forceinline__ uint32_t w4_less_136(uint32_t v) {
-  const __nv_bfloat162 offset = __halves2bfloat162(__ushort_as_bfloat16(0x4308), __ushort_as_bfloat16(0x4308));
-  const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), offset);
-  return *reinterpret_cast<const uint32_t*>(&d);
-}
-constexpr uint32_t kMinus136 = 0xC308C308u;  // a bf16 pair of -136
 
 template <class Cfg>
 __global__ void __launch_bounds__(Cfg::kThreads, 1)
@@ -290,18 +290,9 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
         }
       };
       uint32_t x[2][NT][4];
-      float start[kSets][NT][4];  // -136 sum(x)
+      const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        load_x(e, x[e]);
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          float (&s)[4] = start[e % kSets][j];
-          if (e < kSets) s[0] = s[1] = s[2] = s[3] = 0.0f;
-          mma_m16n8k16(s, kMinus136, kMinus136, kMinus136, kMinus136, x[e][j][0], x[e][j][1]);
-          mma_m16n8k16(s, kMinus136, kMinus136, kMinus136, kMinus136, x[e][j][2], x[e][j][3]);
-        }
-      }
+      for (int e = 0; e < 2; ++e) load_x(e, x[e]);
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
         float sum[NT][4];
@@ -312,7 +303,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
           w4_expand(ld_shared_u32((aw ^ (16u * e)) + i * 2048u + 1024u), w4c, hi);
 #pragma unroll
           for (int j = 0; j < NT; ++j) {
-            if (e < kSets) mma_m16n8k16_onto(sum[j], start[e][j], lo[0], hi[0], lo[1], hi[1], x[e][j][0], x[e][j][1]);
+            if (e < kSets) mma_m16n8k16_onto(sum[j], zero, lo[0], hi[0], lo[1], hi[1], x[e][j][0], x[e][j][1]);
             else mma_m16n8k16(sum[j], lo[0], hi[0], lo[1], hi[1], x[e][j][0], x[e][j][1]);
             mma_m16n8k16(sum[j], lo[2], hi[2], lo[3], hi[3], x[e][j][2], x[e][j][3]);
           }
@@ -354,7 +345,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
       for (int c = 0; c < 4; ++c) {
         // column 2t + b of the fragment is token tok(2t + b) = t + 4b
         const uint32_t tok = j * 8u + t + 4u * (c & 1), row = half * Cfg::kHalf + i * 16u + 8u * (c >> 1) + tokg;
-        sums[part * kSlab + tok * Cfg::kPitch + row] = acc[i][j][c];
+        sums[part * kSlab + tok * Cfg::kPitch + row] = 64.0f * acc[i][j][c];
       }
   __syncthreads();
   const int toks = min(Cfg::kTok, p.M - m0);
@@ -495,9 +486,10 @@ __global__ void __launch_bounds__(256) w4_quantize_kernel(const W4Params p) {
     p.scales[static_cast<long long>(q) * p.N + n0 + lane] = sc[warp][lane];
 }
 
-// W[n,k] = bf16(s (q - 8)): 128 + q (w4_expand) less 136 is exact in bf16, so
-// one bf16 multiplication per pair is the one rounding.  The same blocks; 4 bytes of
-// codes and 16 of results per lane and row.
+// W[n,k] = bf16(s (q - 8)): 0x4300 is 128 in bf16 with a spacing of 1, so a
+// code or-ed in gives 128 + q, and less 136 is exact; one bf16 multiplication
+// per pair is the one rounding.  The same blocks; 4 bytes of codes and 16 of
+// results per lane and row.
 __global__ void __launch_bounds__(256) w4_dequantize_kernel(const W4Params p) {
   __shared__ uint16_t sc[8][32];
   const int warp = static_cast<int>(threadIdx.x >> 5), lane = static_cast<int>(threadIdx.x & 31u);
@@ -516,7 +508,7 @@ __global__ void __launch_bounds__(256) w4_dequantize_kernel(const W4Params p) {
     sc[warp][lane] = __ldg(p.scales + static_cast<long long>(q) * p.N + n0 + lane);
   __syncthreads();
   if (k >= p.K) return;
-  const W4Const c = w4_const();
+  const __nv_bfloat162 offset = __halves2bfloat162(__ushort_as_bfloat16(0x4308), __ushort_as_bfloat16(0x4308));
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int n = n0 + warp + 8 * i;
@@ -524,11 +516,10 @@ __global__ void __launch_bounds__(256) w4_dequantize_kernel(const W4Params p) {
     const __nv_bfloat16 s1 = __ushort_as_bfloat16(sc[lane >> (p.group_shift - 3)][warp + 8 * i]);
     const __nv_bfloat162 s2 = __halves2bfloat162(s1, s1);
     uint32_t v[4];
-    w4_expand(w[i], c, v);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      v[j] = w4_less_136(v[j]);
-      const __nv_bfloat162 d = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&v[j]), s2);
+      v[j] = ((w[i] >> (4 * j)) & 0x000F000Fu) | 0x43004300u;
+      const __nv_bfloat162 d = __hmul2(__hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v[j]), offset), s2);
       v[j] = *reinterpret_cast<const uint32_t*>(&d);
     }
     // pairs (k_j, k_j+4) back into order

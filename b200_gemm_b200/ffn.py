@@ -205,8 +205,8 @@ class FfnOps:
 
     def w4_dequantize(self, codes, scales, out=None, stream=None):
         """The bf16 [N, K] weights that the codes stand for, bf16(s (q - 8)).
-        For long prompts: `bf16_nt` with these beats `w4_nt` from about 200
-        rows on."""
+        For long prompts: `bf16_nt` with these beats `w4_nt` from about 65
+        rows on, from about 160 where they are made for that one call."""
         torch = _torch()
         N, K, group = self._w4(codes, scales, "weights")
         ptr, where = self._where(stream)

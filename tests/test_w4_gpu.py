@@ -16,17 +16,15 @@ BF = torch.bfloat16
 def _w4_product(x, codes, scales):
     """X W^T in 64 bits and the bound of the kernel's sum.
 
-    The kernel sums (128 + q) x over 32 or 64 k's, starting from -136 sum(x),
-    with at most 8 steps of 16 products (4 for the start): each rounds or
-    truncates a value of at most (136 + 143) sum|x|, so a scaled sum is off by
-    at most 8 * 2^-22 * 279 s sum|x|.  Then one fp32 multiply-add per such sum
-    (at least 32 k's), a few more over the warps and the cluster.  With more
-    than 16 rows of X it sums (q - 8) x itself, in the same steps: within the
-    same bound."""
+    The kernels sum (q - 8) x, times a power of two, over at most 128 k's with
+    at most 8 steps of 16 products: a step adds 17 terms, each truncated to
+    2^-22 of a largest one of at most 8 sum|x|, so a scaled sum is off by at
+    most 8 * 17 * 8 * 2^-22 s sum|x|.  Then one fp32 multiply-add per such sum
+    (at least 32 k's), a few more over the warps and the cluster."""
     w = plain.w4_values(codes, scales)
     x = x.double()
     s = scales.double().t().repeat_interleave(x.shape[1] // scales.shape[0], dim=1)
-    err = 8 * 2.0 ** -22 * 279 * (x.abs() @ s.t()) + (x.shape[1] / 32 + 16) * 2.0 ** -23 * (x.abs() @ w.abs().t())
+    err = 8 * 2.0 ** -22 * 136 * (x.abs() @ s.t()) + (x.shape[1] / 32 + 16) * 2.0 ** -23 * (x.abs() @ w.abs().t())
     return x @ w.t(), err
 
 
