@@ -126,6 +126,7 @@ struct FfnCfg {
   static constexpr int kEnd = kAbort + 4;
   static constexpr int kSmemBytes = kEnd + 1024;
   static_assert(kSmemBytes <= 232448, "exceeds the 227 KB per-CTA shared memory limit");
+  static_assert(kSmemBytes > 116 * 1024, "one CTA per SM: two that want TMEM could wait for one another's");
 };
 
 // Matrix descriptor of an MN-major operand in the 128-byte swizzle: 64

@@ -77,11 +77,15 @@ struct W4MmaCfg {
   static constexpr int kTmemCols = 512;
   static_assert(kTmemUsed <= kTmemCols && kTmemUsed > 256, "TMEM columns");
   static constexpr int kBars = 256;
-  static constexpr int kRing = 4;
+  static constexpr int kRing = H == 1 ? 6 : 4;
   static constexpr int kRingAt = 0;                    // X's boxes first in a stage: 1024-byte aligned
   static constexpr int kBarsAt = kRingAt + kRing * kStageBytes;
   static constexpr int kSmemBytes = 1024 + kBarsAt + kBars;
   static_assert((2 * kRing + 2 * kBufs + 4 + 1) * 8 + 8 <= kBars, "barriers");
+  // All of an SM's TMEM for a CTA is safe as long as no other CTA that wants
+  // some fits next to it: clusters of two kernels could otherwise each hold
+  // what the other's last CTA waits for.
+  static_assert(kSmemBytes > 190 * 1024 && kSmemBytes <= 232448, "one CTA per SM");
   // The rows' sums [kTok][kPitch], in the ring once the MMAs are done.
   static constexpr int kPitch = H * 128;
   static_assert(kTok * kPitch * 4 <= kRing * kStageBytes, "sums alias the ring");
@@ -225,7 +229,6 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
     // keeps their operands in uniform registers: issued from a branch of one
     // lane, every MMA took some 60 cycles to issue, four times its work.
     const bool leader = ptx::elect_one();
-    static_assert((RING & (RING - 1)) == 0 && (BUFS & (BUFS - 1)) == 0, "powers of two");
     bool go = true;
     for (int it = static_cast<int>(warp - kMma); it < 2 * count && go; it += Cfg::kMmaWarps) {
       const int stage = (it >> 1) % RING, buf = it % BUFS, odd = it & 1;

@@ -289,3 +289,67 @@ def test_more_rows_repeat_exactly(gpu_handle):
     ref = gpu_handle.w4_nt(x, codes, scales, out_dtype=torch.float32)
     for _ in range(5):
         assert torch.equal(gpu_handle.w4_nt(x, codes, scales, out_dtype=torch.float32), ref)
+
+
+def test_more_rows_streams_graphs_and_overlap(gpu_handle):
+    """Calls at once on two streams (kernels that take a whole SM each, in
+    clusters), a captured and replayed one, and launches that overlap."""
+    h = gpu_handle
+    sets = [(plain.rows(m, k, m), plain.w4_random(n, k, 64, n)) for m, n, k in
+            ((20, 400, 8192), (32, 9000, 1024), (24, 2048, 4096), (70, 30000, 512))]
+    ref = [h.w4_nt(x, *w) for x, w in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    out = [[torch.empty_like(r) for r in ref] for _ in range(2)]
+    for _ in range(25):
+        for s, results in zip(streams, out):
+            for i in (0, 1, 2, 3) if s is streams[0] else (2, 0, 3, 1):
+                h.w4_nt(sets[i][0], *sets[i][1], out=results[i], stream=s)
+    torch.cuda.synchronize()
+    assert h.last_device_status()[0] == 0
+    for results in out:
+        assert all(torch.equal(a, b) for a, b in zip(results, ref))
+
+    x = plain.rows(24, 2048, 5)
+    gate, up, down = (plain.w4_random(2048, 2048, 32, s) for s in (1, 2, 3))
+
+    def step():
+        y = x
+        for _ in range(3):
+            y = h.w4_nt(h.w4_gated(y, *gate, *up, activation="gelu"), *down).mul_(2.0 ** -12)
+        return y
+
+    def chain():
+        y = x
+        for _ in range(4):
+            y = h.w4_nt(y, *down)
+        return y
+
+    want, cwant = step(), chain()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for _ in range(3):
+        got.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+    del graph
+    for mode in (_lib.PDL_ON, _lib.PDL_WEIGHTS_EARLY):
+        h.set_pdl(mode)
+        try:
+            for _ in range(10):
+                assert torch.equal(chain(), cwant)
+        finally:
+            h.set_pdl(_lib.PDL_OFF)
+
+
+@pytest.mark.parametrize("M", [16, 20])
+def test_nt_far_rows(gpu_handle, M):
+    """A result whose last rows lie past 2^31 elements."""
+    x, w = plain.rows(M, 128, 0), plain.w4_random(40, 128, 32, 1)
+    pitch = 2 ** 31 // (M - 2)
+    buf = torch.empty((M - 1) * pitch + 40, dtype=BF, device="cuda")
+    out = torch.as_strided(buf, (M, 40), (pitch, 1))
+    gpu_handle.w4_nt(x, *w, out=out)
+    assert torch.equal(out, gpu_handle.w4_nt(x, *w))
