@@ -384,6 +384,7 @@ int run_gated_decode(b200gemm_t h, const void* Wg, const void* Wu, long long ldw
 // (a second wave only where a CTA's registers and ring cannot hold its share).
 struct W4Plan {
   int rows = 0, mt = 0, split = 1;
+  long long waves = 1;
 };
 W4Plan w4_plan(const b200gemm_handle* h, int N, int token_blocks, int num_stages, int max_mt, bool gated) {
   const int tiles = gated ? 1 : 2;  // 16-row tiles of output per unit of mt
@@ -403,6 +404,7 @@ W4Plan w4_plan(const b200gemm_handle* h, int N, int token_blocks, int num_stages
       best.rows = rows;
       best.mt = mt;
       best.split = split;
+      best.waves = waves;
     }
   }
   return best;
@@ -448,6 +450,7 @@ W4Plan w4_mma_plan(const b200gemm_handle* h, int N, int token_blocks, int num_st
       best.rows = rows;
       best.mt = blocks;
       best.split = split;
+      best.waves = waves;
     }
   }
   return best;
@@ -471,16 +474,28 @@ int run_w4(b200gemm_t h, const void* w0, const void* w1, const void* X, long lon
            cudaStream_t stream) {
   const long long token_blocks = (static_cast<long long>(p.M) + 31) / 32;
   if (token_blocks > 65535) return B200GEMM_ERR_TOO_LARGE;
-  // 16 rows of X and fewer: mma.sync, whose cost grows with them.
-  const bool mma = p.M > kW4MaxSyncRows;
-  const int nt = p.M > 8 ? 2 : 1;
-  const int stage_k = mma ? 256 : 512;
-  p.num_stages = static_cast<int>((static_cast<long long>(p.K) + stage_k - 1) / stage_k);
+  const auto stages = [&](int k) { return static_cast<int>((static_cast<long long>(p.K) + k - 1) / k); };
   W4Launch l;
   l.token_blocks = static_cast<int>(token_blocks);
   l.stream = stream;
-  l.plan = mma ? w4_mma_plan(h, p.N, l.token_blocks, p.num_stages, GATED)
-               : w4_plan(h, p.N, l.token_blocks, p.num_stages, nt == 1 ? kW4MaxMT<1> : kW4MaxMT<2>, GATED);
+  // 16 rows of X and fewer: mma.sync, whose cost grows with them.  From 9 rows
+  // on its registers hold 160 rows of W (gated: 80 of each) instead of 224:
+  // where that means a second wave of CTAs and tcgen05 needs but one, that one,
+  // except in groups of 32, whose sums it has to fetch four times per 128 k's.
+  // (16 rows, mma.sync and tcgen05, us: gated 14336 x 4096 30.5 and 24.0, in
+  // groups of 32 30.9 and 35.8; 28672 x 8192 46.5 and 44.5; two waves of both,
+  // gated 20000 x 2048, 23.0 and 35.6.)
+  const int nt = p.M > 8 ? 2 : 1;
+  W4Plan sync_plan, mma_plan;
+  if (p.M <= kW4MaxSyncRows)
+    sync_plan = w4_plan(h, p.N, l.token_blocks, stages(512), nt == 1 ? kW4MaxMT<1> : kW4MaxMT<2>, GATED);
+  bool mma = p.M > kW4MaxSyncRows || (nt == 2 && sync_plan.waves > 1 && p.group_shift > 5);
+  if (mma) {
+    mma_plan = w4_mma_plan(h, p.N, l.token_blocks, stages(256), GATED);
+    mma = p.M > kW4MaxSyncRows || mma_plan.waves == 1;
+  }
+  l.plan = mma ? mma_plan : sync_plan;
+  p.num_stages = stages(mma ? 256 : 512);
   l.blocks = (p.N + l.plan.rows - 1) / l.plan.rows;
   if (l.blocks > 65535) return B200GEMM_ERR_TOO_LARGE;
   p.rows = l.plan.rows;

@@ -1,5 +1,6 @@
 // Products with 4-bit weights (see w4_sm100.cuh for the format) for more than
-// 16 rows of activations, on the 5th-generation tensor cores:
+// 16 rows of activations (run_w4 says when for fewer), on the 5th-generation
+// tensor cores:
 //   Y = X W^T,   H = act(X Wg^T) * (X Wu^T)
 // at most 32 rows of X per CTA (blocks of 32 rows of X beyond that).
 //

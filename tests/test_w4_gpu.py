@@ -353,3 +353,14 @@ def test_nt_far_rows(gpu_handle, M):
     out = torch.as_strided(buf, (M, 40), (pitch, 1))
     gpu_handle.w4_nt(x, *w, out=out)
     assert torch.equal(out, gpu_handle.w4_nt(x, *w))
+
+
+@pytest.mark.parametrize("M,F,K,group", [(9, 13000, 256, 64), (16, 14336, 384, 128), (12, 12500, 512, 32),
+                                         (16, 20000, 256, 256)])
+def test_gated_many_rows_of_weights(gpu_handle, M, F, K, group):
+    """More rows of weights than the kernel for a few rows holds at once."""
+    x = plain.rows(M, K, 1)
+    gate, up = plain.w4_random(F, K, group, 2), plain.w4_random(F, K, group, 3)
+    out = gpu_handle.w4_gated(x, *gate, *up, activation="silu")
+    assert gpu_handle.last_device_status()[0] == 0
+    plain.close(out, *plain.gated(*_w4_product(x, *gate), *_w4_product(x, *up), "silu"))
