@@ -483,7 +483,7 @@ int run_w4(b200gemm_t h, const void* w0, const void* w1, const void* X, long lon
   // where that means a second wave of CTAs and tcgen05 needs but one, that one,
   // except in groups of 32, whose sums it has to fetch four times per 128 k's.
   // (16 rows, mma.sync and tcgen05, us: gated 14336 x 4096 30.5 and 24.0, in
-  // groups of 32 30.9 and 35.8; 28672 x 8192 46.5 and 44.5; two waves of both,
+  // groups of 32 30.9 and 31.8; 28672 x 8192 46.5 and 43.5; two waves of both,
   // gated 20000 x 2048, 23.0 and 35.6.)
   const int nt = p.M > 8 ? 2 : 1;
   W4Plan sync_plan, mma_plan;

@@ -22,8 +22,8 @@
 // weights at 2.3 TB/s; 8192 x 8192: 18 us (25); gated 14336 x 4096: 24 us (53).
 //
 // Warps: 0 .. 4H-1   epilogue: block w / 4 of 128 rows, TMEM lanes 32 (w % 4) ..
-//        16 more     expansion, two groups of eight for the steps in turn: TMEM
-//                    lanes 32 (w % 4) .., one half of a step's k's
+//        16 or 8     expansion, two groups of eight for the steps in turn, or
+//                    one: TMEM lanes 32 (w % 4) .., one half of a step's k's
 //        2 or 3      TMA producer; MMA issue, the first also TMEM allocation
 // H = 2 blocks of rows per CTA: Wg's and Wu's, or 256 rows of W; H = 1: 128
 // rows of W.  Rows are divided evenly over the SMs and K over the CTAs of a
@@ -54,14 +54,18 @@ struct W4MmaCfg {
   static constexpr int kStageK = 256;                  // k's of a stage of the ring
   static constexpr int kStepK = 128;                   // k's expanded and multiplied at a time: half a stage
   static constexpr int kEpiWarps = 4 * H;
-  static constexpr int kExpWarps = 8;                  // of each of two groups, for steps in turn
+  // Two groups of expansion warps take the steps in turn.  In groups of 32 the
+  // epilogue is what lasts, and one group leaves it the registers to fetch its
+  // next sums ahead (gated 14331 x 4096, 32 rows: 35.7 -> 31.8 us).
+  static constexpr int kExpGroups = SG == 4 ? 1 : 2;
+  static constexpr int kExpWarps = 8;                  // of each group
   // Warps that issue MMAs.  One block's eight MMAs of a step take less than a
   // warp's waits and commits around them, and groups of 32 wait twice: there
   // two warps take the steps in turn (14336 x 4096 turned, 32 rows: 17.2 -> 15.8
   // us).  With two blocks one warp is better, as the earlier step's MMAs all
   // come first (28416 x 4096: 27.2 -> 25.8 us).
   static constexpr int kMmaWarps = H == 1 || SG == 4 ? 2 : 1;
-  static constexpr int kThreads = 32 * (kEpiWarps + 2 * kExpWarps + 1 + kMmaWarps);
+  static constexpr int kThreads = 32 * (kEpiWarps + kExpGroups * kExpWarps + 1 + kMmaWarps);
   static constexpr int kCodes = 128 * 128;             // one block's codes of a stage: 128 bytes a row
   static constexpr int kStageX = 4 * kTok * 128;       // four boxes of 64 k's
   static constexpr int kStageBytes = H * kCodes + kStageX;
@@ -133,7 +137,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
   const uint32_t drain = tempty0 + 16, tmem_slot = drain + 8;
   // (the shuffle tells the compiler that a warp has one value)
   const uint32_t warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31u;
-  constexpr uint32_t kProducer = Cfg::kEpiWarps + 2 * Cfg::kExpWarps, kMma = kProducer + 1;
+  constexpr uint32_t kProducer = Cfg::kEpiWarps + Cfg::kExpGroups * Cfg::kExpWarps, kMma = kProducer + 1;
   const int split = static_cast<int>(gridDim.x);   // CTAs of this cluster: K ranges
   const int rank = static_cast<int>(blockIdx.x);
   const int n0 = static_cast<int>(blockIdx.y) * p.rows;
@@ -152,7 +156,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
     asm volatile("st.shared.u32 [%0], 0;" ::"r"(wd.abort_flag) : "memory");
     for (int s = 0; s < RING; ++s) {
       ptx::mbar_init(full0 + 8 * s, 1);
-      ptx::mbar_init(empty0 + 8 * s, 2 * Cfg::kExpWarps + 2);  // the codes are expanded, the MMAs have read X
+      ptx::mbar_init(empty0 + 8 * s, Cfg::kExpGroups * Cfg::kExpWarps + 2);  // the codes are expanded, the MMAs have read X
     }
     for (int b = 0; b < BUFS; ++b) {
       ptx::mbar_init(afull0 + 8 * b, Cfg::kExpWarps);
@@ -282,9 +286,9 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
     __syncwarp();
   } else if (warp >= Cfg::kEpiWarps) {
     // ----------------------------------------------------------- expansion
-    // Each group of warps takes one half of every stage.  A lane's row of codes
-    // is eight 16-byte chunks, stored by the TMA at chunk c ^ (row % 8): eight
-    // rows' chunks are then in different banks.
+    // Of two groups of warps each takes one half of every stage.  A lane's row
+    // of codes is eight 16-byte chunks, stored by the TMA at chunk c ^ (row % 8):
+    // eight rows' chunks are then in different banks.
     const uint32_t quarter = warp & 3u, half = ((warp - Cfg::kEpiWarps) >> 2) & 1u;
     const uint32_t group = (warp - Cfg::kEpiWarps) / Cfg::kExpWarps;
     const uint32_t row = quarter * 32u + lane;
@@ -292,16 +296,15 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
     // Rows of each block that this CTA needs: whole quarters are left out.
     const int rows0 = Cfg::kGatedOut ? cols : min(cols, 128), rows1 = Cfg::kGatedOut ? cols : max(cols - 128, 0);
     const bool need[2] = {static_cast<int>(quarter * 32u) < rows0, H == 2 && static_cast<int>(quarter * 32u) < rows1};
-    const uint32_t chunk0 = row * 128u + (((4u * group + 2u * half) ^ (row & 7u)) << 4);
-    int stage = 0, buf = static_cast<int>(group);
-    uint32_t phase = 0, bphase = 0;
-    static_assert(BUFS % 2 == 0, "a group's buffers");
-    for (int it = 0; it < count; ++it) {
+    const uint32_t chunk0 = row * 128u + (((2u * half) ^ (row & 7u)) << 4);
+    for (int it = static_cast<int>(group); it < 2 * count; it += Cfg::kExpGroups) {
+      const int stage = (it >> 1) % RING, buf = it % BUFS;
+      const uint32_t phase = static_cast<uint32_t>((it >> 1) / RING) & 1u, bphase = static_cast<uint32_t>(it / BUFS) & 1u;
       const bool got = ptx::mbar_wait_cta(full0 + 8 * stage, phase, wd, kSiteEpilogue, blockIdx.y) &&
                        ptx::mbar_wait_cta(aempty0 + 8 * buf, bphase ^ 1u, wd, kSiteEpilogue, blockIdx.y);
       if (!__all_sync(0xFFFFFFFFu, got)) break;
       ptx::tc_fence_after();
-      const uint32_t codes = base + Cfg::kRingAt + stage * Cfg::kStageBytes + Cfg::kStageX + chunk0;
+      const uint32_t codes = base + Cfg::kRingAt + stage * Cfg::kStageBytes + Cfg::kStageX + (chunk0 ^ ((it & 1u) << 6));
 #pragma unroll
       for (int h = 0; h < H; ++h) {
         if (!need[h]) continue;
@@ -317,15 +320,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
       __syncwarp();
       if (lane == 0) {
         ptx::mbar_arrive_cta(afull0 + 8 * buf);
-        ptx::mbar_arrive_cta(empty0 + 8 * stage);
-      }
-      if (++stage == RING) {
-        stage = 0;
-        phase ^= 1u;
-      }
-      if ((buf += 2) >= BUFS) {
-        buf -= BUFS;
-        bphase ^= 1u;
+        if (Cfg::kExpGroups == 2 || (it & 1)) ptx::mbar_arrive_cta(empty0 + 8 * stage);
       }
     }
     __syncwarp();
@@ -373,25 +368,28 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
       const bool got = ptx::mbar_wait_cta(tfull0 + 8 * set, sphase, wd, kSiteEpilogue, blockIdx.y);
       if (!__all_sync(0xFFFFFFFFu, got)) return false;
       ptx::tc_fence_after();
+      // Chunks of 16 columns; with a register set to spare the next one is on
+      // its way while this one is added.
+      constexpr int CHUNKS = Cfg::kSetGroups * TOK / 16, AHEAD = SG == 4 ? 2 : 1;
+      uint32_t v[AHEAD][16];
+      ptx::tmem_ld_32x32b_x16(t_row + set * Cfg::kTmemSet, v[0]);
 #pragma unroll
-      for (int i = 0; i < Cfg::kSetGroups; ++i) {
+      for (int c = 0; c < CHUNKS; ++c) {
+        ptx::tmem_wait_ld();
+        ptx::reg_fence16(v[c % AHEAD]);
+        if (AHEAD == 2 && c + 1 < CHUNKS) ptx::tmem_ld_32x32b_x16(t_row + set * Cfg::kTmemSet + 16 * (c + 1), v[(c + 1) % AHEAD]);
+        if (c + 1 == CHUNKS) {
+          ptx::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive_cta(tempty0 + 8 * set);
+        }
         // An infinite scale counts as NaN, which is what it makes of a code of 8.
-        const uint32_t bits = sc[j * Cfg::kSetGroups + i];
+        const uint32_t bits = sc[j * Cfg::kSetGroups + c * 16 / TOK];
         const float s = __uint_as_float(((bits & 0x7FFFu) == 0x7F80u ? 0x7FC0u : bits) << 16);
 #pragma unroll
-        for (int t0 = 0; t0 < TOK; t0 += 16) {
-          uint32_t v[16];
-          ptx::tmem_ld_32x32b_x16(t_row + set * Cfg::kTmemSet + i * TOK + t0, v);
-          ptx::tmem_wait_ld();
-          ptx::reg_fence16(v);
-          if (i == Cfg::kSetGroups - 1 && t0 + 16 == TOK) {
-            ptx::tc_fence_before();
-            __syncwarp();
-            if (lane == 0) ptx::mbar_arrive_cta(tempty0 + 8 * set);
-          }
-#pragma unroll
-          for (int t = 0; t < 16; ++t) acc[t0 + t] = fmaf(s, __uint_as_float(v[t]), acc[t0 + t]);
-        }
+        for (int t = 0; t < 16; ++t)
+          acc[c * 16 % TOK + t] = fmaf(s, __uint_as_float(v[c % AHEAD][t]), acc[c * 16 % TOK + t]);
+        if (AHEAD == 1 && c + 1 < CHUNKS) ptx::tmem_ld_32x32b_x16(t_row + set * Cfg::kTmemSet + 16 * (c + 1), v[0]);
       }
       if (j == Cfg::kSetsPerStep - 1) load_scales(it + 2, sc);
       return true;
