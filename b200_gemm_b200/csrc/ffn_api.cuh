@@ -93,15 +93,18 @@ bool prepare_w4_nt() {
   return prepare_w4_instances<GATED, G32, 1>() && prepare_w4_instances<GATED, G32, 2>();
 }
 
-template <bool GATED, int H>
+template <bool GATED, int H, int TOK>
 bool prepare_w4_mma() {
-  return opt_in_smem(w4_mma_sm100<W4MmaCfg<GATED, H, 1>>, W4MmaCfg<GATED, H, 1>::kSmemBytes) &&
-         opt_in_smem(w4_mma_sm100<W4MmaCfg<GATED, H, 2>>, W4MmaCfg<GATED, H, 2>::kSmemBytes) &&
-         opt_in_smem(w4_mma_sm100<W4MmaCfg<GATED, H, 4>>, W4MmaCfg<GATED, H, 4>::kSmemBytes);
+  using C1 = W4MmaCfg<GATED, H, 1, TOK>;
+  using C2 = W4MmaCfg<GATED, H, 2, TOK>;
+  using C4 = W4MmaCfg<GATED, H, 4, TOK>;
+  return opt_in_smem(w4_mma_sm100<C1>, C1::kSmemBytes) && opt_in_smem(w4_mma_sm100<C2>, C2::kSmemBytes) &&
+         opt_in_smem(w4_mma_sm100<C4>, C4::kSmemBytes);
 }
 
 bool prepare_w4_kernels() {
-  return prepare_w4_mma<false, 1>() && prepare_w4_mma<false, 2>() && prepare_w4_mma<true, 2>() &&
+  return prepare_w4_mma<false, 1, 32>() && prepare_w4_mma<false, 2, 32>() && prepare_w4_mma<true, 2, 32>() &&
+         prepare_w4_mma<false, 1, 64>() && prepare_w4_mma<false, 2, 64>() && prepare_w4_mma<true, 2, 64>() &&
          prepare_w4_nt<false, false>() && prepare_w4_nt<false, true>() && prepare_w4_nt<true, false>() &&
          prepare_w4_nt<true, true>();
 }
@@ -412,7 +415,7 @@ W4Plan w4_plan(const b200gemm_handle* h, int N, int token_blocks, int num_stages
 
 struct W4Launch {
   W4Plan plan;
-  int blocks, token_blocks;
+  int blocks, token_blocks, tok;  // blocks of W, and of `tok` rows of X
   cudaStream_t stream;
   CUtensorMap w0, w1, x;
 };
@@ -456,26 +459,39 @@ W4Plan w4_mma_plan(const b200gemm_handle* h, int N, int token_blocks, int num_st
   return best;
 }
 
-template <bool GATED, int H>
-cudaError_t launch_w4_mma(const W4Launch& l, const W4NtParams& p) {
+template <bool GATED, int H, int TOK>
+cudaError_t launch_w4_mma_block(const W4Launch& l, const W4NtParams& p) {
   const auto go = [&](auto kernel, int threads, int smem) {
     return launch_rows(kernel, threads, smem, l.plan.split, l.blocks, l.token_blocks, l.stream, l.w0, l.w1, l.x, p);
   };
-  using C1 = W4MmaCfg<GATED, H, 1>;
-  using C2 = W4MmaCfg<GATED, H, 2>;
-  using C4 = W4MmaCfg<GATED, H, 4>;
+  using C1 = W4MmaCfg<GATED, H, 1, TOK>;
+  using C2 = W4MmaCfg<GATED, H, 2, TOK>;
+  using C4 = W4MmaCfg<GATED, H, 4, TOK>;
   if (p.group_shift == 5) return go(w4_mma_sm100<C4>, C4::kThreads, C4::kSmemBytes);
   if (p.group_shift == 6) return go(w4_mma_sm100<C2>, C2::kThreads, C2::kSmemBytes);
   return go(w4_mma_sm100<C1>, C1::kThreads, C1::kSmemBytes);
 }
 
 template <bool GATED>
+cudaError_t launch_w4_mma(const W4Launch& l, const W4NtParams& p) {
+  if (l.tok == 64) {
+    if constexpr (!GATED)
+      if (l.plan.mt == 1) return launch_w4_mma_block<false, 1, 64>(l, p);
+    return launch_w4_mma_block<GATED, 2, 64>(l, p);
+  }
+  if constexpr (!GATED)
+    if (l.plan.mt == 1) return launch_w4_mma_block<false, 1, 32>(l, p);
+  return launch_w4_mma_block<GATED, 2, 32>(l, p);
+}
+
+template <bool GATED>
 int run_w4(b200gemm_t h, const void* w0, const void* w1, const void* X, long long ldx, W4NtParams p,
            cudaStream_t stream) {
-  const long long token_blocks = (static_cast<long long>(p.M) + 31) / 32;
+  W4Launch l;
+  l.tok = p.M > 32 ? 64 : 32;
+  const long long token_blocks = (static_cast<long long>(p.M) + l.tok - 1) / l.tok;
   if (token_blocks > 65535) return B200GEMM_ERR_TOO_LARGE;
   const auto stages = [&](int k) { return static_cast<int>((static_cast<long long>(p.K) + k - 1) / k); };
-  W4Launch l;
   l.token_blocks = static_cast<int>(token_blocks);
   l.stream = stream;
   // 16 rows of X and fewer: mma.sync, whose cost grows with them.  From 9 rows
@@ -510,7 +526,7 @@ int run_w4(b200gemm_t h, const void* w0, const void* w1, const void* X, long lon
   };
   if (!encode_w(&l.w0, w0) || (GATED && !encode_w(&l.w1, w1)) ||
       !encode_2d(&l.x, X, static_cast<uint64_t>(p.K), static_cast<uint64_t>(p.M), static_cast<uint64_t>(ldx) * 2,
-                 mma ? 64 : 256, mma ? 32u : static_cast<uint32_t>(8 * nt),
+                 mma ? 64 : 256, mma ? static_cast<uint32_t>(l.tok) : static_cast<uint32_t>(8 * nt),
                  mma ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE)) {
     return B200GEMM_ERR_CUDA;
   }
@@ -523,8 +539,7 @@ int run_w4(b200gemm_t h, const void* w0, const void* w1, const void* X, long lon
   p.status = h->status_dev;
   cudaError_t e;
   if (mma) {
-    if constexpr (GATED) e = launch_w4_mma<true, 2>(l, p);
-    else e = l.plan.mt == 2 ? launch_w4_mma<false, 2>(l, p) : launch_w4_mma<false, 1>(l, p);
+    e = launch_w4_mma<GATED>(l, p);
   } else if (p.group_shift == 5) {
     e = nt == 1 ? launch_w4<GATED, true, 1>(l, p) : launch_w4<GATED, true, 2>(l, p);
   } else {

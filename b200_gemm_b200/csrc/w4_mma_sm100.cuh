@@ -2,7 +2,7 @@
 // 16 rows of activations (run_w4 says when for fewer), on the 5th-generation
 // tensor cores:
 //   Y = X W^T,   H = act(X Wg^T) * (X Wu^T)
-// at most 32 rows of X per CTA (blocks of 32 rows of X beyond that).
+// 32 rows of X per CTA, or 64 from 33 on (blocks of 64 rows beyond that).
 //
 // With mma.sync every 8 rows of X cost as many instructions again as the
 // weights' expansion; here they cost the issuing threads nothing.  128 rows of
@@ -20,6 +20,8 @@
 // the rate of wide ones), and next to them the expansion and its stores to
 // TMEM.  28416 x 4096, groups of 128, 32 rows: 26 us (mma.sync: 37), 58 MB of
 // weights at 2.3 TB/s; 8192 x 8192: 18 us (25); gated 14336 x 4096: 24 us (53).
+// 64 rows in one CTA take 32, 21 and 29 us (in two CTAs of 32: 51, 27 and 45):
+// the MMAs take little more, the epilogue twice as long.
 //
 // Warps: 0 .. 4H-1   epilogue: block w / 4 of 128 rows, TMEM lanes 32 (w % 4) ..
 //        16 or 8     expansion, two groups of eight for the steps in turn, or
@@ -42,29 +44,33 @@
 namespace b200gemm {
 
 // SG: groups per 128 k's (1 for groups of 128 and 256).
-template <bool GATED, int H, int SG>
+template <bool GATED, int H, int SG, int TOK>
 struct W4MmaCfg {
+  static_assert(TOK == 32 || TOK == 64, "rows of X");
   static_assert(H == 1 || H == 2, "blocks of 128 rows");
   static_assert(!GATED || H == 2, "Wg and Wu");
   static_assert(SG == 1 || SG == 2 || SG == 4, "groups of 128 or more, 64, 32");
   static constexpr bool kGatedOut = GATED;
   static constexpr int kH = H;
   static constexpr int kSG = SG;
-  static constexpr int kTok = 32;
+  static constexpr int kTok = TOK;
   static constexpr int kStageK = 256;                  // k's of a stage of the ring
   static constexpr int kStepK = 128;                   // k's expanded and multiplied at a time: half a stage
   static constexpr int kEpiWarps = 4 * H;
   // Two groups of expansion warps take the steps in turn.  In groups of 32 the
   // epilogue is what lasts, and one group leaves it the registers to fetch its
   // next sums ahead (gated 14331 x 4096, 32 rows: 35.7 -> 31.8 us).
-  static constexpr int kExpGroups = SG == 4 ? 1 : 2;
+  static constexpr int kExpGroups = SG == 4 || TOK == 64 ? 1 : 2;
   static constexpr int kExpWarps = 8;                  // of each group
+  // Two sets of accumulators, for the even and the odd steps, each of two
+  // groups at most (one with 64 rows of X) and filled again for the others.
+  static constexpr int kSetsPerStep = TOK == 64 ? SG : (SG == 4 ? 2 : 1);
   // Warps that issue MMAs.  One block's eight MMAs of a step take less than a
-  // warp's waits and commits around them, and groups of 32 wait twice: there
+  // warp's waits and commits around them, and sets that are filled again wait more often: there
   // two warps take the steps in turn (14336 x 4096 turned, 32 rows: 17.2 -> 15.8
   // us).  With two blocks one warp is better, as the earlier step's MMAs all
   // come first (28416 x 4096: 27.2 -> 25.8 us).
-  static constexpr int kMmaWarps = H == 1 || SG == 4 ? 2 : 1;
+  static constexpr int kMmaWarps = H == 1 || kSetsPerStep > 1 ? 2 : 1;
   static constexpr int kThreads = 32 * (kEpiWarps + kExpGroups * kExpWarps + 1 + kMmaWarps);
   static constexpr int kCodes = 128 * 128;             // one block's codes of a stage: 128 bytes a row
   static constexpr int kStageX = 4 * kTok * 128;       // four boxes of 64 k's
@@ -72,9 +78,6 @@ struct W4MmaCfg {
   static constexpr int kBlockA = kStepK / 2;           // TMEM columns of one block's operand
   static constexpr int kBufA = H * kBlockA;
   static constexpr int kBufs = H == 1 ? 4 : 2;         // operand buffers
-  // Two sets of accumulators, for the even and the odd steps, each of two
-  // groups at most (groups of 32 fill theirs twice a step).
-  static constexpr int kSetsPerStep = SG == 4 ? 2 : 1;
   static constexpr int kSetGroups = SG / kSetsPerStep;
   static constexpr int kTmemSet = H * kSetGroups * kTok;
   static constexpr int kTmemAcc = kBufs * kBufA;       // the accumulators' first column
@@ -82,7 +85,7 @@ struct W4MmaCfg {
   static constexpr int kTmemCols = 512;
   static_assert(kTmemUsed <= kTmemCols && kTmemUsed > 256, "TMEM columns");
   static constexpr int kBars = 256;
-  static constexpr int kRing = H == 1 ? 6 : 4;
+  static constexpr int kRing = 192 * 1024 / kStageBytes;
   static constexpr int kRingAt = 0;                    // X's boxes first in a stage: 1024-byte aligned
   static constexpr int kBarsAt = kRingAt + kRing * kStageBytes;
   static constexpr int kSmemBytes = 1024 + kBarsAt + kBars;
@@ -188,7 +191,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
   if (warp == kProducer) {
     // ------------------------------------------------------------ producer
     if (lane == 0) {
-      const uint64_t policy_w = ptx::policy_evict_first();  // read once (per 32 rows of X)
+      const uint64_t policy_w = ptx::policy_evict_first();  // read once (per block of rows of X)
       const uint64_t policy_x = ptx::policy_evict_last();   // read by every CTA
       auto load_w = [&](int it, int s) {
         const uint32_t bar = full0 + 8 * s, dst = base + Cfg::kRingAt + s * Cfg::kStageBytes + Cfg::kStageX;
@@ -370,7 +373,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
       ptx::tc_fence_after();
       // Chunks of 16 columns; with a register set to spare the next one is on
       // its way while this one is added.
-      constexpr int CHUNKS = Cfg::kSetGroups * TOK / 16, AHEAD = SG == 4 ? 2 : 1;
+      constexpr int CHUNKS = Cfg::kSetGroups * TOK / 16, AHEAD = SG == 4 && TOK == 32 ? 2 : 1;
       uint32_t v[AHEAD][16];
       ptx::tmem_ld_32x32b_x16(t_row + set * Cfg::kTmemSet, v[0]);
 #pragma unroll

@@ -371,7 +371,7 @@ int b200gemm_w4_dequantize(b200gemm_t handle, int N, int K, const void* codes, c
  * to its elements.  No weight is rounded: the products of a group are summed
  * unscaled in fp32 and the sum is scaled in fp32.  A scale that is a NaN or an
  * infinity makes its weight row's results NaN.  Made for a few rows (the
- * weights are read once per 32 rows of A; b200gemm_bf16_nt with dequantized
+ * weights are read once for up to 64 rows of A; b200gemm_bf16_nt with dequantized
  * ones is faster from about 65 rows on); any M works. */
 int b200gemm_w4_nt(b200gemm_t handle, int M, int N, int K, const void* A, long long lda,
                    const void* codes, const void* scales, int group, void* C, long long ldc,

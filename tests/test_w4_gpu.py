@@ -364,3 +364,17 @@ def test_gated_many_rows_of_weights(gpu_handle, M, F, K, group):
     out = gpu_handle.w4_gated(x, *gate, *up, activation="silu")
     assert gpu_handle.last_device_status()[0] == 0
     plain.close(out, *plain.gated(*_w4_product(x, *gate), *_w4_product(x, *up), "silu"))
+
+
+@pytest.mark.parametrize("group", [32, 64, 128, 256])
+@pytest.mark.parametrize("M,N,K", [(64, 300, 2304), (65, 100, 256), (128, 7000, 1280)])
+def test_nt_blocks_of_64_rows(gpu_handle, M, N, K, group):
+    _check_nt(gpu_handle, M, N, K, group, dtype=torch.float32, seed=M, pad=8)
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_gated_blocks_of_64_rows(gpu_handle, group):
+    x = plain.rows(90, 1536, 1)
+    gate, up = plain.w4_random(3000, 1536, group, 2), plain.w4_random(3000, 1536, group, 3)
+    out = gpu_handle.w4_gated(x, *gate, *up, activation="relu")
+    plain.close(out, *plain.gated(*_w4_product(x, *gate), *_w4_product(x, *up), "relu"))
