@@ -14,6 +14,8 @@ from . import _lib
 ACTIVATIONS = {"none": _lib.ACT_NONE, "relu": _lib.ACT_RELU, "gelu": _lib.ACT_GELU,
                "gelu_tanh": _lib.ACT_GELU_TANH, "silu": _lib.ACT_SILU}
 W4_GROUPS = (32, 64, 128, 256)
+
+
 class _NoContext:
     """contextlib.nullcontext without its cost."""
 
