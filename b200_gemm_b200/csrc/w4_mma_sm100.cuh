@@ -67,7 +67,7 @@ struct W4MmaCfg {
   static constexpr int kSetsPerStep = TOK == 64 ? SG : (SG == 4 ? 2 : 1);
   // Warps that issue MMAs.  One block's eight MMAs of a step take less than a
   // warp's waits and commits around them, and sets that are filled again wait more often: there
-  // two warps take the steps in turn (14336 x 4096 turned, 32 rows: 17.2 -> 15.8
+  // two warps take the steps in turn (4096 x 14336, 32 rows: 17.2 -> 15.8
   // us).  With two blocks one warp is better, as the earlier step's MMAs all
   // come first (28416 x 4096: 27.2 -> 25.8 us).
   static constexpr int kMmaWarps = H == 1 || kSetsPerStep > 1 ? 2 : 1;
