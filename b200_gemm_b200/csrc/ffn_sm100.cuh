@@ -201,6 +201,27 @@ __device__ __forceinline__ bool ffn_unit(const FfnParams& p, int c, int g, int i
   return true;
 }
 
+// The normal distribution's integral Phi(x), and e = e^(-x^2/2).  By its tail,
+// 1 - Phi(|x|) = e t P(t) with t = 1 / (1 + 0.33 |x|), so that it keeps its
+// relative accuracy for x < 0 (as 1 + erf it would have lost all digits at
+// x = -5.6, where x Phi(x) is -6e-8).  P: our own fit of degree 7 for the least
+// maximal relative error over all x >= 0, 2^-19.6 with fp32's roundings.  The
+// gated block 8192 x 14336 x 4096 (G and U kept) with erff, erfcf and this:
+// 1.48, 1.59 and 1.46 ms; its gradients 2.96, 3.09 and 2.91 ms.
+__device__ __forceinline__ float normal_cdf(float x, float& e) {
+  const float t = ptx::rcp_approx(fmaf(0.33f, fabsf(x), 1.0f));
+  float p = fmaf(0.033285525f, t, -0.10566421f);
+  p = fmaf(p, t, 0.06743017f);
+  p = fmaf(p, t, 0.033429552f);
+  p = fmaf(p, t, 0.09100458f);
+  p = fmaf(p, t, 0.11721682f);
+  p = fmaf(p, t, 0.13164698f);
+  p = fmaf(p, t, 0.13165107f);
+  e = __expf(-0.5f * x * x);
+  const float tail = p * t * e;
+  return x < 0.0f ? tail : 1.0f - tail;
+}
+
 // act(x) for bf16 results: e^x and the reciprocal are the fast forms, whose
 // relative error (2^-21) is far below bf16's 2^-9.  The tanh form of GELU
 // goes through the logistic function, 0.5 (1 + tanh z) = 1 / (1 + e^-2z),
@@ -208,7 +229,10 @@ __device__ __forceinline__ bool ffn_unit(const FfnParams& p, int c, int g, int i
 template <int ACT>
 __device__ __forceinline__ float ffn_act(float x) {
   if constexpr (ACT == kActRelu) return fmaxf(x, 0.0f);
-  if constexpr (ACT == kActGelu) return 0.5f * x * (1.0f + erff(x * 0.70710678118654752f));
+  if constexpr (ACT == kActGelu) {
+    float e;
+    return x * normal_cdf(x, e);
+  }
   if constexpr (ACT == kActGeluTanh)
     return x * ptx::rcp_approx(1.0f + __expf(-1.5957691216057308f * fmaf(0.044715f * x, x * x, x)));
   if constexpr (ACT == kActSilu) return x * ptx::rcp_approx(1.0f + __expf(-x));
@@ -226,9 +250,10 @@ __device__ __forceinline__ void ffn_act_grad(float x, float& a, float& da) {
     a = fmaxf(x, 0.0f);
     da = x > 0.0f ? 1.0f : 0.0f;
   } else if constexpr (ACT == kActGelu) {
-    const float phi = 0.5f * (1.0f + erff(x * 0.70710678118654752f));
+    float e;
+    const float phi = normal_cdf(x, e);
     a = x * phi;
-    da = fmaf(x * 0.39894228040143268f, __expf(-0.5f * x * x), phi);
+    da = fmaf(x * 0.39894228040143268f, e, phi);
   } else if constexpr (ACT == kActGeluTanh) {
     const float x2 = x * x;
     const float s = ptx::rcp_approx(1.0f + __expf(-1.5957691216057308f * fmaf(0.044715f * x, x2, x)));
