@@ -225,10 +225,11 @@ __device__ __forceinline__ float normal_cdf(float x, float& e) {
 // act(x) for bf16 results: e^x and the reciprocal are the fast forms, whose
 // relative error (2^-21) is far below bf16's 2^-9.  The tanh form of GELU
 // goes through the logistic function, 0.5 (1 + tanh z) = 1 / (1 + e^-2z),
-// which keeps its relative accuracy where tanh is near -1.
+// which keeps its relative accuracy where tanh is near -1.  A NaN stays one
+// under each of them.
 template <int ACT>
 __device__ __forceinline__ float ffn_act(float x) {
-  if constexpr (ACT == kActRelu) return fmaxf(x, 0.0f);
+  if constexpr (ACT == kActRelu) return ptx::max_nan(x, 0.0f);
   if constexpr (ACT == kActGelu) {
     float e;
     return x * normal_cdf(x, e);
@@ -247,8 +248,8 @@ __device__ __forceinline__ float ffn_act(float x) {
 template <int ACT>
 __device__ __forceinline__ void ffn_act_grad(float x, float& a, float& da) {
   if constexpr (ACT == kActRelu) {
-    a = fmaxf(x, 0.0f);
-    da = x > 0.0f ? 1.0f : 0.0f;
+    a = ptx::max_nan(x, 0.0f);
+    da = x > 0.0f ? 1.0f : (x <= 0.0f ? 0.0f : x);
   } else if constexpr (ACT == kActGelu) {
     float e;
     const float phi = normal_cdf(x, e);

@@ -542,6 +542,12 @@ __device__ __forceinline__ float rcp_approx(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// The larger of two, or NaN if one of them is (fmaxf returns the other).
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
 
 // 16-byte load of data that stays unchanged for the whole kernel (bias,
 // residual) through the non-coherent path.

@@ -313,7 +313,8 @@ int b200gemm_bf16_nt_noalloc(int M, int N, int K, const void* A, const void* B, 
 
 /* Gated block, one kernel:  G = X Wg^T,  U = X Wu^T,  H = act(G) * U
  *   X [M,K], Wg and Wu [F,K] (one pitch ldw), H [M,F], all bf16; fp32 sums,
- *   H rounded once.  activation: B200GEMM_ACT_*.
+ *   H rounded once.  activation: B200GEMM_ACT_*; a NaN in G is a NaN in H under
+ *   each of them.
  * G and U, both or neither, receive the two products rounded to bf16 (one
  * pitch ldgu): what b200gemm_bf16_gated_backward needs.  Any M and F;
  * K % 8 == 0, K > 0; pitches % 8 == 0; every pointer 16-byte aligned.

@@ -98,3 +98,76 @@ def test_lower_tail_gradient(gpu_handle, kind):
     a, ea, da, eda = _tail(g, kind)
     plain.close(dwu[:, 0], a, ea)
     plain.close(dwg[:, 0], da, eda)
+
+
+def _others_equal(got, ref, bad_rows=(), bad_cols=()):
+    rows = [r for r in range(got.shape[0]) if r not in bad_rows]
+    cols = [c for c in range(got.shape[1]) if c not in bad_cols]
+    assert torch.equal(got[rows][:, cols], ref[rows][:, cols])
+
+
+@pytest.mark.parametrize("kind", plain.ACTS)
+@pytest.mark.parametrize("M", [5, 70])
+def test_bad_values_of_the_gated_block(gpu_handle, M, kind):
+    """A NaN among the weights or the activations is a NaN in every result that
+    it is part of, under each activation, an infinity is nothing finite; the
+    other results keep their bits."""
+    x = plain.rows(M, 128, 1)
+    wg, wu = (plain.rows(101, 128, i, 0.1) for i in (2, 3))
+    H, G, U = gpu_handle.gated(x, wg, wu, activation=kind, save=True)
+    for which, col in ((0, 7), (1, 100)):
+        w = [wg.clone(), wu.clone()]
+        w[which][col, 5] = float("nan")
+        h, g, u = gpu_handle.gated(x, *w, activation=kind, save=True)
+        assert h[:, col].isnan().all() and (g, u)[which][:, col].isnan().all()
+        _others_equal(h, H, bad_cols=(col,))
+        _others_equal((g, u)[1 - which], (G, U)[1 - which])
+    y = x.clone()
+    y[1, 9], y[4, 127] = float("nan"), float("-inf")
+    h = gpu_handle.gated(y, wg, wu, activation=kind)
+    assert h[1].isnan().all() and not h[4].isfinite().any()
+    _others_equal(h, H, bad_rows=(1, 4))
+
+
+@pytest.mark.parametrize("kind", plain.ACTS)
+@pytest.mark.parametrize("M,F,K", [(40, 70, 64), (17, 1100, 72)])
+def test_bad_values_of_the_gradients(gpu_handle, M, F, K, kind):
+    """The same backward, for dX of one range and of several: a bad dH, G or U
+    at (m, f) reaches row m of dX and row f of dWg or dWu."""
+    args = {"dH": plain.rows(M, F, 0), "X": plain.rows(M, K, 1), "Wg": plain.rows(F, K, 2), "Wu": plain.rows(F, K, 3),
+            "G": plain.rows(M, F, 4), "U": plain.rows(M, F, 5)}
+    ref = gpu_handle.gated_backward(**args, activation=kind)
+    m, f = 16, F - 1
+    for name, value in (("dH", "nan"), ("G", "nan"), ("U", "nan"), ("dH", "inf"), ("U", "-inf")):
+        bad = dict(args)
+        t = plain.rows(M, F, {"dH": 0, "G": 4, "U": 5}[name])
+        t[m, f] = float(value)
+        bad[name] = t
+        dx, dwg, dwu = gpu_handle.gated_backward(**bad, activation=kind)
+        in_dg, in_du = name != "G" or kind != "none", name != "U"
+        reached = [dx[m]] + ([dwg[f]] if in_dg else []) + ([dwu[f]] if in_du else [])
+        assert all(r.isnan().all() if value == "nan" else not r.isfinite().any() for r in reached)
+        _others_equal(dx, ref[0], bad_rows=(m,))
+        _others_equal(dwg, ref[1], bad_rows=(f,) if in_dg else ())
+        _others_equal(dwu, ref[2], bad_rows=(f,) if in_du else ())
+
+
+@pytest.mark.parametrize("kind", plain.ACTS)
+@pytest.mark.parametrize("M,group", [(3, 32), (3, 128), (12, 32), (12, 64), (40, 32), (40, 128)])
+def test_bad_values_of_the_4bit_gated_block(gpu_handle, M, group, kind):
+    x = plain.rows(M, 384, 1)
+    gate, up = (plain.w4_random(150, 384, group, i) for i in (2, 3))
+    H = gpu_handle.w4_gated(x, *gate, *up, activation=kind)
+    for which, value in ((0, "nan"), (1, "nan"), (0, "inf"), (1, "-inf")):
+        w = [gate, up]
+        s = w[which][1].clone()
+        s[-1, 149] = s[0, 3] = float(value)
+        w[which] = (w[which][0], s)
+        h = gpu_handle.w4_gated(x, *w[0], *w[1], activation=kind)
+        assert h[:, [3, 149]].isnan().all()
+        _others_equal(h, H, bad_cols=(3, 149))
+    y = x.clone()
+    y[0, 380], y[2, 0] = float("nan"), float("inf")
+    h = gpu_handle.w4_gated(y, *gate, *up, activation=kind)
+    assert h[0].isnan().all() and not h[2].isfinite().any()
+    _others_equal(h, H, bad_rows=(0, 2))
