@@ -321,8 +321,9 @@ bool encode_out(CUtensorMap* m, void* ptr, int cols, int rows, long long ld) {
 // estimated to beat the tiled kernel, whose few tiles of a small block leave
 // most SMs idle.  In microseconds, measured on B200: 0.315 per unit of
 // ffn_tile_time; the weights at 5 TB/s with 32 rows of X; 4 of either launch.
+// Never past the 65535 blocks of 32 columns that its grid takes.
 bool gated_uses_decode(const b200gemm_handle* h, int M, int F, int K) {
-  if (h->small_m == 0 || h->tile_width != 0 || M > 128) return false;
+  if (h->small_m == 0 || h->tile_width != 0 || M > 128 || F > 65535 * 32) return false;
   if (M <= 32) return true;
   const int num_kb = (K + kBlockK - 1) / kBlockK;
   const int width = ffn_gated_width(h, 1, F, num_kb);
@@ -358,7 +359,6 @@ int run_gated_decode(b200gemm_t h, const void* Wg, const void* Wu, long long ldw
   const int nt = p.M > 16 ? 4 : (p.M > 8 ? 2 : 1);
   const long long blocks = (static_cast<long long>(p.F) + 31) / 32;
   const int token_blocks = (p.M + 31) / 32;
-  if (blocks > 65535) return B200GEMM_ERR_TOO_LARGE;
   CUtensorMap mg, mu, mx;
   const auto encode = [&](CUtensorMap* m, const void* ptr, int rows, long long ld, int box_rows) {
     return encode_kmajor(m, ptr, p.K, rows, ld, box_rows);

@@ -171,3 +171,15 @@ def test_bad_values_of_the_4bit_gated_block(gpu_handle, M, group, kind):
     h = gpu_handle.w4_gated(y, *gate, *up, activation=kind)
     assert h[0].isnan().all() and not h[2].isfinite().any()
     _others_equal(h, H, bad_rows=(0, 2))
+
+
+@pytest.mark.parametrize("F", [65535 * 32, 65535 * 32 + 1])
+def test_gated_few_rows_of_very_many_columns(gpu_handle, F):
+    """The last width that the kernel for few rows can take, and the next one."""
+    x = plain.rows(2, 8, 0)
+    wg, wu = (torch.randn(F, 8, generator=torch.Generator("cuda").manual_seed(i), device="cuda").to(BF) for i in (1, 2))
+    H = gpu_handle.gated(x, wg, wu, activation="relu")
+    assert gpu_handle.last_device_status()[0] == 0
+    g, eg = plain.product(x, wg)
+    u, eu = plain.product(x, wu)
+    plain.close(H, *plain.gated(g, eg, u, eu, "relu"))
