@@ -487,10 +487,22 @@ cudaError_t launch_w4_mma(const W4Launch& l, const W4NtParams& p) {
 template <bool GATED>
 int run_w4(b200gemm_t h, const void* w0, const void* w1, const void* X, long long ldx, W4NtParams p,
            cudaStream_t stream) {
+  // The grid takes 65535 blocks of rows of X: more of them in several launches.
+  constexpr int kRowsPerLaunch = 65535 * 64;
+  if (p.M > kRowsPerLaunch) {
+    const long long row_bytes = p.ldo * (p.out_type == kOutF32 ? 4 : 2);
+    for (long long m = 0; m < p.M; m += kRowsPerLaunch) {
+      W4NtParams part = p;
+      part.M = static_cast<int>(p.M - m < kRowsPerLaunch ? p.M - m : kRowsPerLaunch);
+      part.out = static_cast<uint8_t*>(p.out) + m * row_bytes;
+      const int rc = run_w4<GATED>(h, w0, w1, static_cast<const uint16_t*>(X) + m * ldx, ldx, part, stream);
+      if (rc != B200GEMM_OK) return rc;
+    }
+    return B200GEMM_OK;
+  }
   W4Launch l;
   l.tok = p.M > 32 ? 64 : 32;
   const long long token_blocks = (static_cast<long long>(p.M) + l.tok - 1) / l.tok;
-  if (token_blocks > 65535) return B200GEMM_ERR_TOO_LARGE;
   const auto stages = [&](int k) { return static_cast<int>((static_cast<long long>(p.K) + k - 1) / k); };
   l.token_blocks = static_cast<int>(token_blocks);
   l.stream = stream;

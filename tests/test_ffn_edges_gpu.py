@@ -183,3 +183,32 @@ def test_gated_few_rows_of_very_many_columns(gpu_handle, F):
     g, eg = plain.product(x, wg)
     u, eu = plain.product(x, wu)
     plain.close(H, *plain.gated(g, eg, u, eu, "relu"))
+
+
+@pytest.mark.parametrize("gated", [False, True])
+def test_4bit_products_of_very_many_rows(gpu_handle, gated):
+    """More rows of X than one launch's grid takes: 65535 blocks of 64."""
+    M, N, K = 65535 * 64 + 5, 3, 32
+    x = torch.randn(M, K, generator=torch.Generator("cuda").manual_seed(0), device="cuda").to(BF)
+    gate, up = plain.w4_random(N, K, 32, 1), plain.w4_random(N, K, 32, 2)
+    buf = torch.full((M + 1, N), 7.0, dtype=BF, device="cuda")
+    if gated:
+        gpu_handle.w4_gated(x, *gate, *up, activation="none", out=buf[:M])
+    else:
+        gpu_handle.w4_nt(x, *gate, out=buf[:M])
+    assert gpu_handle.last_device_status()[0] == 0
+
+    def product(codes, scales):
+        # Two steps of 16 products of (q - 8) x, each of 17 terms truncated to
+        # 2^-22 of the largest, at most 8 sum|x|; scaled, with a few roundings.
+        w = plain.w4_values(codes, scales)
+        x64 = x.double()
+        err = 2 * 17 * 8 * 2.0 ** -22 * x64.abs().sum(1, keepdim=True) * scales.double() + 4 * ULP * (x64.abs() @ w.abs().t())
+        return x64 @ w.t(), err
+
+    g, eg = product(*gate)
+    if gated:
+        plain.close(buf[:M], *plain.gated(g, eg, *product(*up), "none"))
+    else:
+        plain.close(buf[:M], g, eg)
+    assert (buf[M] == 7.0).all()
