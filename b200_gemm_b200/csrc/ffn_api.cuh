@@ -257,11 +257,13 @@ int ffn_gated_width(const b200gemm_handle* h, int tiles_m, int F, int num_kb) {
 // the mean load and half a dW tile, or what the dX tiles take by themselves.
 // Where dX has too few tiles for the clusters, its sum is split into up to 16
 // ranges of at least 8 K blocks (another launch, and their partial sums, cost
-// about 10 units).
+// about 10 units).  The ranges are those of a call for all gradients also where
+// dX alone is asked for, since the order of its sum goes by them.
 struct GradsPlan {
-  int width = 256, split = 1, slice_kb = 0;
+  int width = 256, split = 1, slice_kb = 0, want = 1;
 };
 GradsPlan grads_plan(const b200gemm_handle* h, int m, int f, int k, bool dx, bool dw, bool may_split) {
+  const int ranges = !dx || !may_split ? 1 : (dw ? 0 : grads_plan(h, m, f, k, true, true, true).want);  // 0: any
   GradsPlan best;
   double best_cost = 1e300;
   const double g = h->ffn_clusters;
@@ -271,9 +273,9 @@ GradsPlan grads_plan(const b200gemm_handle* h, int m, int f, int k, bool dx, boo
     const double tn = static_cast<double>((k + width - 1ll) / width);
     const double n1 = dx ? tn * ((m + 255ll) / 256) : 0.0, n2 = dw ? 2.0 * tn * ((f + 255ll) / 256) : 0.0;
     const double t2 = dw_tile_time(width, (m + 63) / 64);
-    for (int want = 1; want <= (dx && may_split ? 16 : 1); want *= 2) {
+    for (int want = ranges > 0 ? ranges : 1; want <= (ranges > 0 ? ranges : 16); want *= 2) {
       const int slice = (kb + want - 1) / want, split = (kb + slice - 1) / slice;
-      if (split > 1 && (slice < 8 || n1 * split > 2.0 * g)) break;
+      if (ranges == 0 && split > 1 && (slice < 8 || n1 * split > 2.0 * g)) break;
       const double t1 = ffn_tile_time(width, slice, 0.0);
       const double mean = (n1 * split * t1 + n2 * t2) / g + (n2 > 0.0 ? 0.5 * t2 : 0.0);
       double cost = static_cast<double>(static_cast<long long>((n1 * split + g - 1.0) / g)) * t1;
@@ -286,6 +288,7 @@ GradsPlan grads_plan(const b200gemm_handle* h, int m, int f, int k, bool dx, boo
         best.width = width;
         best.split = split;
         best.slice_kb = slice;
+        best.want = want;
       }
     }
   }
@@ -668,11 +671,7 @@ extern "C" int b200gemm_bf16_gated(b200gemm_t h, int M, int F, int K, const void
 extern "C" unsigned long long b200gemm_gated_backward_workspace(b200gemm_t h, int M, int F, int K) {
   if (h == nullptr || M <= 0 || F <= 0 || K <= 0 || M > kMaxExtent || F > kMaxExtent || K > kMaxExtent) return 0;
   std::lock_guard<std::mutex> lock(h->mu);
-  int split = 1;
-  for (bool dw : {false, true}) {
-    const int s = grads_plan(h, M, F, K, true, dw, true).split;
-    split = s > split ? s : split;
-  }
+  const int split = grads_plan(h, M, F, K, true, true, true).split;
   return (grads_base_bytes(M, F) + 15) / 16 * 16 + grads_partial_bytes(M, K, split);
 }
 

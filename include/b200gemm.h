@@ -341,9 +341,10 @@ unsigned long long b200gemm_gated_backward_workspace(b200gemm_t handle, int M, i
  * weight gradients are zeros, with F == 0 dX is.  act'(0) of relu is 0.
  * workspace: 16-byte aligned, its contents before and after mean nothing; it
  * is in use until the call's work on `stream` is done.  With less than the
- * size above the call does without partial sums; less than 4 M F' bytes is
- * B200GEMM_ERR_UNSUPPORTED.  The same rules as
- * b200gemm_bf16_gated otherwise. */
+ * size above the call does without partial sums (dX's sum then runs in another
+ * order, as it may with another forced tile width; it does not change with the
+ * results asked for); less than 4 M F' bytes is B200GEMM_ERR_UNSUPPORTED.  The
+ * same rules as b200gemm_bf16_gated otherwise. */
 int b200gemm_bf16_gated_backward(b200gemm_t handle, int M, int F, int K, const void* dH,
                                  long long lddh, const void* X, long long ldx, const void* Wg,
                                  const void* Wu, long long ldw, const void* G, const void* U,

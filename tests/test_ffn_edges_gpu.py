@@ -212,3 +212,17 @@ def test_4bit_products_of_very_many_rows(gpu_handle, gated):
     else:
         plain.close(buf[:M], g, eg)
     assert (buf[M] == 7.0).all()
+
+
+@pytest.mark.parametrize("M,F,K", [(500, 3000, 1000), (300, 4100, 520), (17, 1100, 72), (1, 5003, 2056), (640, 8200, 264)])
+def test_input_gradient_on_its_own(gpu_handle, M, F, K):
+    """dX has the same bits whether the weights' gradients are asked for or
+    not, where its sum is split into ranges too."""
+    size = _lib.load().b200gemm_gated_backward_workspace(gpu_handle._h, M, F, K)
+    assert size > 4 * M * 8 * ((F + 7) // 8)  # a case that is split
+    dh, g, u = (plain.rows(M, F, i) for i in range(3))
+    x, wg, wu = plain.rows(M, K, 3), plain.rows(F, K, 4), plain.rows(F, K, 5)
+    dx, dwg, dwu = gpu_handle.gated_backward(dh, x, wg, wu, g, u)
+    assert torch.equal(gpu_handle.gated_backward(dh, x, wg, wu, g, u, weight_grad=False)[0], dx)
+    parts = gpu_handle.gated_backward(dh, x, wg, wu, g, u, input_grad=False)
+    assert torch.equal(parts[1], dwg) and torch.equal(parts[2], dwu)
