@@ -75,8 +75,10 @@ bool prepare_gated_decode_kernels() {
 // registers and ring allow next to NT tiles of X's rows.
 template <int NT>
 constexpr int kW4MaxMT = NT == 1 ? 7 : 5;
-// Rows of X up to which a 4-bit product runs on mma.sync.
+// Rows of X up to which a 4-bit product runs on mma.sync, whose CTAs hold all
+// of them (8 NT).
 constexpr int kW4MaxSyncRows = 16;
+static_assert(kW4MaxSyncRows <= W4NtCfg<false, false, 1, 2>::kTok, "rows of X of one CTA");
 
 template <bool GATED, bool G32, int NT, int MT = kW4MaxMT<NT>>
 bool prepare_w4_instances() {
@@ -392,13 +394,13 @@ struct W4Plan {
   int rows = 0, mt = 0, split = 1;
   long long waves = 1;
 };
-W4Plan w4_plan(const b200gemm_handle* h, int N, int token_blocks, int num_stages, int max_mt, bool gated) {
+W4Plan w4_plan(const b200gemm_handle* h, int N, int num_stages, int max_mt, bool gated) {
   const int tiles = gated ? 1 : 2;  // 16-row tiles of output per unit of mt
   W4Plan best;
   double best_cost = 1e300;
   for (int i = 0, split = 1; i < 4; ++i, split *= 2) {
     if (split > 1 && num_stages < 2 * split) break;
-    const int fit = h->w4_clusters[i] / token_blocks > 0 ? h->w4_clusters[i] / token_blocks : 1;
+    const int fit = h->w4_clusters[i];
     const long long per_wave = 16ll * max_mt * tiles * fit;
     const long long waves = (N + per_wave - 1) / per_wave;
     const int rows = static_cast<int>((N + waves * fit - 1) / (waves * fit));
@@ -430,7 +432,7 @@ cudaError_t launch_w4(const W4Launch& l, const W4NtParams& p) {
   } else {
     using Cfg = W4NtCfg<GATED, G32, MT, NT>;
     if (l.plan.mt != MT) return launch_w4<GATED, G32, NT, MT - 1>(l, p);
-    return launch_rows(w4_nt_sm100<Cfg>, Cfg::kThreads, Cfg::kSmemBytes, l.plan.split, l.blocks, l.token_blocks,
+    return launch_rows(w4_nt_sm100<Cfg>, Cfg::kThreads, Cfg::kSmemBytes, l.plan.split, l.blocks, 1,
                        l.stream, l.w0, l.w1, l.x, p);
   }
 }
@@ -519,7 +521,7 @@ int run_w4(b200gemm_t h, const void* w0, const void* w1, const void* X, long lon
   const int nt = p.M > 8 ? 2 : 1;
   W4Plan sync_plan, mma_plan;
   if (p.M <= kW4MaxSyncRows)
-    sync_plan = w4_plan(h, p.N, l.token_blocks, stages(512), nt == 1 ? kW4MaxMT<1> : kW4MaxMT<2>, GATED);
+    sync_plan = w4_plan(h, p.N, stages(512), nt == 1 ? kW4MaxMT<1> : kW4MaxMT<2>, GATED);
   bool mma = p.M > kW4MaxSyncRows || (nt == 2 && sync_plan.waves > 1 && p.group_shift > 5);
   if (mma) {
     mma_plan = w4_mma_plan(h, p.N, l.token_blocks, stages(256), GATED);

@@ -149,7 +149,6 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
   const int split = static_cast<int>(gridDim.x);   // CTAs of this cluster: K ranges
   const int rank = static_cast<int>(blockIdx.x);
   const int n0 = static_cast<int>(blockIdx.y) * p.rows;
-  const int m0 = static_cast<int>(blockIdx.z) * 32;
   const int s_begin = rank * p.stages_per_cta;
   const int count = max(0, min(p.num_stages, s_begin + p.stages_per_cta) - s_begin);
 
@@ -175,7 +174,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
 #pragma unroll
     for (int b = 0; b < 2; ++b)
       ptx::tma_load_2d(ring + s * Cfg::kStageBytes + Cfg::kStageW + b * Cfg::kBoxX, &map_x, full0 + 8 * s,
-                       (s_begin + it) * Cfg::kStageK + b * 256, m0, policy_x);
+                       (s_begin + it) * Cfg::kStageK + b * 256, 0, policy_x);
   };
 
   const uint32_t half = warp >> 3, part = warp & 7u;  // rows, and k's 64 part .. of every stage
@@ -226,9 +225,9 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
   }
   __syncwarp();
 
-  // Fragment row (or column) g of 8 stands for row tok(g), so that the 8
-  // lanes of a 16-byte access phase (two rows, 4 chunks each) hit all 8 chunk
-  // places of the 128-byte swizzle.
+  // Fragment row (or column) g of 8 stands for row tok(g), as in the bf16 kernel
+  // for few rows.  The 8 rows of a 4-byte load of codes have their chunks at the
+  // 8 places of the 128-byte swizzle, so a warp's lanes hit all banks.
   const uint32_t g = lane >> 2, t = lane & 3u;
   const uint32_t tokg = (g >> 1) | ((g & 1u) << 2);
   const W4Const w4c = w4_const();
@@ -351,7 +350,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
         sums[part * kSlab + tok * Cfg::kPitch + row] = 64.0f * acc[i][j][c];
       }
   __syncthreads();
-  const int toks = min(Cfg::kTok, p.M - m0);
+  const int toks = min(Cfg::kTok, p.M);
   const int cols = min(p.rows, p.N - n0);  // output columns of this CTA
   auto warp_sum = [&](uint32_t at) {
     float v = sums[at];
@@ -381,7 +380,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
       if constexpr (Cfg::kGatedOut) {
         v = gated_value(p.act, v, total(tok * Cfg::kPitch + Cfg::kHalf + c));
       }
-      const long long off = static_cast<long long>(m0 + tok) * p.ldo + n0 + c;
+      const long long off = static_cast<long long>(tok) * p.ldo + n0 + c;
       if (p.out_type == kOutF32) static_cast<float*>(p.out)[off] = v;
       else static_cast<__nv_bfloat16*>(p.out)[off] = __float2bfloat16_rn(v);
     }
