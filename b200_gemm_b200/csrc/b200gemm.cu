@@ -462,8 +462,8 @@ struct b200gemm_handle {
   int decode_clusters[5] = {};        // [S]: co-resident clusters of the small-M pair kernel, split S
   int decode256_clusters[5] = {};     // the same for its instances covering 256 rows of A
   int smallm1_clusters[5] = {};       // [S]: the same for the single-CTA small-M kernel
-  int w4_clusters[4] = {};            // [i]: co-resident clusters of 2^i CTAs of the 4-bit product
-  int ffn_clusters = 0;               // co-resident clusters of the tiled feed-forward kernels
+  int w4_clusters[4] = {};            // [i]: co-resident clusters of 2^i CTAs of the 4-bit product, 0 before the first
+  int ffn_clusters = 0;               // co-resident clusters of the tiled feed-forward kernels, 0 before the first call
   int tile_width = 0;         // 0 = choose per call, else one of kWidths
   int small_m = -1;           // small-M kernel: -1 or 1 = use it when eligible, 0 = never
   int pdl = 0;                // B200GEMM_PDL_*: launch overlap with the previous kernel
@@ -488,13 +488,6 @@ struct b200gemm_handle {
   std::mutex staging_mu;   // serialises b200gemm_bf16_nt_host calls on one handle
   std::vector<ScheduleEntry> schedules;
 };
-
-namespace b200gemm {
-int prepare_ffn_kernels(int sm_count);
-bool prepare_gated_decode_kernels();
-bool prepare_w4_kernels();
-int w4_clusters_fit(int sm_count, int split);
-}  // namespace b200gemm
 
 extern "C" int b200gemm_version(void) { return kVersion; }
 
@@ -544,11 +537,6 @@ extern "C" int b200gemm_create(b200gemm_t* out, int device) {
   if (dw1 <= 0 || dw2 <= 0 || dw3 <= 0 || dw4 <= 0) return B200GEMM_ERR_CUDA;
   const int sc2 = prepare_smallm1_kernel<SmallMCfg<2>>(sms), sc4 = prepare_smallm1_kernel<SmallMCfg<4>>(sms);
   if (sc2 <= 0 || sc4 <= 0) return B200GEMM_ERR_CUDA;
-  const int fc = prepare_ffn_kernels(sms);
-  if (fc <= 0 || !prepare_gated_decode_kernels() || !prepare_w4_kernels()) return B200GEMM_ERR_CUDA;
-  int w4_fit[4];
-  for (int i = 0; i < 4; ++i)
-    if ((w4_fit[i] = w4_clusters_fit(sms, 1 << i)) <= 0) return B200GEMM_ERR_CUDA;
 
   auto* h = new b200gemm_handle();
   h->device = device;
@@ -562,8 +550,6 @@ extern "C" int b200gemm_create(b200gemm_t* out, int device) {
   h->decode256_clusters[4] = dw4;
   h->smallm1_clusters[2] = sc2;
   h->smallm1_clusters[4] = sc4;
-  h->ffn_clusters = fc;
-  for (int i = 0; i < 4; ++i) h->w4_clusters[i] = w4_fit[i];
   h->max_clusters = cw[0];
   for (int i = 0; i < kNumWidths; ++i) {
     h->clusters_w[i] = cw[i];

@@ -134,6 +134,28 @@ int w4_clusters_fit(int sm_count, int split) {
   return clusters;
 }
 
+// The 79 kernel instances get their shared memory, and the clusters that fit
+// are counted, at a handle's first call of their kind: who multiplies only
+// neither waits nor fails for them (a process's first b200gemm_create 36 -> 32
+// ms; the first gated call takes 1 ms instead, the first 4-bit product 3).  The
+// handle's device is current and h->mu held; false on failure.  None of it is
+// work on a stream, so a stream may be captured meanwhile.
+bool gated_ready(b200gemm_handle* h) {
+  if (h->ffn_clusters > 0) return true;
+  if (!prepare_gated_decode_kernels()) return false;
+  h->ffn_clusters = prepare_ffn_kernels(h->sm_count);
+  return h->ffn_clusters > 0;
+}
+bool w4_ready(b200gemm_handle* h) {
+  if (h->w4_clusters[0] > 0) return true;
+  if (!prepare_w4_kernels()) return false;
+  int fit[4];
+  for (int i = 0; i < 4; ++i)
+    if ((fit[i] = w4_clusters_fit(h->sm_count, 1 << i)) <= 0) return false;
+  for (int i = 0; i < 4; ++i) h->w4_clusters[i] = fit[i];
+  return true;
+}
+
 template <class Cfg>
 cudaError_t launch_ffn(int clusters, cudaStream_t stream, const FfnMaps& m, const FfnParams& p, bool overlap) {
   cudaLaunchConfig_t cfg = {};
@@ -505,6 +527,13 @@ int run_w4(b200gemm_t h, const void* w0, const void* w1, const void* X, long lon
     }
     return B200GEMM_OK;
   }
+  {
+    std::lock_guard<std::mutex> lock(h->mu);
+    if (!w4_ready(h)) return B200GEMM_ERR_CUDA;
+    p.timeout_ns = h->timeout_ns;
+    p.pdl = h->pdl;
+  }
+  p.status = h->status_dev;
   W4Launch l;
   l.tok = p.M > 32 ? 64 : 32;
   const long long token_blocks = (static_cast<long long>(p.M) + l.tok - 1) / l.tok;
@@ -548,12 +577,6 @@ int run_w4(b200gemm_t h, const void* w0, const void* w1, const void* X, long lon
     return B200GEMM_ERR_CUDA;
   }
   if (!GATED) l.w1 = l.w0;
-  {
-    std::lock_guard<std::mutex> lock(h->mu);
-    p.timeout_ns = h->timeout_ns;
-    p.pdl = h->pdl;
-  }
-  p.status = h->status_dev;
   cudaError_t e;
   if (mma) {
     e = launch_w4_mma<GATED>(l, p);
@@ -629,6 +652,7 @@ extern "C" int b200gemm_bf16_gated(b200gemm_t h, int M, int F, int K, const void
   const int num_kb = (K + kBlockK - 1) / kBlockK;
   {
     std::lock_guard<std::mutex> lock(h->mu);
+    if (!gated_ready(h)) return B200GEMM_ERR_CUDA;
     small = gated_uses_decode(h, M, F, K);
     width = ffn_gated_width(h, (M + kTileM - 1) / kTileM, F, num_kb);
   }
@@ -672,9 +696,10 @@ extern "C" int b200gemm_bf16_gated(b200gemm_t h, int M, int F, int K, const void
 
 extern "C" unsigned long long b200gemm_gated_backward_workspace(b200gemm_t h, int M, int F, int K) {
   if (h == nullptr || M <= 0 || F <= 0 || K <= 0 || M > kMaxExtent || F > kMaxExtent || K > kMaxExtent) return 0;
+  DeviceGuard guard(h->device);
   std::lock_guard<std::mutex> lock(h->mu);
-  const int split = grads_plan(h, M, F, K, true, true, true).split;
-  return (grads_base_bytes(M, F) + 15) / 16 * 16 + grads_partial_bytes(M, K, split);
+  if (!guard.ok() || !gated_ready(h)) return grads_base_bytes(M, F);
+  return grads_base_bytes(M, F) + grads_partial_bytes(M, K, grads_plan(h, M, F, K, true, true, true).split);
 }
 
 extern "C" int b200gemm_bf16_gated_backward(b200gemm_t h, int M, int F, int K, const void* dH, long long lddh,
@@ -731,6 +756,14 @@ extern "C" int b200gemm_bf16_gated_backward(b200gemm_t h, int M, int F, int K, c
   DeviceGuard guard(h->device);
   if (!guard.ok()) return B200GEMM_ERR_CUDA;
 
+  GradsPlan plan;
+  {
+    std::lock_guard<std::mutex> lock(h->mu);
+    if (!gated_ready(h)) return B200GEMM_ERR_CUDA;
+    plan = grads_plan(h, M, F, K, dX != nullptr, dWg != nullptr, true);
+    if (plan.split > 1 && workspace_bytes < base_bytes + grads_partial_bytes(M, K, plan.split))
+      plan = grads_plan(h, M, F, K, dX != nullptr, dWg != nullptr, false);
+  }
   GatedGradParams gp{};
   gp.M = M;
   gp.F = F;
@@ -761,13 +794,6 @@ extern "C" int b200gemm_bf16_gated_backward(b200gemm_t h, int M, int F, int K, c
     return B200GEMM_ERR_CUDA;
   if (dX == nullptr) m.c[0] = m.c[1];  // (not written)
   if (dWg == nullptr) m.c[1] = m.c[2] = m.c[0];
-  GradsPlan plan;
-  {
-    std::lock_guard<std::mutex> lock(h->mu);
-    plan = grads_plan(h, M, F, K, dX != nullptr, dWg != nullptr, true);
-    if (plan.split > 1 && workspace_bytes < base_bytes + grads_partial_bytes(M, K, plan.split))
-      plan = grads_plan(h, M, F, K, dX != nullptr, dWg != nullptr, false);
-  }
   const int width = plan.width;
   FfnParams p{};
   p.seg_kb = (F + kBlockK - 1) / kBlockK;

@@ -6,6 +6,9 @@ Bounds are relative and counted in steps of fp32 (2^-23, `ULP`), plus one
 rounding of the result to bf16 (plain.BF16).  A weight matrix of one non-zero
 column makes a gate of every chosen value without any rounding."""
 import math
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 
@@ -19,6 +22,7 @@ import ffn_plain as plain  # noqa: E402
 
 BF = torch.bfloat16
 ULP = 2.0 ** -23
+ROOT = Path(__file__).resolve().parent.parent
 
 
 def _gates():
@@ -226,3 +230,46 @@ def test_input_gradient_on_its_own(gpu_handle, M, F, K):
     assert torch.equal(gpu_handle.gated_backward(dh, x, wg, wu, g, u, weight_grad=False)[0], dx)
     parts = gpu_handle.gated_backward(dh, x, wg, wu, g, u, input_grad=False)
     assert torch.equal(parts[1], dwg) and torch.equal(parts[2], dwu)
+
+
+_FIRST_CALLS = """
+import sys
+import torch
+import b200_gemm_b200 as b200
+
+BF = torch.bfloat16
+g = torch.Generator("cuda").manual_seed(0)
+r = lambda m, n: torch.randn(m, n, generator=g, device="cuda").to(BF)
+h = b200.Gemm(0)
+x, w, v, dh, gu = r(300, 256), r(520, 256), r(520, 256), r(300, 520), r(300, 520)
+codes = torch.randint(0, 256, (520, 128), generator=g, device="cuda", dtype=torch.uint8)
+scales = torch.full((2, 520), 0.01, dtype=BF, device="cuda")
+calls = [
+    lambda: h.gated(x[:2], w, v),
+    lambda: h.gated(x, w, v, save=True)[0],
+    lambda: torch.cat(h.gated_backward(dh, x, w, v, gu, gu)),
+    lambda: torch.cat(h.gated_backward(dh[:17], x[:17], w, v, gu[:17], gu[:17])),
+    lambda: h.w4_nt(x[:2], codes, scales),
+    lambda: h.w4_nt(x[:40], codes, scales),
+    lambda: h.w4_gated(x[:12], codes, scales, codes, scales),
+    lambda: h.w4_quantize(w)[1],
+    lambda: h.w4_dequantize(codes, scales),
+]
+for i in [int(a) for a in sys.argv[1:]]:
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = calls[i]()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, calls[i]()), i
+    del graph
+assert h.last_device_status()[0] == 0
+"""
+
+
+@pytest.mark.parametrize("order", ["012345678", "876543210", "360"])
+def test_first_calls_are_captured(order):
+    """The first call of every kind in a process, made while a stream is
+    captured: it loads its kernels and is replayed like any other."""
+    run = subprocess.run([sys.executable, "-c", _FIRST_CALLS, *order], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0, run.stderr[-2000:]
