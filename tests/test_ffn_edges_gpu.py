@@ -273,3 +273,29 @@ def test_first_calls_are_captured(order):
     captured: it loads its kernels and is replayed like any other."""
     run = subprocess.run([sys.executable, "-c", _FIRST_CALLS, *order], cwd=ROOT, capture_output=True, text=True, timeout=300)
     assert run.returncode == 0, run.stderr[-2000:]
+
+
+@pytest.mark.parametrize("group", [32, 64, 128, 256])
+@pytest.mark.parametrize("M", [1, 12, 20, 70])
+def test_scales_of_both_signs(gpu_handle, M, group):
+    """Scales of either sign and exactly zero; the bound is that of the sums of
+    (q - 8) x over at most 128 k's: 8 steps of 16 products, each of 17 terms
+    truncated to 2^-22 of the largest, at most 8 sum|x|; scaled and added up
+    over K / 32 such sums."""
+    N, K = 210, 1280
+    x = plain.rows(M, K, 1)
+    codes, scales = plain.w4_random(N, K, group, 2)
+    gen = torch.Generator("cuda").manual_seed(3)
+    scales = scales * (torch.randint(0, 3, scales.shape, generator=gen, device="cuda") - 1).to(BF)
+    w, x64 = plain.w4_values(codes, scales), x.double()
+    s = scales.double().abs().t().repeat_interleave(group, dim=1)
+    err = 8 * 17 * 8 * 2.0 ** -22 * (x64.abs() @ s.t()) + (K / 32 + 16) * ULP * (x64.abs() @ w.abs().t())
+    plain.close(gpu_handle.w4_nt(x, codes, scales, out_dtype=torch.float32), x64 @ w.t(), err, plain.F32)
+    assert torch.equal(gpu_handle.w4_dequantize(codes, scales), w.to(BF))
+
+
+def test_dequantize_among_subnormals(gpu_handle):
+    """Scales down to the smallest bf16 subnormal: the scaled codes as they are."""
+    codes, _ = plain.w4_random(64, 256, 32, 1)
+    scales = (2.0 ** torch.linspace(-133, -120, 8 * 64, device="cuda").round()).reshape(8, 64).to(BF)
+    assert torch.equal(gpu_handle.w4_dequantize(codes, scales), plain.w4_values(codes, scales).to(BF))
