@@ -1,8 +1,9 @@
 // Host side of the feed-forward entry points of include/b200gemm.h: argument
 // checks, plans and launches of the kernels in ffn_sm100.cuh,
-// gated_decode_sm100.cuh and w4_sm100.cuh.  Part of b200gemm.cu's translation unit (it uses the
-// handle and the helpers there).  Nothing here allocates, builds a table or
-// waits, so every call can be captured into a CUDA graph from the first one.
+// gated_decode_sm100.cuh, w4_sm100.cuh and w4_mma_sm100.cuh.  Part of
+// b200gemm.cu's translation unit (it uses the handle and the helpers there).
+// Nothing here allocates, builds a table or waits, so every call can be captured
+// into a CUDA graph from the first one.
 #pragma once
 
 namespace b200gemm {
@@ -412,6 +413,17 @@ int run_gated_decode(b200gemm_t h, const void* Wg, const void* Wu, long long ldw
 // the splits of K over clusters of 1, 2, 4 and 8 CTAs, the one with the least
 // estimated time.  Rows are divided evenly over the clusters that fit at once
 // (a second wave only where a CTA's registers and ring cannot hold its share).
+// The estimate's unit, a warp's 16 x 64 weights times a tile of X, is some 0.2
+// us; a CTA costs 6 of them besides, 10 in a cluster.  Measured with K in 1, 2,
+// 4 and 8 ranges (us, * the choice; groups of 128 unless said otherwise):
+//   1 x 4096 x 14336          18.6  13.5  11.6* 18.7
+//   1 x 8192 x 8192           14.0  12.5* 16.8  21.6
+//   1 x 28672 x 8192          27.8* 34.4  42.5  64.6
+//   1 x 14336 x 4096          11.6  11.5* 16.1
+//   8 x 2048 x 8192 (64)      11.4   7.7   6.7*  7.3
+//   12 x 1024 x 8192 (32)     14.1   9.3   6.8*  7.0
+//   16 x 4096 x 8192          12.9  11.2  11.1* 17.5
+//   gated 5 x 14331 x 4096 (32) 18.7* 25.5  34.4
 struct W4Plan {
   int rows = 0, mt = 0, split = 1;
   long long waves = 1;
@@ -462,8 +474,13 @@ cudaError_t launch_w4(const W4Launch& l, const W4NtParams& p) {
 // The same for the tcgen05 kernel, whose CTA holds 128 rows of W or 256 (128
 // of Wg and of Wu); plan.mt = 128-row blocks.  A stage of 256 k's takes some
 // 1200 cycles with one block and 2100 with two, however few of their rows are
-// there (the MMAs' time; DRAM's share of 256 rows is 1400), and a CTA some 6000
-// besides, 700 more in a cluster.
+// there (a fit of whole calls; DRAM's share of 256 rows is 1400), and a CTA
+// some 6000 besides, 700 more in a cluster.  Measured with K in 1, 2, 4 and 8
+// ranges (us, * the choice; groups of 128 unless said otherwise):
+//   32 x 8192 x 8192 (64)     26.4  17.9  18.7* 37.0
+//   32 x 4096 x 14336         35.9  22.5  15.0* 29.3
+//   32 x 1024 x 8192          22.2  14.9  10.2   7.9*
+//   64 x 28416 x 8192         55.5* 66.9  78.8 107.3
 W4Plan w4_mma_plan(const b200gemm_handle* h, int N, int token_blocks, int num_stages, bool gated) {
   W4Plan best;
   double best_cost = 1e300;
@@ -614,10 +631,11 @@ int run_ffn(b200gemm_t h, const FfnMaps& maps, FfnParams p, cudaStream_t stream,
   return launch_ffn<Cfg>(clusters, stream, maps, p, overlap) == cudaSuccess ? B200GEMM_OK : B200GEMM_ERR_CUDA;
 }
 
+// Blocks of 2048 columns, and enough rows of them for 32 blocks per SM.
 template <int ACT>
-void launch_gated_grad(const GatedGradParams& p, cudaStream_t stream) {
+void launch_gated_grad(const GatedGradParams& p, int sm_count, cudaStream_t stream) {
   const int bx = (p.F + 2047) / 2048;
-  int by = (148 * 32 + bx - 1) / bx;
+  int by = (sm_count * 32 + bx - 1) / bx;
   if (by > p.M) by = p.M;
   gated_grad_kernel<ACT><<<dim3(static_cast<unsigned>(bx), static_cast<unsigned>(by)), 256, 0, stream>>>(p);
 }
@@ -776,11 +794,11 @@ extern "C" int b200gemm_bf16_gated_backward(b200gemm_t h, int M, int F, int K, c
   gp.du = gp.dg + static_cast<long long>(M) * f8;
   gp.ldo = f8;
   switch (activation) {
-    case B200GEMM_ACT_RELU: launch_gated_grad<kActRelu>(gp, stream); break;
-    case B200GEMM_ACT_GELU: launch_gated_grad<kActGelu>(gp, stream); break;
-    case B200GEMM_ACT_GELU_TANH: launch_gated_grad<kActGeluTanh>(gp, stream); break;
-    case B200GEMM_ACT_SILU: launch_gated_grad<kActSilu>(gp, stream); break;
-    default: launch_gated_grad<kActNone>(gp, stream); break;
+    case B200GEMM_ACT_RELU: launch_gated_grad<kActRelu>(gp, h->sm_count, stream); break;
+    case B200GEMM_ACT_GELU: launch_gated_grad<kActGelu>(gp, h->sm_count, stream); break;
+    case B200GEMM_ACT_GELU_TANH: launch_gated_grad<kActGeluTanh>(gp, h->sm_count, stream); break;
+    case B200GEMM_ACT_SILU: launch_gated_grad<kActSilu>(gp, h->sm_count, stream); break;
+    default: launch_gated_grad<kActNone>(gp, h->sm_count, stream); break;
   }
   if (cudaGetLastError() != cudaSuccess) return B200GEMM_ERR_CUDA;
 

@@ -26,12 +26,13 @@
 //
 // Bound by the tensor cores where M is large: their pipe is active for 83% of
 // the cycles forward (2048 x 14336 x 4096, 256-wide tiles) and 90% backward.
-// Measured: forward with G and U kept, 8192 x 14336 x 4096, 1.28 ms = 1.51
-// PFLOP/s, gradients 2.55 ms = 1.51 PFLOP/s, near the power limit and within 2%
-// of library products of the same operations.  Smaller sizes lose to whole
-// tiles and waves and to the first fetches and last epilogue, which nothing
-// overlaps: 777 x 5120 x 2048 (a quarter of the tiles' rows are padding) takes
-// 41 us, twice its operations' time.
+// Measured, 8192 x 14336 x 4096: forward with G and U kept 1.27 ms = 1.52
+// PFLOP/s, gradients 2.55 ms = 1.51 PFLOP/s for a few calls after a pause; 1.49
+// and 2.99 ms = 1.29 PFLOP/s in a loop of seconds, under the power cap.  Library
+// products of the same operations, without the element-wise work: 1.24 and 2.49,
+// 1.44 and 2.91 ms.  Smaller sizes lose to whole tiles and waves and to the first
+// fetches and last epilogue, which nothing overlaps: 777 x 5120 x 2048 (a quarter
+// of the tiles' rows are padding) takes 40 us, twice its operations' time.
 #pragma once
 
 #include <cstdint>
@@ -222,11 +223,13 @@ __device__ __forceinline__ float normal_cdf(float x, float& e) {
   return x < 0.0f ? tail : 1.0f - tail;
 }
 
-// act(x) for bf16 results: e^x and the reciprocal are the fast forms, whose
-// relative error (2^-21) is far below bf16's 2^-9.  The tanh form of GELU
-// goes through the logistic function, 0.5 (1 + tanh z) = 1 / (1 + e^-2z),
-// which keeps its relative accuracy where tanh is near -1.  A NaN stays one
-// under each of them.
+// act(x) for bf16 results: e^x and the reciprocal are the fast forms.  __expf(a)
+// is off by up to 2 + 1.173 |a| steps of 2^-23 and what a's own roundings make
+// of it, the reciprocal by one step: relative errors below 2^-16 for |a| up to
+// 20 and below 2^-14 as far as e^a is finite, where bf16 rounds by 2^-8.  The
+// tanh form of GELU goes through the logistic function, 0.5 (1 + tanh z) = 1 /
+// (1 + e^-2z), which keeps its relative accuracy where tanh is near -1.  A NaN
+// stays one under each of them.
 template <int ACT>
 __device__ __forceinline__ float ffn_act(float x) {
   if constexpr (ACT == kActRelu) return ptx::max_nan(x, 0.0f);
@@ -659,8 +662,9 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1) __cluster_dims__(2, 1, 1)
 }
 
 // dG and dU from dH, G and U, element by element: 6 bytes read and 4 written
-// per element, so DRAM-bound (2048 x 14336: 43 us, 6.9 TB/s); a thread takes 8
-// columns (16 bytes of each).
+// per element, so DRAM-bound (2048 x 14336: 43 us, in which 241 MB reach DRAM,
+// 5.7 TB/s; 52 MB of the results are still in L2, where the products read them);
+// a thread takes 8 columns (16 bytes of each).
 // They are rounded to bf16 once, to be operands of the tensor cores.  Rows of
 // the results are ldo elements (F rounded up to 8) and their padding columns
 // are set to 0: the products below sum over them.
@@ -699,7 +703,7 @@ __global__ void __launch_bounds__(256) gated_grad_kernel(const GatedGradParams p
 
 // dX from its K ranges' partial sums, added in range order and rounded once;
 // a thread takes 8 columns.  500 x 1000 from 4 ranges: 7 us by itself, mostly
-// its launch, which overlaps the products' last tiles.
+// its launch and first loads; it starts when the products have ended.
 __global__ void __launch_bounds__(256) dx_sum_kernel(const float* partials, int split, int M, int N, uint16_t* dx,
                                                      long long ld) {
   const int groups = N / 8;

@@ -16,12 +16,17 @@
 // warps, whose lanes are rows of W, multiply it by the group's scale in fp32
 // and add it to the row's sums in registers.  No weight is rounded.
 //
-// What bounds it: the MMAs, at some 60 cycles for 128 x 32 x 16 (a quarter of
-// the rate of wide ones), and next to them the expansion and its stores to
-// TMEM.  28416 x 4096, groups of 128, 32 rows: 26 us (mma.sync: 37), 58 MB of
+// What bounds it is not taken apart.  Of 28672 x 8192, 32 rows, the tensor pipe
+// is active 21% of the time, the issue slots 58%, DRAM 31%.  By w4_mma_plan's fit
+// a step of 128 x 32 x 16 takes some 60 cycles with all that goes with it, a
+// quarter of the rate of wide MMAs; what sets that pace (A from TMEM, sums that
+// wait for one another, the hand-overs between warps) was not timed alone.
+// 28416 x 4096, groups of 128, 32 rows: 26 us (mma.sync: 37), 58 MB of
 // weights at 2.3 TB/s; 8192 x 8192: 18 us (25); gated 14336 x 4096: 24 us (53).
 // 64 rows in one CTA take 32, 21 and 29 us (in two CTAs of 32: 51, 27 and 45):
-// the MMAs take little more, the epilogue twice as long.
+// the MMAs take little more, the epilogue twice as long.  Its 64 sums a thread
+// do not fit the 96 registers that all warps share: 48 to 108 bytes are spilled
+// with two blocks of rows, but for the gated block in groups of 128 and more.
 //
 // Warps: 0 .. 4H-1   epilogue: block w / 4 of 128 rows, TMEM lanes 32 (w % 4) ..
 //        16 or 8     expansion, two groups of eight for the steps in turn, or
@@ -386,7 +391,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
           __syncwarp();
           if (lane == 0) ptx::mbar_arrive_cta(tempty0 + 8 * set);
         }
-        // An infinite scale counts as NaN, which is what it makes of a code of 8.
+        // An infinite scale counts as NaN, as it makes one of a code of 8.
         const uint32_t bits = sc[j * Cfg::kSetGroups + c * 16 / TOK];
         const float s = __uint_as_float(((bits & 0x7FFFu) == 0x7F80u ? 0x7FC0u : bits) << 16);
 #pragma unroll

@@ -267,8 +267,8 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
     for (int e = 0; e < kSets; ++e)
 #pragma unroll
       for (int r = 0; r < kHold; ++r) {
-        // An infinite scale counts as NaN, which is what it makes of a code of
-        // 0: the sums below are not exactly 0 there.
+        // An infinite scale counts as NaN, whatever its group's codes are: of
+        // a code of 8 it makes one, and the group's sum does not tell.
         const uint32_t s = next_sc[e][r];
         sc[e][r] = __uint_as_float((s & 0x7F80u) == 0x7F80u ? 0x7FC00000u : s << 16);
       }

@@ -6,7 +6,9 @@ Activations are 2-D bf16 CUDA tensors whose rows may be slices of wider ones
 (stride(1) == 1, row stride a multiple of 8 elements, 16-byte aligned); all
 tensors of a call live on the handle's device.  A call runs on `stream` (a
 torch stream or a raw pointer; default: the current stream of the handle's
-device); tensors that it allocates are allocated for that stream."""
+device); tensors that it allocates are allocated for that stream.  Autograd
+records none of these calls, whatever their inputs require: `gated_backward` is
+called by hand, or from a torch.autograd.Function of the caller's."""
 from __future__ import annotations
 
 from . import _lib

@@ -362,7 +362,8 @@ int b200gemm_bf16_gated_backward(b200gemm_t handle, int M, int F, int K, const v
  * aligned), per group of a row s = bf16(max|w| / 7), q = clamp(rint(w / s),
  * -8, 7) + 8 (rint: ties to even; q = 8 where s is 0).  A group that holds a
  * NaN or an infinity comes back as NaN.
- * b200gemm_w4_dequantize: W = bf16(s * (q - 8)). */
+ * b200gemm_w4_dequantize: W = bf16(s * (q - 8)).
+ * Both take N up to 2097120 (B200GEMM_ERR_TOO_LARGE beyond). */
 int b200gemm_w4_quantize(b200gemm_t handle, int N, int K, const void* W, long long ldw, int group,
                          void* codes, void* scales, void* stream);
 int b200gemm_w4_dequantize(b200gemm_t handle, int N, int K, const void* codes, const void* scales,
@@ -374,13 +375,14 @@ int b200gemm_w4_dequantize(b200gemm_t handle, int N, int K, const void* codes, c
  * unscaled in fp32 and the sum is scaled in fp32.  A scale that is a NaN or an
  * infinity makes its weight row's results NaN.  Made for a few rows (the
  * weights are read once for up to 64 rows of A; b200gemm_bf16_nt with dequantized
- * ones is faster from about 65 rows on); any M works. */
+ * ones is faster from about 65 rows on); any M works, and any N up to 5000000
+ * (well beyond, B200GEMM_ERR_TOO_LARGE). */
 int b200gemm_w4_nt(b200gemm_t handle, int M, int N, int K, const void* A, long long lda,
                    const void* codes, const void* scales, int group, void* C, long long ldc,
                    int out_type, void* stream);
 
 /* H = act(X Wg^T) * (X Wu^T) for 4-bit Wg and Wu [F,K] of one group size, H
- * bf16 [M,F], ldh >= F; X as A above. */
+ * bf16 [M,F], ldh >= F; X as A above, F as N. */
 int b200gemm_w4_gated(b200gemm_t handle, int M, int F, int K, const void* X, long long ldx,
                       const void* gate_codes, const void* gate_scales, const void* up_codes,
                       const void* up_scales, int group, int activation, void* H, long long ldh,
